@@ -1,0 +1,382 @@
+"""The low-bit operators of a decode round: the full KV cache in 8 bits and the weights in 4.
+
+A case is a dict of plain values; ``kind`` names the operator:
+
+* ``append``: ``tokens`` rows per sequence go into one layer of an 8-bit paged cache that holds ``ctx`` rows
+  (``PagedKVCache.append_layer``). Returns the values that the touched blocks then stand for.
+* ``attn``: the same append, then the causal attention of the new rows over the cache
+  (``PagedKVCache.append_attend``): decode (one row), verify (a few) or a prompt (many).
+* ``quantize``: rows to microscaled 4-bit floating point (``ops.mx4_quantize``) and the values they stand for.
+* ``linear``: ``x . W^T`` with W in microscaled 4 bits (``ops.gemm_mx4``); ``x`` says what x is: bf16, f32 (rounded to
+  bf16 as it is read), or mx4, where x is quantized to 4 bits within the pass and both operands are 4-bit.
+
+The 8-bit cache. Rows are held to bf16. Of each block of ``block`` tokens and KV head, K and V apart, a = max |x|; e is
+the least integer with a <= 448 * 2^e (0 where a = 0, at least -126) and a value is e4m3(x * 2^-e) * 2^e. A query at
+position p reads the blocks before its own in 8 bits and its own block's rows up to p in bf16.
+
+The 4-bit format (OCP MX, MXFP4): of each 32 values along k, e = floor(log2 max |x|) - 2 (0 where all are 0, at least
+-126), and a value is e2m1(x * 2^-e) * 2^e, saturating at 6 * 2^e. Both round to nearest even.
+"""
+
+import math
+import os
+import sys
+
+import torch
+
+own = False
+
+sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "draft-kv_amd"))
+
+DEV = "cuda"
+F32, F64, BF16, F8 = torch.float32, torch.float64, torch.bfloat16, torch.float8_e4m3fn
+# query heads, KV heads, head width of the models that the framework names
+HEADS = {"llama3_8b": (32, 8, 128), "smollm2": (9, 3, 64), "distilgpt2": (12, 12, 64)}
+# rows and columns of their weights W[n, k]
+WEIGHTS = {"llama3_8b": [(6144, 4096), (4096, 4096), (28672, 4096), (4096, 14336)],
+           "smollm2": [(960, 576), (576, 576), (576, 1536), (49152, 576)],
+           "distilgpt2": [(2304, 768), (768, 768), (50257, 768)]}
+
+
+def listed():
+    return [
+        # one decode step's rows of a batch of 32, into 16-token blocks
+        dict(name="append_decode_b32", kind="append", model="llama3_8b", block=16, batch=32, tokens=1, ctx=4095, kv="f32"),
+        # a 4096-token prompt's rows
+        dict(name="append_prompt", kind="append", model="llama3_8b", block=16, batch=1, tokens=4096, ctx=0, kv="f32"),
+        # one decode step of a small model at batch 1, an odd context: latency counts
+        dict(name="attn_decode_b1", kind="attn", model="smollm2", block=16, batch=1, tokens=1, ctx=4001, q="f32"),
+        # plain decoding of a batch over a long context
+        dict(name="attn_decode_b32_32k", kind="attn", model="llama3_8b", block=16, batch=32, tokens=1, ctx=32700, q="bf16"),
+        # the benchmark's verify pass: batch 32, context 32k, gamma 4
+        dict(name="attn_verify_b32_32k", kind="attn", model="llama3_8b", block=16, batch=32, tokens=5, ctx=32763, q="f32"),
+        # the attention of a 4096-token prompt, larger blocks
+        dict(name="attn_prompt", kind="attn", model="llama3_8b", block=64, batch=1, tokens=4096, ctx=0, q="bf16"),
+        # the weight of a SwiGLU MLP's gate and up projections, laid out at load time
+        dict(name="quantize_weight", kind="quantize", rows=28672, width=4096, dtype="bf16"),
+        # a decode step's activations
+        dict(name="quantize_rows", kind="quantize", rows=32, width=4096, dtype="f32"),
+        # one token of a small model: the smallest product
+        dict(name="linear_m1", kind="linear", model="smollm2", rows=1, n=960, k=576, x="f32", out="bf16", swiglu=False),
+        # the verify block of a batch of 32 with gamma 4 through the gate and up projections
+        dict(name="linear_verify_swiglu", kind="linear", model="llama3_8b", rows=160, n=28672, k=4096, x="bf16", out="bf16", swiglu=True),
+        # the down projection of a batch of 32, one token each, both operands in 4 bits
+        dict(name="linear_mx4_b32", kind="linear", model="llama3_8b", rows=32, n=4096, k=14336, x="mx4", out="f32", swiglu=False),
+        # a prompt's rows through the gate and up projections, both operands in 4 bits
+        dict(name="linear_mx4_prompt", kind="linear", model="llama3_8b", rows=4096, n=28672, k=4096, x="mx4", out="bf16", swiglu=False),
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    kind = rng.choice(["append", "attn", "attn", "attn", "quantize", "linear", "linear", "linear"])
+    if kind in ("append", "attn"):
+        c = dict(kind=kind, model=rng.choice(["llama3_8b", "llama3_8b", "smollm2", "distilgpt2"]), block=rng.choice([16, 16, 32, 64, 128]))
+        c[dict(append="kv", attn="q")[kind]] = rng.choice(["f32", "bf16"])
+        if rng.random() < 0.4:   # a prompt, or a further part of one
+            return dict(c, batch=rng.choice([1, 1, 2]), tokens=_log(rng, 20, 2000), ctx=rng.choice([0, 0, rng.randrange(1, 2000)]))
+        batch = _log(rng, 1, 32)
+        return dict(c, batch=batch, tokens=rng.choice([1, 1, 2, 3, 5, 9, 17]), ctx=_log(rng, 16, min(32000, 800000 // batch)))
+    if kind == "quantize":
+        return dict(kind=kind, rows=_log(rng, 1, 20000), width=rng.choice([64, 100, 576, 768, 1000, 4096, 5000]), dtype=rng.choice(["f32", "bf16"]))
+    model = rng.choice(["llama3_8b", "llama3_8b", "smollm2", "distilgpt2"])
+    n, k = rng.choice(WEIGHTS[model])
+    x = rng.choice(["bf16", "f32", "mx4"])
+    rows = _log(rng, 1, 4000 if n * k < 60e6 else 2000)
+    return dict(kind=kind, model=model, rows=rows, n=n, k=k, x=x, out=rng.choice(["bf16", "f32"]), swiglu=False)
+
+
+# ---------------------------------------------------------------- inputs
+_TYPES = {"f32": F32, "bf16": BF16}
+
+
+def _normal(g, *shape, std=1.0, dtype=F32):
+    return torch.empty(shape, dtype=dtype, device=DEV).normal_(0.0, std, generator=g)
+
+
+def _kv(g, b, n, heads, d, dtype):
+    """K and V rows [b, n, heads, d]: normal, K with the uneven channel gains that trained models show."""
+    gain = torch.exp(0.4 * _normal(g, heads, d)).to(dtype)
+    return _normal(g, b, n, heads, d, dtype=dtype).mul_(gain), _normal(g, b, n, heads, d, dtype=dtype)
+
+
+def _inputs(case, seed):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed)
+    s = {"case": case}
+    if case["kind"] == "quantize":
+        # rows of different size, as activations and weights have
+        gain = torch.exp(_normal(g, case["rows"], 1))
+        s["x"] = (_normal(g, case["rows"], case["width"]) * gain).to(_TYPES[case["dtype"]])
+    elif case["kind"] == "linear":
+        s["w"] = _normal(g, case["n"], case["k"], std=0.02, dtype=BF16)
+        s["x"] = _normal(g, case["rows"], case["k"], dtype=BF16 if case["x"] == "bf16" else F32)
+    else:
+        hq, h, d = HEADS[case["model"]]
+        b, t = case["batch"], case["tokens"]
+        s["ck"], s["cv"] = _kv(g, b, case["ctx"], h, d, BF16)
+        s["k"], s["v"] = _kv(g, b, t, h, d, _TYPES[case.get("kv", "f32")])
+        if case["kind"] == "attn":
+            s["q"] = _normal(g, b, t, hq, d, dtype=_TYPES[case["q"]])
+    return s
+
+
+def prepare(case, seed):
+    s = _inputs(case, seed)
+    if case["kind"] == "linear":
+        w = s.pop("w")
+        if own:
+            from draftkv import ops
+            s["w"] = ops.mx4_quantize(w)
+        else:   # codes of two values a byte, and a scale exponent for each 32
+            e, code = _mx4(w.float())
+            code = (_E2M1_INDEX(code.abs()) + 8 * (code < 0)).to(torch.uint8).view(case["n"], case["k"])
+            s["w"] = code[:, 0::2] | (code[:, 1::2] << 4)
+            s["e"] = e.to(torch.int8)
+    elif case["kind"] != "quantize":
+        b, t, ctx, blk = case["batch"], case["tokens"], case["ctx"], case["block"]
+        ck, cv = s.pop("ck"), s.pop("cv")
+        if own:
+            from draftkv.paged import PagedKVCache
+            nb = -(-(ctx + t) // blk)
+            c = PagedKVCache(1, ck.shape[2], ck.shape[3], blk, nb, F8, batch=b, max_tokens=nb * blk, device=DEV)
+            c.reserve([ctx + t] * b)
+            if ctx:
+                c.append_layer(0, ck, cv, torch.zeros(b, dtype=torch.int32, device=DEV))
+            s["cache"] = c
+            s["start"] = torch.full((b,), ctx, dtype=torch.int32, device=DEV)
+            s["first"] = torch.full((b,), ctx // blk * blk, dtype=torch.int32, device=DEV)
+            s["end"] = torch.full((b,), ctx + t, dtype=torch.int32, device=DEV)
+        else:
+            n = ctx // blk * blk
+            s["kc"], s["ke"] = _seal(ck[:, :n], blk)
+            s["vc"], s["ve"] = _seal(cv[:, :n], blk)
+            s["kt"], s["vt"] = ck[:, n:].clone(), cv[:, n:].clone()
+    return s
+
+
+# ---------------------------------------------------------------- plain forms
+def _pow2(e):
+    """2^e of whole numbers in -149 .. 127, exactly."""
+    return torch.ldexp(torch.ones_like(e, dtype=F32), e)
+
+
+def _seal(x, blk):
+    """bf16 rows [b, n, heads, d], n whole blocks: e4m3 codes [b, heads, n / blk, blk, d] and exponents [b, heads, n / blk]."""
+    b, n, h, d = x.shape
+    x = x.view(b, n // blk, blk, h, d).permute(0, 3, 1, 2, 4).float()
+    m, ex = torch.frexp(x.abs().amax(dim=(3, 4)))
+    e = torch.where(m <= 0.875, ex - 9, ex - 8)
+    e = torch.where(m == 0, torch.zeros_like(e), e).clamp(min=-126)
+    return (x * _pow2(-e)[..., None, None]).to(F8), e.to(torch.int8)
+
+
+def _open(codes, e):
+    """The values of _seal's codes as [b, heads, n, d]."""
+    b, h, nb, blk, d = codes.shape
+    return (codes.float() * _pow2(e.int())[..., None, None]).view(b, h, nb * blk, d)
+
+
+def _append(s):
+    """The state after the new rows: codes and exponents of all sealed blocks, and the bf16 rows from the block that
+    the first new row lies in."""
+    blk = s["case"]["block"]
+    kt, vt = torch.cat([s["kt"], s["k"].to(BF16)], 1), torch.cat([s["vt"], s["v"].to(BF16)], 1)
+    n = kt.shape[1] // blk * blk
+    kc, ke = _seal(kt[:, :n], blk)
+    vc, ve = _seal(vt[:, :n], blk)
+    return (kc, ke), (vc, ve), kt, vt
+
+
+def _attend(s):
+    case = s["case"]
+    q = s["q"].float()
+    b, t, hq, d = q.shape
+    (kc, ke), (vc, ve), kt, vt = _append(s)
+    kc, ke = torch.cat([s["kc"], kc], 2), torch.cat([s["ke"], ke], 2)
+    vc, ve = torch.cat([s["vc"], vc], 2), torch.cat([s["ve"], ve], 2)
+    h, blk, ctx = kt.shape[2], case["block"], case["ctx"]
+    g = hq // h
+    k8, v8 = _open(kc, ke), _open(vc, ve)                                  # [b, h, n8, d]
+    kt, vt = kt.permute(0, 2, 1, 3).float(), vt.permute(0, 2, 1, 3).float()   # [b, h, nt, d]
+    n8, nt, t0 = k8.shape[2], kt.shape[2], ctx // blk * blk
+    q = q.view(b, t, h, g, d).permute(0, 2, 3, 1, 4).reshape(b, h, g * t, d) / math.sqrt(d)
+    p = (ctx + torch.arange(t, device=DEV)).repeat(g)[:, None]             # the rows' positions
+    lim = p // blk * blk
+    j8, jt = torch.arange(n8, device=DEV)[None], (t0 + torch.arange(nt, device=DEV))[None]
+    s8 = torch.where(j8 < lim, q @ k8.transpose(2, 3), -math.inf)
+    st = torch.where((jt >= lim) & (jt <= p), q @ kt.transpose(2, 3), -math.inf)
+    m = st.amax(-1, keepdim=True)                                          # a row sees its own key at least
+    m = torch.maximum(m, s8.amax(-1, keepdim=True)) if n8 else m
+    s8, st = torch.exp(s8 - m), torch.exp(st - m)
+    o = (s8 @ v8 + st @ vt) / (s8.sum(-1, keepdim=True) + st.sum(-1, keepdim=True))
+    return o.view(b, h, g, t, d).permute(0, 3, 1, 2, 4).reshape(b, t, hq, d).to(s["q"].dtype)
+
+
+def _E2M1_INDEX(a):
+    """0, .5, 1, 1.5, 2, 3, 4, 6 -> 0 .. 7."""
+    return torch.where(a < 2, 2 * a, torch.where(a < 4, a + 2, a / 2 + 4))
+
+
+def _mx4(x):
+    """float32 rows [r, k]: scale exponents [r, ceil(k / 32)] and the e2m1 values [r, ceil(k / 32), 32]."""
+    r, k = x.shape
+    x = torch.nn.functional.pad(x, (0, -k % 32)).view(r, -1, 32)
+    m, ex = torch.frexp(x.abs().amax(-1))
+    e = torch.where(m == 0, torch.zeros_like(ex), ex - 3).clamp(min=-126)
+    x = x * _pow2(-e)[..., None]
+    step = torch.where(x.abs() < 2, 0.5, torch.where(x.abs() < 4, 1.0, 2.0))
+    return e, (torch.round(x / step) * step).clamp(-6, 6)
+
+
+def _values(e, code, k):
+    r = e.shape[0]
+    return (code * _pow2(e)[..., None]).view(r, -1)[:, :k]
+
+
+def _weight(s):
+    n, k = s["case"]["n"], s["case"]["k"]
+    c = torch.stack([s["w"] & 15, s["w"] >> 4], -1).view(n, k // 32, 32)
+    table = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6, 0, -0.5, -1, -1.5, -2, -3, -4, -6], dtype=F32, device=DEV)
+    return _values(s["e"].int(), table[c.int()], k)
+
+
+def _silu_mul(y):
+    g, u = y[:, 0::2], y[:, 1::2]
+    return g / (1 + torch.exp(-g)) * u
+
+
+def run(s):
+    case = s["case"]
+    kind = case["kind"]
+    if own:
+        return _run_own(s, case, kind)
+    if kind == "append":
+        (kc, ke), (vc, ve), kt, vt = _append(s)
+        n = kc.shape[2] * kc.shape[3]
+        return [torch.cat([_open(c, e).permute(0, 2, 1, 3), rows[:, n:].float()], 1) for c, e, rows in ((kc, ke, kt), (vc, ve, vt))]
+    if kind == "attn":
+        return _attend(s)
+    if kind == "quantize":
+        return _values(*_mx4(s["x"].float()), case["width"]).contiguous()
+    x = s["x"].float() if case["x"] != "f32" else s["x"].to(BF16).float()
+    if case["x"] == "mx4":
+        x = _values(*_mx4(x), case["k"])
+    y = x @ _weight(s).t()
+    return (_silu_mul(y) if case["swiglu"] else y).to(_TYPES[case["out"]])
+
+
+def _run_own(s, case, kind):
+    from draftkv import ops
+    if kind == "append":
+        s["cache"].append_layer(0, s["k"], s["v"], s["start"])
+        return list(s["cache"].read_rows(0, s["first"], s["end"], case["ctx"] % case["block"] + case["tokens"]))
+    if kind == "attn":
+        return s["cache"].append_attend(0, s["q"], s["k"], s["v"], s["start"], case["ctx"] + case["tokens"])
+    if kind == "quantize":
+        return ops.mx4_quantize(s["x"], values=True)[1]
+    x = ops.mx4_quantize(s["x"]) if case["x"] == "mx4" else s["x"]
+    return ops.gemm_mx4(x, s["w"], out_dtype=_TYPES[case["out"]], swiglu=case["swiglu"])
+
+
+# ---------------------------------------------------------------- work
+def work(case):
+    kind = case["kind"]
+    if kind == "quantize":
+        n = case["rows"] * case["width"]
+        return {"bytes": n * (4 if case["dtype"] == "f32" else 2) + n * (4 + 0.53125), "flops": 0}
+    if kind == "linear":
+        m, n, k = case["rows"], case["n"], case["k"]
+        return {"bytes": n * k * 0.53125 + m * k * (2 if case["x"] == "bf16" else 4)
+                + m * n * (2 if case["out"] == "bf16" else 4) / (2 if case["swiglu"] else 1), "flops": 2 * m * n * k}
+    hq, h, d = HEADS[case["model"]]
+    b, t, ctx, blk = case["batch"], case["tokens"], case["ctx"], case["block"]
+    fresh = 2 * b * t * h * d           # K and V values of the new rows
+    if kind == "append":
+        # the new rows read and held; the touched rows returned
+        return {"bytes": fresh * (4 if case["kv"] == "f32" else 2) + fresh + 2 * b * (t + ctx % blk) * h * d * 4, "flops": 0}
+    keys = t * ctx + t * (t + 1) // 2   # (row, key) pairs per query head
+    return {"bytes": fresh * 5 + 2 * b * ctx * h * (d + 1 / blk) + 2 * b * t * hq * d * (4 if case["q"] == "f32" else 2),
+            "flops": 4 * b * hq * d * keys}
+
+
+# ---------------------------------------------------------------- the definitions in 64 bits
+def _grid(x, a, lowest, bits, top):
+    """x rounded to nearest even on the grid of a floating type of `bits` mantissa bits and least exponent `lowest`,
+    scaled so that a (the block's largest magnitude) is at most `top` times the scale."""
+    y = x / a
+    mag = y.abs()
+    ex = torch.floor(torch.log2(torch.where(mag > 0, mag, torch.ones_like(mag))))
+    ex = torch.where(torch.exp2(ex) > mag, ex - 1, ex)
+    ex = torch.where(torch.exp2(ex + 1) <= mag, ex + 1, ex).clamp(min=lowest)
+    step = torch.exp2(ex - bits)
+    return (torch.round(y / step) * step).clamp(-top, top) * a
+
+
+def _least_scale(amax, top):
+    """The least power of two a with amax <= top * a; 1 where amax is 0."""
+    e = torch.ceil(torch.log2(torch.where(amax > 0, amax, torch.full_like(amax, top)) / top))
+    e = torch.where(amax > top * torch.exp2(e), e + 1, e)
+    e = torch.where((amax > 0) & (amax <= top * torch.exp2(e - 1)), e - 1, e)
+    return torch.exp2(e.clamp(min=-126))
+
+
+def _blocks64(rows, blk):
+    """[n, d] bf16 rows of one sequence and head, whole blocks, as the 8-bit cache holds them."""
+    x = rows.to(F64).view(-1, blk * rows.shape[1])
+    return _grid(x, _least_scale(x.abs().amax(1, keepdim=True), 448.0), -6, 3, 448.0).view(rows.shape)
+
+
+def _mx4_64(x):
+    r, k = x.shape
+    x = torch.cat([x.to(F64), torch.zeros(r, -k % 32, dtype=F64, device=DEV)], 1).reshape(-1, 32)
+    amax = x.abs().amax(1, keepdim=True)
+    # a power of two with 4 <= amax / a < 8
+    a = 2 * _least_scale(torch.where(amax > 0, amax, torch.full_like(amax, 2.0)), 8.0)
+    a = torch.where(amax / a < 4, a / 2, a).clamp(min=2.0 ** -126)
+    return _grid(x, a, 0, 1, 6.0).view(r, -1)[:, :k]
+
+
+def exact(case, seed):
+    s = _inputs(case, seed)
+    kind = case["kind"]
+    if kind == "quantize":
+        return _mx4_64(s["x"]).contiguous()
+    if kind == "linear":
+        w = torch.cat([_mx4_64(part) for part in s["w"].split(4096)])
+        y = (_mx4_64(s["x"]) if case["x"] == "mx4" else s["x"].to(BF16).to(F64)) @ w.t()
+        return y[:, 0::2] * torch.sigmoid(y[:, 0::2]) * y[:, 1::2] if case["swiglu"] else y
+    b, t, ctx, blk = case["batch"], case["tokens"], case["ctx"], case["block"]
+    k, v = (torch.cat([s["c" + x], s[x].to(BF16)], 1) for x in "kv")
+    h, d = k.shape[2:]
+    n, first = (ctx + t) // blk * blk, ctx // blk * blk
+    if kind == "append":
+        out = []
+        for x in (k, v):
+            y = x[:, first:].to(F64)
+            for i in range(b):
+                for j in range(h):
+                    y[i, : n - first, j] = _blocks64(x[i, first:n, j], blk)
+            out.append(y)
+        return out
+    q = s["q"].to(F64)
+    g = q.shape[2] // h
+    o = torch.empty_like(q)
+    p = ctx + torch.arange(t, device=DEV)
+    key = torch.arange(ctx + t, device=DEV)
+    own_block = (key[None] >= (p // blk * blk)[:, None])[:, None]      # [t, 1, keys]
+    seen = (key[None] <= p[:, None])[:, None]
+    for i in range(b):
+        for j in range(h):
+            kk, vv = k[i, :, j].to(F64), v[i, :, j].to(F64)
+            k8, v8 = kk.clone(), vv.clone()
+            k8[:n], v8[:n] = _blocks64(k[i, :n, j], blk), _blocks64(v[i, :n, j], blk)
+            qq = q[i, :, j * g:(j + 1) * g]
+            sc = torch.where(own_block, (qq.reshape(t * g, d) @ kk.t()).view(t, g, -1), (qq.reshape(t * g, d) @ k8.t()).view(t, g, -1))
+            w = torch.softmax(torch.where(seen, sc / math.sqrt(d), -math.inf), -1)
+            near, far = torch.where(own_block, w, 0.0), torch.where(own_block, 0.0, w)
+            o[i, :, j * g:(j + 1) * g] = (near.reshape(t * g, -1) @ vv + far.reshape(t * g, -1) @ v8).view(t, g, d)
+    return o
