@@ -11,7 +11,7 @@ A case is a dict of plain values; ``kind`` names the operator:
   bf16 as it is read), or mx4, where x is quantized to 4 bits within the pass and both operands are 4-bit.
 
 The 8-bit cache. Rows are held to bf16. Of each block of ``block`` tokens and KV head, K and V apart, a = max |x|; e is
-the least integer with a <= 448 * 2^e (0 where a = 0, at least -126) and a value is e4m3(x * 2^-e) * 2^e. A query at
+the least integer with a <= 448 * 2^e (0 where a = 0, within -126 .. 119) and a value is e4m3(x * 2^-e) * 2^e. A query at
 position p reads the blocks before its own in 8 bits and its own block's rows up to p in bf16.
 
 The 4-bit format (OCP MX, MXFP4): of each 32 values along k, e = floor(log2 max |x|) - 2 (0 where all are 0, at least
@@ -170,8 +170,8 @@ def _seal(x, blk):
     x = x.view(b, n // blk, blk, h, d).permute(0, 3, 1, 2, 4).float()
     m, ex = torch.frexp(x.abs().amax(dim=(3, 4)))
     e = torch.where(m <= 0.875, ex - 9, ex - 8)
-    e = torch.where(m == 0, torch.zeros_like(e), e).clamp(min=-126)
-    return (x * _pow2(-e)[..., None, None]).to(F8), e.to(torch.int8)
+    e = torch.where(m == 0, torch.zeros_like(e), e).clamp(-126, 119)
+    return (x * _pow2(-e)[..., None, None]).clamp(-448, 448).to(F8), e.to(torch.int8)
 
 
 def _open(codes, e):
@@ -321,7 +321,7 @@ def _least_scale(amax, top):
     e = torch.ceil(torch.log2(torch.where(amax > 0, amax, torch.full_like(amax, top)) / top))
     e = torch.where(amax > top * torch.exp2(e), e + 1, e)
     e = torch.where((amax > 0) & (amax <= top * torch.exp2(e - 1)), e - 1, e)
-    return torch.exp2(e.clamp(min=-126))
+    return torch.exp2(e.clamp(-126, 119))
 
 
 def _blocks64(rows, blk):
