@@ -11,6 +11,7 @@
 #include <type_traits>
 
 #include "mirror_layout.h"
+#include "paged8.h"
 
 namespace dkv {
 
@@ -607,7 +608,8 @@ __device__ __forceinline__ int evict(const RowCtx& c, int n, int budget, dkv_qcf
 // positions start.. from the input tensors or the full cache, then evict.
 struct OpArgs {
     dkv_drafter_t m;
-    dkv_paged_t full;        // used when src_full
+    dkv_paged_t full;        // used when src_full (full8 by the kernel over an 8-bit full cache)
+    dkv_paged8_t full8;
     dkv_qcfg_t cfgs[64];     // per layer arm
     const void* k;           // [batch][T][Hkv][D] when !src_full
     const void* v;
@@ -619,6 +621,7 @@ struct OpArgs {
     int budget_per_layer;
 };
 
+template <bool FULL8>
 __global__ void __launch_bounds__(OP_BLK) drafter_op_kernel(OpArgs a) {
     const int s = blockIdx.x, L = a.layer0 + blockIdx.y;
     const dkv_drafter_t& m = a.m;
@@ -681,6 +684,11 @@ __global__ void __launch_bounds__(OP_BLK) drafter_op_kernel(OpArgs a) {
             const int i = slot % PAGE;
             if (pre && h == w) {   // (T == 1: t == 0) the channels loaded above
                 quant_row_vals(pk, pv, c.f, cfg.bits, page, i, lane);
+            } else if (FULL8) {
+                const dkv_paged8_t& f = a.full8;
+                const int pos = p0 + t, len = a.end[s];
+                quant_row([&](int d) { return p8_value(f, s, L, pos, len, h, d, 0); },
+                          [&](int d) { return p8_value(f, s, L, pos, len, h, d, 1); }, c.f, cfg.bits, page, i, lane);
             } else if (a.src_full) {
                 const dkv_paged_t& f = a.full;
                 const int pos = p0 + t;
@@ -717,12 +725,14 @@ __global__ void __launch_bounds__(OP_BLK) drafter_op_kernel(OpArgs a) {
 struct RebuildArgs {
     dkv_drafter_t m;
     dkv_paged_t full;
+    dkv_paged8_t full8;      // in its place for the kernel over an 8-bit full cache
     dkv_qcfg_t cfgs[64];
     int32_t layers[64];
     const int32_t* len;
     const int32_t* budget;
 };
 
+template <bool FULL8>
 __global__ void __launch_bounds__(BLK) drafter_rebuild_kernel(RebuildArgs a) {
     const int s = blockIdx.y, L = a.layers[blockIdx.z];
     const dkv_drafter_t& m = a.m;
@@ -760,14 +770,16 @@ __global__ void __launch_bounds__(BLK) drafter_rebuild_kernel(RebuildArgs a) {
                 const int r = page * PAGE + i;
                 if (r >= kept) continue;
                 const int p = r < sink ? r : n - (kept - sink) + (r - sink);
-                const int32_t blk = paged_block(f, s, L, p);
-                const int off = p % f.block_size;
+                const int32_t blk = FULL8 ? 0 : paged_block(f, s, L, p);
+                const int off = FULL8 ? 0 : p % f.block_size;
                 LaneCodes lc;
-                quant_lane([&](int d) { return load_elem(f.pool, paged_k_off(f, blk, off, h, d), f.dtype); }, pf,
-                           cfg.bits, lane, lc);
+                quant_lane([&](int d) {
+                    return FULL8 ? p8_value(a.full8, s, L, p, n, h, d, 0)
+                                 : load_elem(f.pool, paged_k_off(f, blk, off, h, d), f.dtype); }, pf, cfg.bits, lane, lc);
                 put_k_lane(pg, pf, i, lane, lc);
-                quant_lane([&](int d) { return load_elem(f.pool, paged_v_off(f, blk, off, h, d), f.dtype); }, pf,
-                           cfg.bits, lane, lc);
+                quant_lane([&](int d) {
+                    return FULL8 ? p8_value(a.full8, s, L, p, n, h, d, 1)
+                                 : load_elem(f.pool, paged_v_off(f, blk, off, h, d), f.dtype); }, pf, cfg.bits, lane, lc);
                 if (pf.cb == 4) {
 #pragma unroll
                     for (int x = 0; x < 8; ++x) vw[x] |= static_cast<uint32_t>(lc.code[x]) << code_shift(4, e);
@@ -1365,7 +1377,7 @@ extern "C" int dkv_drafter_append(const dkv_drafter_t* mirror, int32_t layer, dk
     a.start = start;
     a.count = count;
     a.budget = budget;
-    hipLaunchKernelGGL(drafter_op_kernel, dim3(mirror->batch, 1), dim3(OP_BLK), 0, as_stream(stream), a);
+    hipLaunchKernelGGL(drafter_op_kernel<false>, dim3(mirror->batch, 1), dim3(OP_BLK), 0, as_stream(stream), a);
     return check_launch("dkv_drafter_append");
 }
 
@@ -1384,7 +1396,7 @@ extern "C" int dkv_drafter_truncate(const dkv_drafter_t* mirror, const dkv_qcfg_
     a.T = 0;              // nothing appended, so no eviction and budget is never read
     a.start = start;
     a.budget = start;
-    hipLaunchKernelGGL(drafter_op_kernel, dim3(mirror->batch, mirror->n_layers), dim3(OP_BLK), 0, as_stream(stream), a);
+    hipLaunchKernelGGL(drafter_op_kernel<false>, dim3(mirror->batch, mirror->n_layers), dim3(OP_BLK), 0, as_stream(stream), a);
     return check_launch("dkv_drafter_truncate");
 }
 
@@ -1413,7 +1425,7 @@ extern "C" int dkv_drafter_sync(const dkv_drafter_t* mirror, const dkv_paged_t* 
     a.end = end;
     a.budget = budget;
     a.budget_per_layer = 1;
-    hipLaunchKernelGGL(drafter_op_kernel, dim3(mirror->batch, mirror->n_layers), dim3(OP_BLK), 0, as_stream(stream), a);
+    hipLaunchKernelGGL(drafter_op_kernel<false>, dim3(mirror->batch, mirror->n_layers), dim3(OP_BLK), 0, as_stream(stream), a);
     return check_launch("dkv_drafter_sync");
 }
 
@@ -1475,10 +1487,64 @@ extern "C" int dkv_drafter_rebuild(const dkv_drafter_t* mirror, const dkv_paged_
             hipLaunchKernelGGL(drafter_rebuild_page_kernel<false>, grid, dim3(BLK), 0, as_stream(stream), a);
         }
     } else {
-        hipLaunchKernelGGL(drafter_rebuild_kernel, dim3(mirror->cap / PAGE, mirror->batch, n_changed), dim3(BLK), 0,
+        hipLaunchKernelGGL(drafter_rebuild_kernel<false>, dim3(mirror->cap / PAGE, mirror->batch, n_changed), dim3(BLK), 0,
                            as_stream(stream), a);
     }
     return check_launch("dkv_drafter_rebuild");
+}
+
+static int same_shape8(const dkv_drafter_t* m, const dkv_paged8_t* f) {
+    return f->n_layers == m->n_layers && f->n_kv_heads == m->n_kv_heads && f->head_dim == m->head_dim &&
+           f->batch == m->batch;
+}
+
+extern "C" int dkv_drafter_sync_paged8(const dkv_drafter_t* mirror, const dkv_paged8_t* full, const dkv_qcfg_t* cfgs,
+                                       const int32_t* start, const int32_t* end, const int32_t* budget,
+                                       dkv_stream_t stream) {
+    int rc = check_mirror(mirror, "dkv_drafter_sync_paged8");
+    if (rc || (rc = p8_check(full, 0, "dkv_drafter_sync_paged8"))) return rc;
+    DKV_REQUIRE(cfgs && start && end && budget, "dkv_drafter_sync_paged8: NULL argument");
+    DKV_REQUIRE(same_shape8(mirror, full), "dkv_drafter_sync_paged8: full cache and mirror shapes differ");
+    OpArgs a{};
+    a.m = *mirror;
+    a.full8 = *full;
+    for (int L = 0; L < mirror->n_layers; ++L) {
+        if ((rc = check_cfg(mirror, cfgs[L], "dkv_drafter_sync_paged8"))) return rc;
+        a.cfgs[L] = cfgs[L];
+    }
+    a.src_full = 1;
+    a.do_trunc = 1;
+    a.start = start;
+    a.end = end;
+    a.budget = budget;
+    a.budget_per_layer = 1;
+    hipLaunchKernelGGL(drafter_op_kernel<true>, dim3(mirror->batch, mirror->n_layers), dim3(OP_BLK), 0, as_stream(stream), a);
+    return check_launch("dkv_drafter_sync_paged8");
+}
+
+extern "C" int dkv_drafter_rebuild_paged8(const dkv_drafter_t* mirror, const dkv_paged8_t* full, const int32_t* layers,
+                                          int32_t n_changed, const dkv_qcfg_t* cfgs, const int32_t* len,
+                                          const int32_t* budget, dkv_stream_t stream) {
+    int rc = check_mirror(mirror, "dkv_drafter_rebuild_paged8");
+    if (rc || (rc = p8_check(full, 0, "dkv_drafter_rebuild_paged8"))) return rc;
+    DKV_REQUIRE(layers && cfgs && len && budget, "dkv_drafter_rebuild_paged8: NULL argument");
+    DKV_REQUIRE(same_shape8(mirror, full), "dkv_drafter_rebuild_paged8: full cache and mirror shapes differ");
+    DKV_REQUIRE(n_changed >= 0 && n_changed <= mirror->n_layers, "dkv_drafter_rebuild_paged8: bad layer count");
+    if (n_changed == 0) return DKV_OK;
+    RebuildArgs a{};
+    a.m = *mirror;
+    a.full8 = *full;
+    for (int L = 0; L < mirror->n_layers; ++L) a.cfgs[L] = cfgs[L];
+    for (int i = 0; i < n_changed; ++i) {
+        DKV_REQUIRE(layers[i] >= 0 && layers[i] < mirror->n_layers, "dkv_drafter_rebuild_paged8: layer out of range");
+        if ((rc = check_cfg(mirror, cfgs[layers[i]], "dkv_drafter_rebuild_paged8"))) return rc;
+        a.layers[i] = layers[i];
+    }
+    a.len = len;
+    a.budget = budget;
+    hipLaunchKernelGGL(drafter_rebuild_kernel<true>, dim3(mirror->cap / PAGE, mirror->batch, n_changed), dim3(BLK), 0,
+                       as_stream(stream), a);
+    return check_launch("dkv_drafter_rebuild_paged8");
 }
 
 extern "C" int dkv_drafter_gather(const dkv_drafter_t* mirror, int32_t seq, int32_t layer, dkv_qcfg_t cfg,

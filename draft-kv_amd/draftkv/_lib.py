@@ -26,6 +26,13 @@ class Paged(C.Structure):
                 ("dtype", C.c_int32)]
 
 
+class Paged8(C.Structure):
+    _fields_ = [("pool", C.c_void_p), ("block_table", C.c_void_p), ("tail", C.c_void_p), ("hot", C.c_void_p),
+                ("batch", C.c_int32), ("n_layers", C.c_int32), ("n_kv_heads", C.c_int32),
+                ("head_dim", C.c_int32), ("block_size", C.c_int32), ("max_blocks", C.c_int32),
+                ("tail_rows", C.c_int32), ("hot_rows", C.c_int32)]
+
+
 class Drafter(C.Structure):
     _fields_ = [("pages", C.c_void_p), ("pos", C.c_void_p), ("score", C.c_void_p), ("n_rows", C.c_void_p),
                 ("batch", C.c_int32), ("n_layers", C.c_int32), ("n_kv_heads", C.c_int32),
@@ -38,18 +45,27 @@ class QCfg(C.Structure):
 
 
 P, I32, I64, F32, SZ = C.c_void_p, C.c_int32, C.c_int64, C.c_float, C.c_size_t
-PPaged, PDrafter, PQCfg = C.POINTER(Paged), C.POINTER(Drafter), C.POINTER(QCfg)
+PPaged, PPaged8, PDrafter, PQCfg = C.POINTER(Paged), C.POINTER(Paged8), C.POINTER(Drafter), C.POINTER(QCfg)
 
 _SIGS = {
     "dkv_quantize": (C.c_int, [P, I64, I32, I32, I32, I32, P, P, P, P, P]),
     "dkv_paged_append": (C.c_int, [PPaged, I32, P, P, I32, I32, P, P, P]),
     "dkv_paged_attention_workspace": (SZ, [PPaged, I32, I32, I32, I32]),
     "dkv_paged_attention": (C.c_int, [PPaged, I32, P, I32, I32, P, P, I32, I32, P, P, SZ, P]),
+    "dkv_paged8_block_bytes": (I64, [I32, I32, I32]),
+    "dkv_paged8_row_bytes": (I64, [I32, I32]),
+    "dkv_paged8_hot_rows": (I32, [PPaged8, I32]),
+    "dkv_paged8_append": (C.c_int, [PPaged8, I32, P, P, I32, I32, P, P, P]),
+    "dkv_paged8_attention_workspace": (SZ, [PPaged8, I32, I32, I32]),
+    "dkv_paged8_attention": (C.c_int, [PPaged8, I32, P, I32, I32, I32, P, P, I32, P, P, SZ, P]),
+    "dkv_paged8_read": (C.c_int, [PPaged8, I32, P, P, I32, P, P, P]),
     "dkv_page_bytes": (I64, [I32, I32, I32, I32]),
     "dkv_drafter_append": (C.c_int, [PDrafter, I32, QCfg, P, P, I32, I32, P, P, P, P]),
     "dkv_drafter_truncate": (C.c_int, [PDrafter, PQCfg, P, P]),
     "dkv_drafter_sync": (C.c_int, [PDrafter, PPaged, PQCfg, P, P, P, P]),
     "dkv_drafter_rebuild": (C.c_int, [PDrafter, PPaged, C.POINTER(I32), I32, PQCfg, P, P, P]),
+    "dkv_drafter_sync_paged8": (C.c_int, [PDrafter, PPaged8, PQCfg, P, P, P, P]),
+    "dkv_drafter_rebuild_paged8": (C.c_int, [PDrafter, PPaged8, C.POINTER(I32), I32, PQCfg, P, P, P]),
     "dkv_drafter_attention_workspace": (SZ, [PDrafter, I32, I32]),
     "dkv_drafter_attention": (C.c_int, [PDrafter, I32, QCfg, P, I32, I32, P, P, SZ, P]),
     "dkv_drafter_kernel_timing": (C.c_int, [I32]),

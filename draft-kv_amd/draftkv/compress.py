@@ -52,9 +52,9 @@ class FullKVCache(PagedKVCache):
 
     def __init__(self, n_layers: int, n_heads: Optional[int] = None, d_head: Optional[int] = None, *,
                  dtype=np.float32, batch: int = 1, max_tokens: int = 1 << 20, device=None,
-                 block_size: int = 16, chunk_keys: Optional[int] = None) -> None:
+                 block_size: int = 16, chunk_keys: Optional[int] = None, tail_rows: Optional[int] = None) -> None:
         self._lazy = dict(n_layers=n_layers, dtype=dtype, batch=batch, max_tokens=max_tokens, device=device,
-                          block_size=block_size, chunk_keys=chunk_keys)
+                          block_size=block_size, chunk_keys=chunk_keys, tail_rows=tail_rows)
         self.n_layers = n_layers
         self._ready = False
         if n_heads is not None and d_head is not None:
@@ -64,14 +64,14 @@ class FullKVCache(PagedKVCache):
         a = self._lazy
         super().__init__(a["n_layers"], n_heads, d_head, a["block_size"], n_blocks, a["dtype"],
                          batch=a["batch"], max_tokens=a["max_tokens"], device=a["device"],
-                         chunk_keys=a["chunk_keys"])
+                         chunk_keys=a["chunk_keys"], tail_rows=a["tail_rows"])
         self._ready = True
 
     def _grow(self) -> None:
         old = self.n_blocks
         new = old * 2
         per_block = self.store.shape[1]
-        store = torch.empty((self.batch * new, per_block), dtype=self.dtype, device=self.device)
+        store = torch.empty((self.batch * new, per_block), dtype=self.store.dtype, device=self.device)
         for s in range(self.batch):
             store[s * new: s * new + old].copy_(self.store[s * old: (s + 1) * old])
         self.store = store

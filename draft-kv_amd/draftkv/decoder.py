@@ -71,7 +71,7 @@ class Decoder:
         if dtype not in (torch.float32, torch.bfloat16):
             raise ValueError("dtype must be torch.float32 or torch.bfloat16")
         self.act_dtype = dtype           # dtype of GEMM inputs
-        self.kv_dtype = dtype            # dtype of the full cache
+        self.kv_dtype = dtype            # dtype of the full cache; torch.float8_e4m3fn holds it in 8 bits
         self._cs: Optional[torch.Tensor] = None
         self._cs_len = 0
 
@@ -92,7 +92,8 @@ class Decoder:
     def new_cache(self, batch: int = 1, max_tokens: int = 1 << 20, chunk_keys: Optional[int] = None) -> FullKVCache:
         """The full cache for ``batch`` sequences of up to ``max_tokens`` rows;
         ``chunk_keys`` fixes the attention kernel's key chunk (by default
-        chosen from the shape, ``paged.auto_chunk_keys``)."""
+        chosen from the shape, ``paged.auto_chunk_keys``). Its type is
+        ``kv_dtype``: the model's, or torch.float8_e4m3fn when set so."""
         return FullKVCache(self.n_layers, self.n_kv_heads, self.d_head, dtype=self.kv_dtype, batch=batch,
                            max_tokens=max_tokens, device=self.device, chunk_keys=chunk_keys)
 
@@ -287,8 +288,7 @@ class Decoder:
         key count of every sequence: it sizes the launch and the workspace,
         and keys past it may go unseen."""
         def attn(L, q, k, v):
-            cache.append_layer(L, k, v, start_d, count_d)
-            return cache.attend(L, q, start_d, max_len, count=count_d)
+            return cache.append_attend(L, q, k, v, start_d, max_len, count_d)
 
         attn.finish = lambda: None
         return attn

@@ -400,6 +400,8 @@ class DecodeBatch:
         room = int(getattr(full, "max_tokens", 0) or 0)
         if room:
             gamma = max(0, min(gamma, room - int(n[active].max()), self.cap_tokens - int(n[active].max())))
+        # an 8-bit cache can take back as many rows as its bf16 tail holds beside a block
+        gamma = min(gamma, getattr(full, "max_rollback", gamma))
         flen = full.lengths()
 
         ph, ev = self.phases, {}

@@ -12,7 +12,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import _lib
-from ._lib import DKV_BF16, DKV_F32, DKV_GEMM_DEFER, DKV_GEMM_SWIGLU, DKV_GEMM_WTILED, Drafter, Paged, QCfg, check, lib
+from ._lib import DKV_BF16, DKV_F32, DKV_GEMM_DEFER, DKV_GEMM_SWIGLU, DKV_GEMM_WTILED, Drafter, Paged, Paged8, QCfg, check, lib
 
 
 _get_device = getattr(torch._C, "_cuda_getDevice", None)
@@ -27,6 +27,13 @@ def _stream() -> int:
     if _raw_stream is not None and _get_device is not None:
         return _raw_stream(_get_device())
     return torch.cuda.current_stream().cuda_stream
+
+
+def _device(dev: torch.device):
+    """The launch's device made current, where it is not (the stream is then that device's current one)."""
+    if dev.index is None or _get_device is not None and _get_device() == dev.index:
+        return contextlib.nullcontext()
+    return torch.cuda.device(dev)
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -193,6 +200,77 @@ def paged_attention(desc: Paged, layer: int, q: torch.Tensor, start: torch.Tenso
     return out
 
 
+# ------------------------------------------------------------------ paged full cache in 8 bits
+def _need_rows(t: Optional[torch.Tensor], name: str, batch: int, device) -> None:
+    """A per-sequence int32 vector beside the cache."""
+    if t is None:
+        return
+    _need(t, name, torch.int32)
+    if t.numel() != batch:
+        raise ValueError(f"{name} must hold one value per sequence ({batch}), got {tuple(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{name} must be on {device}")
+
+
+def paged8_append(desc: Paged8, layer: int, k: torch.Tensor, v: torch.Tensor, start: torch.Tensor,
+                  count: Optional[torch.Tensor] = None) -> None:
+    """Append k, v [batch, T, Hkv, D] (float32 or bfloat16) at positions start[s].. to a full cache in 8 bits;
+    blocks that fill up are coded (``dkv_paged8_append``)."""
+    _need(k, "k", ndim=4)
+    _need(v, "v", ndim=4)
+    if k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
+        raise ValueError("k and v must match")
+    b, T, H, D = k.shape
+    if b != desc.batch or H != desc.n_kv_heads or D != desc.head_dim:
+        raise ValueError(f"k shape {tuple(k.shape)} does not match the cache")
+    _need_rows(start, "start", b, k.device)
+    _need_rows(count, "count", b, k.device)
+    with _device(k.device):
+        check(lib().dkv_paged8_append(C.byref(desc), layer, k.data_ptr(), v.data_ptr(), _dt(k), T, start.data_ptr(),
+                                      _ptr(count), _stream()), "dkv_paged8_append")
+
+
+def paged8_attention(desc: Paged8, layer: int, q: torch.Tensor, start: torch.Tensor, max_len: int,
+                     out: Optional[torch.Tensor] = None, count: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention of q [batch, T, Hq, D] (float32 or bfloat16; the result has its type) over a full cache in
+    8 bits, of the rows that ``paged8_append`` just wrote (same T, start and count). max_len bounds start + count."""
+    _need(q, "q", ndim=4)
+    b, T, Hq, D = q.shape
+    if b != desc.batch or D != desc.head_dim:
+        raise ValueError(f"q shape {tuple(q.shape)} does not match the cache")
+    _need_rows(start, "start", b, q.device)
+    _need_rows(count, "count", b, q.device)
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        _need(out, "out", q.dtype, 4)
+        if out.shape != q.shape or out.device != q.device:
+            raise ValueError(f"out must have q's shape {tuple(q.shape)} and device")
+    with _device(q.device):
+        nbytes = lib().dkv_paged8_attention_workspace(C.byref(desc), T, Hq, max_len)
+        ws = _WS.get(q.device, nbytes)
+        check(lib().dkv_paged8_attention(C.byref(desc), layer, q.data_ptr(), _dt(q), T, Hq, start.data_ptr(), _ptr(count),
+                                         max_len, out.data_ptr(), ws.data_ptr(), ws.numel(), _stream()),
+              "dkv_paged8_attention")
+    return out
+
+
+def paged8_read(desc: Paged8, layer: int, first: torch.Tensor, length: torch.Tensor, T: int):
+    """float32 k, v [batch, T, Hkv, D] that the cache stands for at positions first[s] .. first[s] + T - 1 (zeros past
+    length[s], the rows the sequence holds)."""
+    b, dev = desc.batch, first.device
+    _need_rows(first, "first", b, dev)
+    _need_rows(length, "length", b, dev)
+    if T < 0:
+        raise ValueError("T must not be negative")
+    k = torch.empty((b, T, desc.n_kv_heads, desc.head_dim), dtype=torch.float32, device=dev)
+    v = torch.empty_like(k)
+    with _device(dev):
+        check(lib().dkv_paged8_read(C.byref(desc), layer, first.data_ptr(), length.data_ptr(), T, k.data_ptr(),
+                                    v.data_ptr(), _stream()), "dkv_paged8_read")
+    return k, v
+
+
 # ------------------------------------------------------------------ mirror
 def _qarr(cfgs: Sequence[QCfg]):
     arr = (QCfg * len(cfgs))(*cfgs)
@@ -219,21 +297,23 @@ def drafter_truncate(desc: Drafter, cfgs: Sequence[QCfg], start: torch.Tensor) -
           "dkv_drafter_truncate")
 
 
-def drafter_sync(desc: Drafter, full: Paged, cfgs: Sequence[QCfg], start: torch.Tensor, end: torch.Tensor,
+def drafter_sync(desc: Drafter, full, cfgs: Sequence[QCfg], start: torch.Tensor, end: torch.Tensor,
                  budget: torch.Tensor) -> None:
     for t, n in ((start, "start"), (end, "end"), (budget, "budget")):
         _need(t, n, torch.int32)
-    check(lib().dkv_drafter_sync(C.byref(desc), C.byref(full), _qarr(cfgs), start.data_ptr(), end.data_ptr(),
-                                 budget.data_ptr(), _stream()), "dkv_drafter_sync")
+    fn = "dkv_drafter_sync_paged8" if isinstance(full, Paged8) else "dkv_drafter_sync"
+    check(getattr(lib(), fn)(C.byref(desc), C.byref(full), _qarr(cfgs), start.data_ptr(), end.data_ptr(),
+                             budget.data_ptr(), _stream()), fn)
 
 
-def drafter_rebuild(desc: Drafter, full: Paged, layers: Sequence[int], cfgs: Sequence[QCfg],
+def drafter_rebuild(desc: Drafter, full, layers: Sequence[int], cfgs: Sequence[QCfg],
                     length: torch.Tensor, budget: torch.Tensor) -> None:
     _need(length, "length", torch.int32)
     _need(budget, "budget", torch.int32)
     la = (C.c_int32 * max(1, len(layers)))(*layers)
-    check(lib().dkv_drafter_rebuild(C.byref(desc), C.byref(full), la, len(layers), _qarr(cfgs),
-                                    length.data_ptr(), budget.data_ptr(), _stream()), "dkv_drafter_rebuild")
+    fn = "dkv_drafter_rebuild_paged8" if isinstance(full, Paged8) else "dkv_drafter_rebuild"
+    check(getattr(lib(), fn)(C.byref(desc), C.byref(full), la, len(layers), _qarr(cfgs), length.data_ptr(),
+                             budget.data_ptr(), _stream()), fn)
 
 
 def drafter_attention(desc: Drafter, layer: int, cfg: QCfg, q: torch.Tensor, want_mass: bool,

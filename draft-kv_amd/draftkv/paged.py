@@ -14,6 +14,13 @@ of physical blocks, so each sequence's block ids are exactly those of a
 batch-1 reference run. Block tables are mirrored to the device (int32
 ``[batch][n_layers][max_blocks]``) once per forward, before the kernels read
 them.
+
+``dtype=torch.float8_e4m3fn`` holds the cache in 8 bits: blocks are coded with
+a power-of-two scale per block and head once they are full, and the last
+``tail_rows`` rows of a sequence are also kept in bf16. A query reads its own
+block's rows in bf16 and the blocks before it in 8 bits, so its result does not
+depend on how the rows came (a verify block, one by one, after a rollback):
+greedy speculative decoding equals plain decoding over the same cache.
 """
 
 from __future__ import annotations
@@ -25,7 +32,7 @@ import numpy as np
 import torch
 
 from . import ops
-from ._lib import DKV_BF16, DKV_F32, Paged
+from ._lib import DKV_BF16, DKV_F32, Paged, Paged8, lib
 
 
 class BlockPoolExhausted(RuntimeError):
@@ -85,7 +92,9 @@ def _torch_dtype(dtype) -> torch.dtype:
         return torch.float32
     if dtype in (torch.bfloat16, "bfloat16", "bf16"):
         return torch.bfloat16
-    raise ValueError(f"unsupported cache dtype {dtype!r} (float32 or bfloat16)")
+    if dtype in (torch.float8_e4m3fn, "float8_e4m3fn", "fp8"):
+        return torch.float8_e4m3fn
+    raise ValueError(f"unsupported cache dtype {dtype!r} (float32, bfloat16 or float8_e4m3fn)")
 
 
 def auto_chunk_keys(batch: int, n_heads: int, max_tokens: int) -> int:
@@ -113,12 +122,17 @@ class PagedKVCache:
     dtype=np.float32)`` is the reference signature (n_heads = KV heads);
     ``batch``, ``max_tokens``, ``device`` and ``chunk_keys`` (the fixed key
     chunk of the attention kernel; by default ``auto_chunk_keys``) are
-    additions.
+    additions. With ``dtype=torch.float8_e4m3fn`` block_size is 16, 32, 64 or
+    128 and ``tail_rows`` (a multiple of 16, by default block_size + 112) rows
+    per sequence stay in bf16: ``truncate`` to a position inside a block needs
+    that block's rows among them, which any rollback by up to ``max_rollback``
+    rows has.
     """
 
     def __init__(self, n_layers: int, n_heads: int, d_head: int, block_size: int = 16,
                  n_blocks: int = 512, dtype=np.float32, *, batch: int = 1,
-                 max_tokens: Optional[int] = None, device=None, chunk_keys: Optional[int] = None) -> None:
+                 max_tokens: Optional[int] = None, device=None, chunk_keys: Optional[int] = None,
+                 tail_rows: Optional[int] = None) -> None:
         self.n_layers, self.n_heads, self.d_head = n_layers, n_heads, d_head
         self.block_size, self.n_blocks, self.batch = block_size, n_blocks, batch
         self.dtype = _torch_dtype(dtype)
@@ -127,16 +141,55 @@ class PagedKVCache:
         self.chunk_keys = chunk_keys if chunk_keys is not None else auto_chunk_keys(batch, n_heads, self.max_tokens)
         self.max_blocks = -(-self.max_tokens // block_size)
         self.pools = [BlockPool(n_blocks, block_size) for _ in range(batch)]
-        per_block = 2 * n_heads * block_size * d_head
-        self.store = torch.empty((batch * n_blocks, per_block), dtype=self.dtype, device=self.device)
+        self.fp8 = self.dtype == torch.float8_e4m3fn
+        if self.fp8:
+            self._init_fp8(tail_rows)
+        else:
+            per_block = 2 * n_heads * block_size * d_head
+            self.store = torch.empty((batch * n_blocks, per_block), dtype=self.dtype, device=self.device)
         self.tables = np.full((batch, n_layers, self.max_blocks), -1, np.int32)   # local ids
         self.table_len = np.zeros((batch, n_layers), np.int64)
         self.n_tokens = np.zeros((batch, n_layers), np.int64)
         self.d_tables = torch.full((batch, n_layers, self.max_blocks), 0, dtype=torch.int32, device=self.device)
         self._dirty: Optional[tuple[int, int]] = None   # [lo, hi) block-index range to upload
 
+    # ------------------------------------------------------------ 8 bits
+    def _init_fp8(self, tail_rows: Optional[int]) -> None:
+        bs, H, D = self.block_size, self.n_heads, self.d_head
+        if bs not in (16, 32, 64, 128):
+            raise ValueError(f"an 8-bit cache's block_size is 16, 32, 64 or 128, got {bs}")
+        if not 1 <= D <= 256:
+            raise ValueError(f"an 8-bit cache's d_head is at most 256, got {D}")
+        self.tail_rows = bs + 112 if tail_rows is None else int(tail_rows)
+        if self.tail_rows % 16 or self.tail_rows < bs + 16:
+            raise ValueError(f"tail_rows must be a multiple of 16, at least block_size + 16, got {self.tail_rows}")
+        self.max_rollback = self.tail_rows - bs - 15
+        self._row_bytes = int(lib().dkv_paged8_row_bytes(H, D))
+        kw = dict(dtype=torch.uint8, device=self.device)
+        self.store = torch.empty((self.batch * self.n_blocks, int(lib().dkv_paged8_block_bytes(H, D, bs))), **kw)
+        self.tail = torch.empty((self.batch, self.n_layers, self.tail_rows, self._row_bytes), **kw)
+        self.hot = torch.empty((self.batch, 0, self._row_bytes), **kw)      # rows of long appends, grown by need
+        # the first position whose bf16 row is still there, per (sequence, layer)
+        self.tail_from = np.zeros((self.batch, self.n_layers), np.int64)
+
+    def _hot_room(self, T: int) -> None:
+        """Room for an append of T rows that the tail does not hold beside an open block."""
+        need = int(lib().dkv_paged8_hot_rows(self.desc(), T))
+        if need > self.hot.shape[1]:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"append of {T} rows under graph capture: run one of that length before")
+            self.hot = torch.empty((self.batch, need, self._row_bytes), dtype=torch.uint8, device=self.device)
+
+    def _written(self, end: np.ndarray, layers) -> None:
+        """Rows up to end [batch, ...] are in ``layers``: the tail holds the last tail_rows (whole 16s) of them."""
+        self.tail_from[:, layers] = np.maximum(self.tail_from[:, layers], -(-end // 16) * 16 - self.tail_rows)
+
     # ------------------------------------------------------------ descriptor
-    def desc(self) -> Paged:
+    def desc(self):
+        if self.fp8:
+            return Paged8(self.store.data_ptr(), self.d_tables.data_ptr(), self.tail.data_ptr(), self.hot.data_ptr(),
+                          self.batch, self.n_layers, self.n_heads, self.d_head, self.block_size, self.max_blocks,
+                          self.tail_rows, self.hot.shape[1])
         return Paged(self.store.data_ptr(), self.d_tables.data_ptr(), self.batch, self.n_layers, self.n_heads,
                      self.d_head, self.block_size, self.max_blocks,
                      DKV_BF16 if self.dtype == torch.bfloat16 else DKV_F32)
@@ -203,17 +256,42 @@ class PagedKVCache:
                      count: Optional[torch.Tensor] = None) -> None:
         """Write ``k, v`` [batch, T, heads, d_head] at positions start[s]..; blocks
         must have been reserved."""
+        if self.fp8:
+            self._hot_room(k.shape[1])
+            ops.paged8_append(self.desc(), layer, k, v, start, count)
+            return
         ops.paged_append(self.desc(), layer, k, v, start, count)
 
     def attend(self, layer: int, q: torch.Tensor, start: torch.Tensor, max_len: int,
                out: Optional[torch.Tensor] = None, count: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Causal attention of q [batch, T, heads, d_head] at positions start[s]..;
-        count: the rows appended this forward when not all T (see append_layer)."""
+        count: the rows appended this forward when not all T (see append_layer).
+        An 8-bit cache takes the queries of the rows that were just appended
+        (the same T, start and count), float32 or bfloat16."""
+        if self.fp8:
+            return ops.paged8_attention(self.desc(), layer, q, start, max_len, out, count)
         return ops.paged_attention(self.desc(), layer, q, start, max_len, self.chunk_keys, out, count)
+
+    def append_attend(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, start: torch.Tensor,
+                      max_len: int, count: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """append_layer, then attend: one layer's share of a forward."""
+        self.append_layer(layer, k, v, start, count)
+        return self.attend(layer, q, start, max_len, count=count)
+
+    def read_rows(self, layer: int, first: torch.Tensor, length: torch.Tensor, T: int):
+        """The values an 8-bit cache stands for: float32 k, v [batch, T, heads,
+        d_head] of positions first[s] .. first[s] + T - 1 (int32 [batch], on
+        the device); rows past length[s], the rows the sequence holds, are zero."""
+        if not self.fp8:
+            raise ValueError("read_rows() is the 8-bit cache's; use read()")
+        return ops.paged8_read(self.desc(), layer, first, length, T)
 
     def commit(self, counts: Sequence[int]) -> None:
         """Record that ``counts[s]`` rows were appended to every layer."""
-        self.n_tokens += np.asarray(counts, np.int64)[:, None]
+        cnt = np.asarray(counts, np.int64)[:, None]
+        self.n_tokens += cnt
+        if self.fp8:
+            self._written(np.where(cnt > 0, self.n_tokens, 0), slice(None))
 
     # ------------------------------------------------------------ reference protocol (batch 1 view)
     def append(self, layer: int, k, v, pos) -> None:                  # paged.py:120-128
@@ -232,8 +310,10 @@ class PagedKVCache:
         self._ensure_capacity(0, layer, T)
         self._upload()
         st = torch.tensor([start], dtype=torch.int32, device=self.device)
-        ops.paged_append(self.desc(), layer, k.float().contiguous()[None], v.float().contiguous()[None], st)
+        self.append_layer(layer, k.float().contiguous()[None], v.float().contiguous()[None], st)
         self.n_tokens[0, layer] += T
+        if self.fp8:
+            self._written(self.n_tokens[:, layer], layer)
 
     def read(self, layer: int, seq: int = 0):                          # paged.py:130-138
         n = int(self.n_tokens[seq, layer])
@@ -241,6 +321,14 @@ class PagedKVCache:
             z = np.zeros((0, self.n_heads, self.d_head), np.float32)
             return z, z.copy(), np.zeros(0, np.int64)
         H, D, bs = self.n_heads, self.d_head, self.block_size
+        if self.fp8:   # the one sequence's part of the cache
+            d = self.desc()
+            d.batch = 1
+            d.block_table += 4 * seq * self.n_layers * self.max_blocks
+            d.tail += seq * self.tail[0].numel()
+            at = torch.tensor([0, n], dtype=torch.int32, device=self.device)
+            k, v = ops.paged8_read(d, layer, at[:1], at[1:], n)
+            return k[0].cpu().numpy(), v[0].cpu().numpy(), np.arange(n, dtype=np.int64)
         nb = -(-n // bs)
         phys = self.tables[seq, layer, :nb].astype(np.int64) + seq * self.n_blocks
         blocks = self.store[torch.from_numpy(phys).to(self.device)].float().cpu().numpy()
@@ -258,6 +346,14 @@ class PagedKVCache:
         changed = keep != self.n_tokens
         if not changed.any():
             return
+        if self.fp8:
+            lost = changed & (keep % self.block_size != 0) & (keep // self.block_size * self.block_size < self.tail_from)
+            if lost.any():
+                s, L = (int(x[0]) for x in np.nonzero(lost))
+                raise ValueError(f"sequence {s}: cannot cut {int(self.n_tokens[s, L])} rows to {int(keep[s, L])}: the "
+                                 f"bf16 rows of that block are gone (kept from {int(self.tail_from[s, L])} on; a multiple "
+                                 f"of block_size {self.block_size}, or a larger tail_rows, can)")
+            self.tail_from = np.where(changed, np.minimum(self.tail_from, keep), self.tail_from)
         self.n_tokens = np.where(changed, keep, self.n_tokens)
         need = np.where(changed, -(-keep // self.block_size), self.table_len)
         # emptied tail blocks go back per sequence, layer by layer, last first

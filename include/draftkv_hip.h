@@ -128,6 +128,69 @@ int dkv_paged_attention(const dkv_paged_t* cache, int32_t layer, const float* q,
                         int32_t max_len, int32_t chunk_keys, float* out, void* work,
                         size_t work_bytes, dkv_stream_t stream);
 
+/* ---------------------------------------------------------------- the full cache in 8 bits */
+/* The paged full cache held in 8 bits, with a power-of-two scale per block of
+ * tokens and head (no counterpart in the reference, whose full cache is
+ * float32, paged.py:76-176). A block of block_size (16, 32, 64 or 128) tokens
+ * is coded in e4m3 once all its rows are there; e is the least integer with
+ * max |x| <= 448 * 2^e over the block's finite K (V) values of the head,
+ * within -126 .. 119; NaN and infinities become NaN. A query at position p reads the blocks before
+ * its own in 8 bits and its own block's rows up to p in bf16, so its result
+ * is a function of rows 0..p alone, whatever rows share a call and however
+ * they were appended or rolled back.
+ * pool: blocks of dkv_paged8_block_bytes(), 16-byte aligned; block_table as in
+ * dkv_paged_t. tail: the last tail_rows rows in bf16 (a ring; a multiple of
+ * 16, at least block_size + 16), batch * n_layers * tail_rows *
+ * dkv_paged8_row_bytes() bytes. hot: batch * hot_rows * row bytes, used by
+ * calls whose rows do not fit the ring beside an open block
+ * (dkv_paged8_hot_rows(cache, T) > 0: hot_rows must be at least that); it is
+ * written by the append and read by the attention of the same layer that
+ * follows it on the stream. Rolling back: an append may start at any earlier
+ * position p that is a multiple of block_size, or whose block's rows are
+ * still in the ring (block start >= the rows ever written, rounded up to 16,
+ * minus tail_rows). head_dim 1..256. The layout inside blocks and rows is
+ * described in draft-kv_amd/csrc/paged8.h. */
+typedef struct {
+    void* pool;
+    const int32_t* block_table;
+    void* tail;
+    void* hot;
+    int32_t batch, n_layers, n_kv_heads, head_dim, block_size, max_blocks, tail_rows, hot_rows;
+} dkv_paged8_t;
+
+int64_t dkv_paged8_block_bytes(int32_t n_kv_heads, int32_t head_dim, int32_t block_size);
+int64_t dkv_paged8_row_bytes(int32_t n_kv_heads, int32_t head_dim);
+int32_t dkv_paged8_hot_rows(const dkv_paged8_t* cache, int32_t T);
+
+/* dkv_paged_append for this cache: same arguments. A sequence whose rows would
+ * lie outside its block table gets none (and no result from the attention:
+ * zeros). */
+int dkv_paged8_append(const dkv_paged8_t* cache, int32_t layer, const void* k, const void* v, int32_t in_dtype,
+                      int32_t T, const int32_t* start, const int32_t* count, dkv_stream_t stream);
+
+/* dkv_paged_attention for this cache, of the T rows per sequence that the
+ * append before it wrote (same T, start and count). q and out: DKV_F32 or
+ * DKV_BF16 (q_dtype both), [batch][T][Hq][D]. float32 queries and
+ * probabilities enter the products in three bf16 parts, bf16 queries whole
+ * and their probabilities rounded to bf16; sums are float32. Keys are cut
+ * at absolute positions into units of 256 and chunks of 2048 that fold in
+ * order, the query's own block last: a row's result depends neither on T nor
+ * on the launch. A padding row t >= count[s] sees what the last row does, and
+ * is zero where count[s] is 0. max_len bounds start + count of
+ * every sequence (it sizes the launch). work: dkv_paged8_attention_workspace()
+ * bytes, 16-byte aligned. */
+size_t dkv_paged8_attention_workspace(const dkv_paged8_t* cache, int32_t T, int32_t n_q_heads, int32_t max_len);
+int dkv_paged8_attention(const dkv_paged8_t* cache, int32_t layer, const void* q, int32_t q_dtype, int32_t T,
+                         int32_t n_q_heads, const int32_t* start, const int32_t* count, int32_t max_len, void* out,
+                         void* work, size_t work_bytes, dkv_stream_t stream);
+
+/* The values the cache stands for: rows first[s] .. first[s] + T - 1 of one
+ * layer as float32 k, v [batch][T][Hkv][D]; rows past the sequence's `length`
+ * are zero. Rows of sealed blocks come from their codes, the open block's
+ * from the ring. */
+int dkv_paged8_read(const dkv_paged8_t* cache, int32_t layer, const int32_t* first, const int32_t* length, int32_t T,
+                    float* k, float* v, dkv_stream_t stream);
+
 /* ------------------------------------------------------------ mirror append / evict */
 /* Quantize and append T rows per sequence to one layer of the mirror, then
  * evict down to budget[s] -- replaces draftkv/compress.py:122-133 (`append`)
@@ -166,6 +229,16 @@ int dkv_drafter_sync(const dkv_drafter_t* mirror, const dkv_paged_t* full, const
 int dkv_drafter_rebuild(const dkv_drafter_t* mirror, const dkv_paged_t* full,
                         const int32_t* layers, int32_t n_changed, const dkv_qcfg_t* cfgs,
                         const int32_t* len, const int32_t* budget, dkv_stream_t stream);
+
+/* dkv_drafter_sync / dkv_drafter_rebuild from a full cache in 8 bits: the rows
+ * are the values it stands for (sealed blocks' codes, the open block's bf16
+ * rows). */
+int dkv_drafter_sync_paged8(const dkv_drafter_t* mirror, const dkv_paged8_t* full, const dkv_qcfg_t* cfgs,
+                            const int32_t* start, const int32_t* end, const int32_t* budget,
+                            dkv_stream_t stream);
+int dkv_drafter_rebuild_paged8(const dkv_drafter_t* mirror, const dkv_paged8_t* full, const int32_t* layers,
+                               int32_t n_changed, const dkv_qcfg_t* cfgs, const int32_t* len,
+                               const int32_t* budget, dkv_stream_t stream);
 
 /* ---------------------------------------------------------------- drafter attention */
 /* Drafter attention: one query position per sequence over the live rows of
