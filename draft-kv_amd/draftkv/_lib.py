@@ -13,7 +13,7 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "_lib", "libdraftkv_hip.so")
 
-DKV_F32, DKV_BF16 = 0, 1
+DKV_F32, DKV_BF16, DKV_MX4 = 0, 1, 2
 DKV_GEMM_SWIGLU, DKV_GEMM_DEFER, DKV_GEMM_WTILED = 1, 2, 4
 DKV_ACT_SWIGLU, DKV_ACT_GELU, DKV_ACT_RELU = 1, 2, 3
 _ERRORS = {-1: ValueError, -2: RuntimeError, -3: MemoryError, -4: MemoryError}
@@ -95,6 +95,11 @@ _SIGS = {
     "dkv_gemm_bf16_workspace": (SZ, [I32, I32, I32]),
     "dkv_gemm_bf16_partials": (I32, [I32, I32, I32]),
     "dkv_gemm_bf16": (C.c_int, [P, I32, P, P, I32, I32, I32, P, I32, I32, P, SZ, P]),
+    "dkv_mx4_code_bytes": (I64, [I32, I32]),
+    "dkv_mx4_scale_bytes": (I64, [I32, I32]),
+    "dkv_mx4_quantize": (C.c_int, [P, I32, I32, I32, P, P, P, P]),
+    "dkv_mx4_values": (C.c_int, [P, P, I32, I32, P, P]),
+    "dkv_gemm_mx4": (C.c_int, [P, I32, P, P, P, P, I32, I32, I32, I32, P, I32, I32, P]),
     "dkv_last_error": (C.c_char_p, []),
     "dkv_version": (I32, []),
 }

@@ -120,6 +120,8 @@ class Decoder:
     def _proj(self, x: torch.Tensor, w: torch.Tensor, bias=None, defer: bool = False):
         """x @ W (+ bias); float32 out for float32 models, bf16 out for bf16 models
         (with ``defer``, possibly the bf16 GEMM's partials for a consumer that takes them)."""
+        if isinstance(w, ops.MX4):
+            return ops.gemm_mx4(x, w, bias, self.act_dtype)
         if self.wdtype == torch.float32:
             return ops.gemm_f32(x, w, self.layout, bias)
         return self._linear(x, w, bias, defer=defer)
@@ -136,7 +138,10 @@ class Decoder:
 
     def _residual(self, h: torch.Tensor, x: torch.Tensor, w: torch.Tensor, bias, nw, nb) -> torch.Tensor:
         """h += x @ W (+ bias), then return the next norm of h (weights nw, nb).
-        float32: the GEMM accumulates into h; bf16: the add is fused into the norm."""
+        float32: the GEMM accumulates into h; bf16 and 4-bit weights: the add is fused into the norm."""
+        if isinstance(w, ops.MX4):
+            return ops.add_norm(h, ops.gemm_mx4(x, w, out_dtype=self.act_dtype), bias, nw, nb, self.eps,
+                                self.norm == "layer", self.act_dtype)
         if self.wdtype == torch.float32:
             ops.gemm_f32(x, w, self.layout, bias, out=h, accumulate=True)
             return self._norm(h, nw, nb)
@@ -183,7 +188,29 @@ class Decoder:
             p.w1 = p.w1.view(2, ff2 // 2, k).transpose(0, 1).reshape(ff2, k).contiguous()
         self.gate_up_interleaved = True
 
+    def quantize_weights(self) -> None:
+        """Hold every projection of the layers in microscaled 4-bit floating
+        point (``ops.MX4``) from here on, in place of the weights: a quarter of
+        bf16's bytes, which is what a decode step streams. Embeddings, norms,
+        biases and the head stay. The activations of a product are rounded to
+        bf16; verify rows and one-token rows still agree bit for bit."""
+        inter = getattr(self, "gate_up_interleaved", False)
+        for p in self.layers:
+            for name in ("wqkv", "wo", "w1", "w2"):
+                w = getattr(p, name)
+                if isinstance(w, ops.MX4):
+                    continue
+                w = w.rows() if isinstance(w, ops.TiledW) else w.t() if self.w_layout == 0 else w
+                if name == "w1" and self.mlp == "swiglu" and not inter:   # rows (gate_0, up_0, gate_1, ...)
+                    w = w.reshape(2, w.shape[0] // 2, w.shape[1]).transpose(0, 1).reshape(w.shape)
+                setattr(p, name, ops.mx4_quantize(w.contiguous()))
+
     def _mlp_inner(self, x: torch.Tensor, p: Layer) -> torch.Tensor:
+        if isinstance(p.w1, ops.MX4):
+            if self.mlp == "swiglu":
+                return ops.gemm_mx4(x, p.w1, out_dtype=self.act_dtype, swiglu=True)
+            y = ops.gemm_mx4(x, p.w1, out_dtype=self.act_dtype)
+            return ops.bias_gelu(y, p.b1, self.act_dtype) if self.mlp == "gelu" else ops.relu(y, self.act_dtype)
         if self.wdtype == torch.float32:
             return ops.gemm_f32_act(x, p.w1, self.layout, self.mlp, p.b1 if self.mlp == "gelu" else None)
         if self.mlp == "swiglu":

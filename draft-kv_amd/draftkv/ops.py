@@ -12,7 +12,8 @@ from typing import Optional, Sequence
 import torch
 
 from . import _lib
-from ._lib import DKV_BF16, DKV_F32, DKV_GEMM_DEFER, DKV_GEMM_SWIGLU, DKV_GEMM_WTILED, Drafter, Paged, Paged8, QCfg, check, lib
+from ._lib import (DKV_BF16, DKV_F32, DKV_GEMM_DEFER, DKV_GEMM_SWIGLU, DKV_GEMM_WTILED, DKV_MX4, Drafter, Paged, Paged8,
+                   QCfg, check, lib)
 
 
 _get_device = getattr(torch._C, "_cuda_getDevice", None)
@@ -722,4 +723,88 @@ def gemm_bf16(x: torch.Tensor, w, bias: Optional[torch.Tensor] = None,
     check(lib().dkv_gemm_bf16(x.data_ptr(), _odt(x.dtype), w.data_ptr(), _ptr(bias), M, N, K, out.data_ptr(),
                               _odt(out_dtype), (DKV_GEMM_SWIGLU if swiglu else 0) | wflag,
                               _ptr(ws), 0 if ws is None else ws.numel(), _stream()), "dkv_gemm_bf16")
+    return out
+
+
+# ------------------------------------------------------------------ microscaled 4 bits
+class MX4:
+    """A matrix [rows, k] in microscaled 4-bit floating point (MXFP4: e2m1
+    codes, a power-of-two scale for each 32 values along k), stored in tiles
+    as the matrix instructions take them (csrc/mx4.hip). Made by
+    ``mx4_quantize``; ``values()`` gives the float32 matrix it stands for."""
+
+    __slots__ = ("codes", "scales", "shape")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape: tuple) -> None:
+        self.codes, self.scales, self.shape = codes, scales, shape
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    @property
+    def is_cuda(self) -> bool:
+        return self.codes.is_cuda
+
+    def nbytes(self) -> int:
+        return self.codes.numel() + self.scales.numel()
+
+    def values(self) -> torch.Tensor:
+        out = torch.empty(self.shape, dtype=torch.float32, device=self.device)
+        with _device(self.device):
+            check(lib().dkv_mx4_values(self.codes.data_ptr(), self.scales.data_ptr(), *self.shape, out.data_ptr(),
+                                       _stream()), "dkv_mx4_values")
+        return out
+
+
+def mx4_quantize(x: torch.Tensor, values: bool = False):
+    """x [rows, k] (float32 or bfloat16, any sizes) as ``MX4``; with
+    ``values`` also the float32 values it stands for: (MX4, values)."""
+    _need(x, "x", ndim=2)
+    dt = _dt(x)
+    rows, k = x.shape
+    if k < 1 or max(rows, k) >= 1 << 31:
+        raise ValueError(f"mx4_quantize: bad shape {tuple(x.shape)}")
+    codes = torch.empty(int(lib().dkv_mx4_code_bytes(rows, k)), dtype=torch.uint8, device=x.device)
+    scales = torch.empty(int(lib().dkv_mx4_scale_bytes(rows, k)), dtype=torch.uint8, device=x.device)
+    out = torch.empty((rows, k), dtype=torch.float32, device=x.device) if values else None
+    if rows:
+        with _device(x.device):
+            check(lib().dkv_mx4_quantize(x.data_ptr(), dt, rows, k, codes.data_ptr(), scales.data_ptr(), _ptr(out),
+                                         _stream()), "dkv_mx4_quantize")
+    q = MX4(codes, scales, (rows, k))
+    return (q, out) if values else q
+
+
+def gemm_mx4(x, w: MX4, bias: Optional[torch.Tensor] = None, out_dtype=torch.bfloat16, swiglu: bool = False) -> torch.Tensor:
+    """x [M, K] @ w[N, K]^T (+ bias), w in microscaled 4 bits; x a bfloat16
+    tensor, a float32 one (rounded to bfloat16 as it is read) or ``MX4`` too.
+    float32 accumulation, bfloat16 or float32 out; a row's result is the same
+    for any M. swiglu: w's rows interleave (gate_i, up_i) and the result is
+    silu(gate) * up, [M, N / 2] (no bias)."""
+    if not isinstance(w, MX4):
+        raise ValueError("gemm_mx4: w must be MX4 (mx4_quantize)")
+    if out_dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"gemm_mx4: unsupported out_dtype {out_dtype} (float32 or bfloat16)")
+    mx = isinstance(x, MX4)
+    if not mx:
+        _need(x, "x", ndim=2)
+    M, K = x.shape
+    N = w.shape[0]
+    if w.shape[1] != K or x.device != w.device:
+        raise ValueError(f"gemm_mx4: x {tuple(x.shape)} on {x.device} and w {tuple(w.shape)} on {w.device} disagree")
+    if bias is not None:
+        _need(bias, "bias", ndim=1)
+        if bias.shape[0] != N or bias.device != x.device:
+            raise ValueError(f"gemm_mx4: bias must be [{N}] on {x.device}, got {tuple(bias.shape)} on {bias.device}")
+    if swiglu and (bias is not None or N % 2):
+        raise ValueError("gemm_mx4: the SwiGLU epilogue takes no bias and needs an even N")
+    out = torch.empty((M, N // 2 if swiglu else N), dtype=out_dtype, device=x.device)
+    if M == 0 or N == 0:
+        return out
+    bp, bd = _bias(bias)
+    with _device(x.device):
+        check(lib().dkv_gemm_mx4(x.codes.data_ptr() if mx else x.data_ptr(), DKV_MX4 if mx else _dt(x),
+                                 x.scales.data_ptr() if mx else None, w.codes.data_ptr(), w.scales.data_ptr(), bp, bd, M, N, K,
+                                 out.data_ptr(), _odt(out_dtype), DKV_GEMM_SWIGLU if swiglu else 0, _stream()), "dkv_gemm_mx4")
     return out

@@ -447,6 +447,38 @@ int dkv_gemm_bf16(const void* x, int32_t x_dtype, const void* w, const void* bia
                   int32_t K, void* y, int32_t y_dtype, int32_t flags, void* work, size_t work_bytes,
                   dkv_stream_t stream);
 
+/* ------------------------------------------------------ microscaled 4-bit weights and rows */
+/* Microscaled 4-bit floating point (OCP MX 1.0, MXFP4; no counterpart in the
+ * reference, whose weights are float32): of every 32 values along k,
+ * e = floor(log2 max |x|) - 2 (0 where all are 0, at least -126) and codes
+ * e2m1(x * 2^-e), nearest even, saturating at 6; a block with a NaN or an
+ * infinity is NaN. Codes and scales lie in tiles of 16 rows x 128 k (the
+ * layout is described in draft-kv_amd/csrc/mx4.hip), rows past the last and
+ * columns past k as zeros: dkv_mx4_code_bytes() and dkv_mx4_scale_bytes()
+ * bytes, 16- and 4-byte aligned. Any rows and k.
+ * dkv_mx4_quantize: x [rows][k] float32 or bf16 to codes and scales, and to
+ * the values that they stand for (float32 [rows][k], or NULL).
+ * dkv_mx4_values: those values from codes and scales. */
+#define DKV_MX4 2   /* x_dtype of dkv_gemm_mx4 */
+int64_t dkv_mx4_code_bytes(int32_t rows, int32_t k);
+int64_t dkv_mx4_scale_bytes(int32_t rows, int32_t k);
+int dkv_mx4_quantize(const void* x, int32_t x_dtype, int32_t rows, int32_t k, uint8_t* codes, uint8_t* scales,
+                     float* values, dkv_stream_t stream);
+int dkv_mx4_values(const uint8_t* codes, const uint8_t* scales, int32_t rows, int32_t k, float* out,
+                   dkv_stream_t stream);
+/* y[M][N] = x[M][K] . w[N][K]^T (+ bias[N]), w in microscaled 4 bits. x is
+ * bf16, float32 (rounded to bf16, nearest even, as it is read), or DKV_MX4
+ * codes with x_scales (else NULL). float32 accumulation; y float32 or bf16
+ * (rounded once), 16-byte aligned; bias float32 or bf16 or NULL. flags:
+ * DKV_GEMM_SWIGLU: w's rows interleave (gate_i, up_i) and y[m][i] = silu(gate)
+ * * up of the float32 outputs, [M][N/2] (N even, no bias). K is cut into
+ * chunks fixed by (N, K) whose sums are added in order, so a row's result is
+ * the same for any M  -- the x @ W (+ b) products of the model forwards
+ * (model.py:113-133, gpt2.py:191-213, llama.py:187-225) */
+int dkv_gemm_mx4(const void* x, int32_t x_dtype, const uint8_t* x_scales, const uint8_t* w,
+                 const uint8_t* w_scales, const void* bias, int32_t bias_dtype, int32_t M, int32_t N, int32_t K,
+                 void* y, int32_t y_dtype, int32_t flags, dkv_stream_t stream);
+
 /* ---------------------------------------------------------------- misc */
 const char* dkv_last_error(void);
 int32_t dkv_version(void);
