@@ -16,6 +16,7 @@
 // Arithmetic. K is cut into S chunks of whole tiles, S a function of (N, K) only; a chunk is one chain of matrix
 // instructions in order, the chunks' sums are added in order, the bias last. A row's result is the same for any M.
 #include <algorithm>
+#include <initializer_list>
 
 #include "dkv_common.h"
 
@@ -184,6 +185,16 @@ __device__ __forceinline__ void mx_store(const MxArgs& A, int64_t m, int n, mx_f
 
 enum { MX_XF32, MX_XBF16, MX_XMX4 };
 
+// tile b of four of the 4-bit product: the scale bytes are selected by the instruction
+__device__ __forceinline__ mx_f32x4 mx_mfma4(mx_i32x8 w, mx_i32x8 x, mx_f32x4 c, int b, uint32_t sw, uint32_t sx) {
+    switch (b) {
+        case 0: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, 4, 4, 0, (int)sw, 0, (int)sx);
+        case 1: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, 4, 4, 1, (int)sw, 1, (int)sx);
+        case 2: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, 4, 4, 2, (int)sw, 2, (int)sx);
+        default: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, 4, 4, 3, (int)sw, 3, (int)sx);
+    }
+}
+
 // Grid (row fragment of W, group of MB 16-row tiles of x). One wave per chunk; the sums meet in LDS.
 template <int XM, int MB>
 __global__ void __launch_bounds__(512) mx4_gemm_kernel(MxArgs A) {
@@ -244,6 +255,316 @@ __global__ void __launch_bounds__(512) mx4_gemm_kernel(MxArgs A) {
         const int64_t m = m0 + 16 * i + col;
         if (m < A.M) mx_store(A, m, (int)f * 16 + 4 * q, t);
     }
+}
+
+// ---------------------------------------------------------------- product, many rows
+// One workgroup: BN rows of W x BM rows of x, in steps of one tile (128 k). The order of the workgroups gives each XCD
+// (workgroup g runs on XCD g % 8) one contiguous run of tiles, GM tiles of x by one of W at a time, so the 32 CUs of an
+// XCD share both in its L2.
+constexpr int MX_GM = 8;
+__device__ __forceinline__ bool mx_tile_of(int mtiles, int ntiles, int& mt, int& nt) {
+    const int groups = (mtiles + MX_GM - 1) / MX_GM, total = groups * MX_GM * ntiles, per = (total + 7) / 8;
+    const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= per || id >= total) return false;
+    const int grp = id / (MX_GM * ntiles), r = id % (MX_GM * ntiles);
+    mt = grp * MX_GM + r % MX_GM, nt = r / MX_GM;
+    return mt < mtiles;
+}
+__host__ inline unsigned mx_grid(int mtiles, int ntiles) {
+    const int total = (mtiles + MX_GM - 1) / MX_GM * MX_GM * ntiles;
+    return (unsigned)((total + 7) / 8 * 8);
+}
+
+// bf16 or float32 rows: four waves, NF fragments of W (16 NF rows) each, against the same 16 MB rows of x. W's codes go
+// from memory to registers a tile ahead and are converted there (a conversion per two values, a ninth of the matrix
+// instructions' time at NF x MB = 4 x 8); x goes through LDS, two stages. LDS holds x by rows of 16 pieces (8 values),
+// piece p of row r in slot p ^ (r % 16): a row's pieces arrive together, and the 16 rows that an operand read takes lie
+// on different banks. DMA: bf16 rows of whole tiles, straight to LDS; else through registers (rounding float32, zeros
+// past K).
+template <int XM, bool DMA, int NF, int MB, bool MULTI>
+__global__ void __launch_bounds__(256, 2) mx4_tile_kernel(MxArgs A, int mtiles, int ntiles) {
+#pragma clang fp contract(off)
+    constexpr int BM = 16 * MB, STAGE = BM * 256;
+    extern __shared__ __align__(16) char mx_smem[];   // [2][BM][16 slots] of 16 bytes
+    int mt, nt;
+    if (!mx_tile_of(mtiles, ntiles, mt, nt)) return;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / WAVE), lane = tid % WAVE;
+    const int col = lane % 16, q = lane / 16;
+    const int64_t m0 = (int64_t)mt * BM;
+    const int64_t frags = mx_frags(A.N), f0 = ((int64_t)nt * 4 + wave) * NF;
+    const mx_u32x4* wp[NF];
+    const uint32_t* sp[NF];
+#pragma unroll
+    for (int i = 0; i < NF; ++i) {
+        const int64_t f = min(f0 + i, frags - 1);
+        wp[i] = reinterpret_cast<const mx_u32x4*>(A.w + f * A.tiles * 1024) + lane;
+        sp[i] = A.ws + f * A.quads * 64 + lane;
+    }
+    // x piece i of this thread: row 4 (wave + 4 i) + lane / 16, slot lane % 16
+    auto x_row = [&](int i) { return 4 * (wave + 4 * i) + q; };
+    auto x_at = [&](int i, int t) {   // its offset in x
+        const int r = x_row(i);
+        return min(m0 + r, (int64_t)A.M - 1) * A.K + 128 * t + 8 * (col ^ (r & 15));
+    };
+    auto dma = [&](int t) {
+        const uint32_t base = lds_offset(mx_smem) + t % 2 * STAGE;
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+            dma_b128<false>(A.x, (uint32_t)(2 * x_at(i, t)), base + (wave + 4 * i) * 1024);
+    };
+    constexpr int HALF = (MB + 1) / 2;   // pieces through registers at once
+    mx_u32x4 xr[HALF];
+    auto x_load = [&](int t, int h) {
+#pragma unroll
+        for (int i = 0; i < HALF; ++i) {
+            const int p = h * HALF + i;
+            if (p >= MB) break;
+            const int r = x_row(p), k = 128 * t + 8 * (col ^ (r & 15));
+            xr[i] = __builtin_bit_cast(mx_u32x4, mx_x8<XM == MX_XF32>(A, min(m0 + r, (int64_t)A.M - 1), k));
+        }
+    };
+    auto x_store = [&](int t, int h) {
+#pragma unroll
+        for (int i = 0; i < HALF; ++i) {
+            const int p = h * HALF + i;
+            if (p < MB) *reinterpret_cast<mx_u32x4*>(mx_smem + t % 2 * STAGE + (wave + 4 * p) * 1024 + 16 * lane) = xr[i];
+        }
+    };
+    mx_f32x4 acc[NF][MB], tot[MULTI ? NF : 1][MULTI ? MB : 1];
+#pragma unroll
+    for (int i = 0; i < NF; ++i)
+#pragma unroll
+        for (int j = 0; j < MB; ++j) acc[i][j] = mx_f32x4{0.f, 0.f, 0.f, 0.f};
+    mx_u32x4 w[2][NF];
+    uint32_t sc[NF], sn[NF];
+    if constexpr (DMA) dma(0);
+    else {
+        x_load(0, 0);
+        x_store(0, 0);
+        x_load(0, 1);
+        x_store(0, 1);
+    }
+#pragma unroll
+    for (int i = 0; i < NF; ++i) {
+        w[0][i] = *wp[i];
+        sn[i] = *sp[i];
+    }
+    const int last = A.tiles - 1;
+    int left = A.CT;
+    for (int t0 = 0; t0 < A.tiles; t0 += 4) {
+#pragma unroll
+        for (int i = 0; i < NF; ++i) sc[i] = sn[i];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const int t = t0 + b;
+            if (t > last) break;   // uniform
+            wait_loads_barrier<0>();   // stage t % 2 is there, and every wave is done with the other
+            const int tn = min(t + 1, last);
+            if constexpr (DMA) {
+                if (t < last) dma(tn);
+            } else {
+                x_load(tn, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < NF; ++i) w[(b + 1) % 2][i] = wp[i][(int64_t)tn * 64];
+            if (b == 0) {
+                const int64_t qn = min(t0 / 4 + 1, A.quads - 1);
+#pragma unroll
+                for (int i = 0; i < NF; ++i) sn[i] = sp[i][qn * 64];
+            }
+            const char* xs = mx_smem + t % 2 * STAGE + col * 256;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (!DMA && j == 2 && t < last) {
+                    x_store(tn, 0);
+                    x_load(tn, 1);
+                }
+                mx_bf16x8 wv[NF];
+#pragma unroll
+                for (int i = 0; i < NF; ++i) wv[i] = mx_operand(w[b % 2][i][j], __uint_as_float((sc[i] >> 8 * b & 0xff) << 23));
+#pragma unroll
+                for (int m = 0; m < MB; ++m) {
+                    const mx_bf16x8 xv = *reinterpret_cast<const mx_bf16x8*>(xs + m * 4096 + ((4 * q + j) ^ col) * 16);
+#pragma unroll
+                    for (int i = 0; i < NF; ++i) acc[i][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv[i], xv, acc[i][m], 0, 0, 0);
+                }
+            }
+            if (!DMA && t < last) x_store(tn, 1);
+            if constexpr (MULTI) {
+                if (--left == 0 || t == last) {   // a chunk ends
+                    const bool first = t < A.CT;
+                    left = A.CT;
+#pragma unroll
+                    for (int i = 0; i < NF; ++i)
+#pragma unroll
+                        for (int m = 0; m < MB; ++m) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) tot[i][m][e] = first ? acc[i][m][e] : tot[i][m][e] + acc[i][m][e];
+                            acc[i][m] = mx_f32x4{0.f, 0.f, 0.f, 0.f};
+                        }
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NF; ++i)
+#pragma unroll
+        for (int m = 0; m < MB; ++m) {
+            const int64_t r = m0 + 16 * m + col;
+            if (r >= A.M || f0 + i >= frags) continue;
+            mx_f32x4 o;
+            if constexpr (MULTI) o = tot[i][m];
+            else o = acc[i][m];
+            mx_store(A, r, (int)(f0 + i) * 16 + 4 * q, o);
+        }
+}
+
+// 4-bit rows: eight waves, four along W by two along x, 4 x MB fragments each. Both operands' tiles go to LDS as they
+// are (1 KB, one load instruction each, two stages); the scale words straight to registers, once in four tiles. At
+// 4 x 8 a tile of 256 x 256 reads 32 KB per 1024 cycles of matrix instructions, half of what an XCD's L2 gives its CUs.
+template <int MB, bool MULTI>
+__global__ void __launch_bounds__(512, 2) mx4_tile4_kernel(MxArgs A, int mtiles, int ntiles) {
+#pragma clang fp contract(off)
+    constexpr int NF = 4, WF = 4 * NF, XF = 2 * MB, STAGE = (WF + XF) * 1024, PER = (WF + XF) / 8;
+    static_assert((WF + XF) % 8 == 0, "a stage's loads split evenly over the waves");
+    extern __shared__ __align__(16) char mx_smem[];   // [2][W fragments, x fragments][1 KB]
+    int mt, nt;
+    if (!mx_tile_of(mtiles, ntiles, mt, nt)) return;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), lane = threadIdx.x % WAVE;
+    const int col = lane % 16, q = lane / 16, wn = wave % 4, wm = wave / 4;
+    const int64_t frags = mx_frags(A.N), xfrags = mx_frags(A.M), f0 = (int64_t)nt * WF, x0 = (int64_t)mt * XF;
+    const char* src[PER];   // this wave's fragments of a stage: wave, wave + 8, ...
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int p = wave + 8 * i;
+        src[i] = p < WF ? reinterpret_cast<const char*>(A.w) + min(f0 + p, frags - 1) * A.tiles * 1024
+                        : static_cast<const char*>(A.x) + min(x0 + (p - WF), xfrags - 1) * A.tiles * 1024;
+    }
+    auto dma = [&](int t) {
+        const uint32_t base = lds_offset(mx_smem) + t % 2 * STAGE;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) dma_b128<false>(src[i] + (int64_t)t * 1024, 16 * lane, base + (wave + 8 * i) * 1024);
+    };
+    const uint32_t *wsp[NF], *xsp[MB];
+#pragma unroll
+    for (int i = 0; i < NF; ++i) wsp[i] = A.ws + min(f0 + wn * NF + i, frags - 1) * A.quads * 64 + lane;
+#pragma unroll
+    for (int m = 0; m < MB; ++m) xsp[m] = A.xs + min(x0 + wm * MB + m, xfrags - 1) * A.quads * 64 + lane;
+    mx_f32x4 acc[NF][MB], tot[MULTI ? NF : 1][MULTI ? MB : 1];
+#pragma unroll
+    for (int i = 0; i < NF; ++i)
+#pragma unroll
+        for (int j = 0; j < MB; ++j) acc[i][j] = mx_f32x4{0.f, 0.f, 0.f, 0.f};
+    uint32_t sw[NF], sx[MB], nw[NF], nx[MB];
+    dma(0);
+#pragma unroll
+    for (int i = 0; i < NF; ++i) nw[i] = *wsp[i];
+#pragma unroll
+    for (int m = 0; m < MB; ++m) nx[m] = *xsp[m];
+    const int last = A.tiles - 1;
+    int left = A.CT;
+    for (int t0 = 0; t0 < A.tiles; t0 += 4) {
+#pragma unroll
+        for (int i = 0; i < NF; ++i) sw[i] = nw[i];
+#pragma unroll
+        for (int m = 0; m < MB; ++m) sx[m] = nx[m];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const int t = t0 + b;
+            if (t > last) break;
+            wait_loads_barrier<0>();
+            if (t < last) dma(t + 1);
+            if (b == 0) {
+                const int64_t qn = min(t0 / 4 + 1, A.quads - 1);
+#pragma unroll
+                for (int i = 0; i < NF; ++i) nw[i] = wsp[i][qn * 64];
+#pragma unroll
+                for (int m = 0; m < MB; ++m) nx[m] = xsp[m][qn * 64];
+            }
+            const mx_u32x4* at = reinterpret_cast<const mx_u32x4*>(mx_smem + t % 2 * STAGE) + lane;
+            mx_i32x8 wv[NF];
+#pragma unroll
+            for (int i = 0; i < NF; ++i) {
+                const mx_u32x4 v = at[(wn * NF + i) * WAVE];
+                wv[i] = mx_i32x8{(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0};
+            }
+#pragma unroll
+            for (int m = 0; m < MB; ++m) {
+                const mx_u32x4 v = at[(WF + wm * MB + m) * WAVE];
+                const mx_i32x8 xv = {(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < NF; ++i) acc[i][m] = mx_mfma4(wv[i], xv, acc[i][m], b, sw[i], sx[m]);
+            }
+            if constexpr (MULTI) {
+                if (--left == 0 || t == last) {
+                    const bool first = t < A.CT;
+                    left = A.CT;
+#pragma unroll
+                    for (int i = 0; i < NF; ++i)
+#pragma unroll
+                        for (int m = 0; m < MB; ++m) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) tot[i][m][e] = first ? acc[i][m][e] : tot[i][m][e] + acc[i][m][e];
+                            acc[i][m] = mx_f32x4{0.f, 0.f, 0.f, 0.f};
+                        }
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NF; ++i)
+#pragma unroll
+        for (int m = 0; m < MB; ++m) {
+            const int64_t r = (x0 + wm * MB + m) * 16 + col, f = f0 + wn * NF + i;
+            if (r >= A.M || f >= frags) continue;
+            mx_f32x4 o;
+            if constexpr (MULTI) o = tot[i][m];
+            else o = acc[i][m];
+            mx_store(A, r, (int)f * 16 + 4 * q, o);
+        }
+}
+
+// 16-row tiles of x per workgroup, of the ones there are kernels for: the fewest rounds of 256 workgroups, by their
+// length (a tile of W costs about what one of x does)
+__host__ inline int mx_rows(int M, int64_t ntiles, std::initializer_list<int> mbs) {
+    int best = 0;
+    int64_t cost = 0;
+    for (const int mb : mbs) {
+        const int64_t wgs = (M + 16 * mb - 1) / (16 * mb) * ntiles, c = (wgs + 255) / 256 * (mb + 1);
+        if (!best || c < cost) best = mb, cost = c;
+    }
+    return best;
+}
+
+template <int XM, bool DMA, int MB, bool MULTI>
+static int mx_launch_tile(const MxArgs& a, hipStream_t st) {
+    const int mtiles = (a.M + 16 * MB - 1) / (16 * MB), ntiles = (int)((mx_frags(a.N) + 15) / 16);
+    hipLaunchKernelGGL((mx4_tile_kernel<XM, DMA, 4, MB, MULTI>), dim3(mx_grid(mtiles, ntiles)), dim3(256), 2 * 16 * MB * 256, st, a,
+                       mtiles, ntiles);
+    return DKV_OK;
+}
+template <int XM, bool DMA>
+static int mx_launch_rows(const MxArgs& a, hipStream_t st) {
+    const int64_t ntiles = (mx_frags(a.N) + 15) / 16;
+    if (a.S > 1)
+        switch (mx_rows(a.M, ntiles, {4, 2})) {
+            case 4: return mx_launch_tile<XM, DMA, 4, true>(a, st);
+            default: return mx_launch_tile<XM, DMA, 2, true>(a, st);
+        }
+    switch (mx_rows(a.M, ntiles, {8, 5, 4, 2})) {
+        case 8: return mx_launch_tile<XM, DMA, 8, false>(a, st);
+        case 5: return mx_launch_tile<XM, DMA, 5, false>(a, st);
+        case 4: return mx_launch_tile<XM, DMA, 4, false>(a, st);
+        default: return mx_launch_tile<XM, DMA, 2, false>(a, st);
+    }
+}
+template <int MB, bool MULTI>
+static int mx_launch_tile4(const MxArgs& a, hipStream_t st) {
+    const size_t lds = 2 * (16 + 2 * MB) * 1024;
+    auto fn = mx4_tile4_kernel<MB, MULTI>;
+    const int mtiles = (a.M + 32 * MB - 1) / (32 * MB), ntiles = (int)((mx_frags(a.N) + 15) / 16);
+    hipLaunchKernelGGL(fn, dim3(mx_grid(mtiles, ntiles)), dim3(512), lds, st, a, mtiles, ntiles);
+    return DKV_OK;
 }
 
 }  // namespace dkv
@@ -310,11 +631,28 @@ extern "C" int dkv_gemm_mx4(const void* x, int32_t x_dtype, const uint8_t* x_sca
     a.vec = K % 8 == 0 && aligned(x, 16);
     a.M = M, a.N = N, a.K = K, a.tiles = (int)mx_tiles(K), a.quads = (int)mx_quads(K), a.y = y;
     mx_chunks(N, K, a.S, a.CT);
+    hipStream_t st = as_stream(stream);
+    if (M > 64 && (x_dtype == DKV_MX4 || a.vec)) {
+        int rc;
+        if (x_dtype == DKV_MX4) {
+            const int64_t ntiles = (mx_frags(N) + 15) / 16;
+            // (rows of two waves: 32 MB)
+            if (a.S > 1) rc = mx_launch_tile4<4, true>(a, st);
+            else if (mx_rows((M + 1) / 2, ntiles, {8, 4}) == 8) rc = mx_launch_tile4<8, false>(a, st);
+            else rc = mx_launch_tile4<4, false>(a, st);
+        } else if (x_dtype == DKV_F32) {
+            rc = mx_launch_rows<MX_XF32, false>(a, st);
+        } else if (K % 128 == 0 && (int64_t)M * K < (1LL << 31)) {   // (32-bit byte offsets)
+            rc = mx_launch_rows<MX_XBF16, true>(a, st);
+        } else {
+            rc = mx_launch_rows<MX_XBF16, false>(a, st);
+        }
+        return rc ? rc : check_launch("dkv_gemm_mx4");
+    }
     const int mb = M <= 16 ? 1 : M <= 32 ? 2 : 4;
     const dim3 grid((unsigned)mx_frags(N), (unsigned)((M + 16 * mb - 1) / (16 * mb))), blk(64 * a.S);
     DKV_REQUIRE(grid.y <= 65535, "dkv_gemm_mx4: too many rows");
     const size_t lds = a.S > 1 ? (size_t)a.S * mb * 1024 : 0;
-    hipStream_t st = as_stream(stream);
 #define DKV_MX(XX)                                                                                    \
     do {                                                                                              \
         if (mb == 1) hipLaunchKernelGGL((mx4_gemm_kernel<XX, 1>), grid, blk, lds, st, a);             \
