@@ -99,7 +99,8 @@ _SIGS = {
     "dkv_mx4_scale_bytes": (I64, [I32, I32]),
     "dkv_mx4_quantize": (C.c_int, [P, I32, I32, I32, P, P, P, P]),
     "dkv_mx4_values": (C.c_int, [P, P, I32, I32, P, P]),
-    "dkv_gemm_mx4": (C.c_int, [P, I32, P, P, P, P, I32, I32, I32, I32, P, I32, I32, P]),
+    "dkv_gemm_mx4_workspace": (SZ, [P, I32, I32, I32, I32]),
+    "dkv_gemm_mx4": (C.c_int, [P, I32, P, P, P, P, I32, I32, I32, I32, P, I32, I32, P, SZ, P]),
     "dkv_last_error": (C.c_char_p, []),
     "dkv_version": (I32, []),
 }

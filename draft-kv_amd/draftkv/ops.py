@@ -803,8 +803,12 @@ def gemm_mx4(x, w: MX4, bias: Optional[torch.Tensor] = None, out_dtype=torch.bfl
     if M == 0 or N == 0:
         return out
     bp, bd = _bias(bias)
+    dt = DKV_MX4 if mx else _dt(x)
+    xp = x.codes.data_ptr() if mx else x.data_ptr()
     with _device(x.device):
-        check(lib().dkv_gemm_mx4(x.codes.data_ptr() if mx else x.data_ptr(), DKV_MX4 if mx else _dt(x),
-                                 x.scales.data_ptr() if mx else None, w.codes.data_ptr(), w.scales.data_ptr(), bp, bd, M, N, K,
-                                 out.data_ptr(), _odt(out_dtype), DKV_GEMM_SWIGLU if swiglu else 0, _stream()), "dkv_gemm_mx4")
+        nbytes = 0 if mx else lib().dkv_gemm_mx4_workspace(xp, dt, M, N, K)
+        ws = _WS.get(x.device, nbytes) if nbytes else None
+        check(lib().dkv_gemm_mx4(xp, dt, x.scales.data_ptr() if mx else None, w.codes.data_ptr(), w.scales.data_ptr(), bp, bd, M, N, K,
+                                 out.data_ptr(), _odt(out_dtype), DKV_GEMM_SWIGLU if swiglu else 0, _ptr(ws),
+                                 0 if ws is None else ws.numel(), _stream()), "dkv_gemm_mx4")
     return out

@@ -473,11 +473,15 @@ int dkv_mx4_values(const uint8_t* codes, const uint8_t* scales, int32_t rows, in
  * DKV_GEMM_SWIGLU: w's rows interleave (gate_i, up_i) and y[m][i] = silu(gate)
  * * up of the float32 outputs, [M][N/2] (N even, no bias). K is cut into
  * chunks fixed by (N, K) whose sums are added in order, so a row's result is
- * the same for any M  -- the x @ W (+ b) products of the model forwards
+ * the same for any M. work: dkv_gemm_mx4_workspace() bytes, 16-byte
+ * aligned (for float rows that are packed first: those of K % 8 != 0 or not
+ * 16-byte aligned, float32 ones past a few rows of a small w, more than 16 of
+ * K % 128 != 0; and for the chunks' sums of some narrow products)  -- the x @ W (+ b) products of the model forwards
  * (model.py:113-133, gpt2.py:191-213, llama.py:187-225) */
+size_t dkv_gemm_mx4_workspace(const void* x, int32_t x_dtype, int32_t M, int32_t N, int32_t K);
 int dkv_gemm_mx4(const void* x, int32_t x_dtype, const uint8_t* x_scales, const uint8_t* w,
                  const uint8_t* w_scales, const void* bias, int32_t bias_dtype, int32_t M, int32_t N, int32_t K,
-                 void* y, int32_t y_dtype, int32_t flags, dkv_stream_t stream);
+                 void* y, int32_t y_dtype, int32_t flags, void* work, size_t work_bytes, dkv_stream_t stream);
 
 /* ---------------------------------------------------------------- misc */
 const char* dkv_last_error(void);

@@ -79,7 +79,9 @@ def tol(x, w, dtype, want):
 
 
 SIZES = [(1, 16, 32), (1, 960, 576), (3, 17, 100), (16, 100, 128), (17, 64, 640), (33, 250, 1000), (64, 48, 4096), (65, 1030, 257),
-         (160, 512, 512), (130, 33, 2304), (300, 768, 768), (2, 5, 1), (1, 20000, 96), (70, 9000, 160)]
+         (160, 512, 512), (130, 33, 2304), (300, 768, 768), (2, 5, 1), (4096, 1021, 384), (200, 4099, 512), (90, 16390, 256), (700, 257, 128), (1, 20000, 96), (70, 9000, 160),
+         (1, 64, 640), (12, 90, 200), (20, 100, 4224), (100, 130, 10112), (30, 8200, 256), (50, 8210, 130), (2100, 4099, 640), (330, 16402, 256),
+         (250, 33002, 384), (640, 33002, 256), (300, 49000, 128)]
 
 
 @pytest.mark.gpu
@@ -250,7 +252,7 @@ def test_bad_calls_are_refused():
     good = dict(x=16, xd=0, xs=None, w=16, ws=16, b=None, bd=0, M=4, N=16, K=32, y=16, yd=0, fl=0)
 
     def gemm(**kw):
-        return L.dkv_gemm_mx4(*{**good, **kw}.values(), None)
+        return L.dkv_gemm_mx4(*{**good, **kw}.values(), None, 0, None)
 
     for kw, word in ((dict(x=None), "NULL"), (dict(w=None), "NULL"), (dict(ws=None), "NULL"), (dict(y=None), "NULL"), (dict(xd=3), "dtype"),
                      (dict(xd=2), "scales"), (dict(yd=2), "dtype"), (dict(b=16, bd=2), "bias"), (dict(N=0), "shape"), (dict(K=0), "shape"),
@@ -258,6 +260,8 @@ def test_bad_calls_are_refused():
                      (dict(w=24), "aligned"), (dict(ws=18), "aligned"), (dict(y=24), "aligned"), (dict(xd=2, xs=16, x=20), "aligned")):
         err(gemm(**kw), word)
     assert gemm(M=0) == 0
+    assert gemm(M=5) == -3 and "workspace" in L.dkv_last_error().decode()
+    assert L.dkv_gemm_mx4_workspace(16, 0, 65, 16, 32) == 65 * 256 and L.dkv_gemm_mx4_workspace(16, 1, 65, 16, 128) == 0
     assert L.dkv_mx4_code_bytes(17, 129) == 2 * 2 * 1024 and L.dkv_mx4_scale_bytes(17, 513) == 2 * 2 * 256
 
 
@@ -280,14 +284,17 @@ def test_bad_tensors_are_refused():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("M,N,K", [(16, 100, 128), (3, 17, 100), (130, 36, 64), (40, 1028, 256)])
+@pytest.mark.parametrize("M,N,K", [(16, 100, 128), (3, 17, 100), (130, 36, 64), (40, 1028, 256), (50, 260, 2048), (20, 102, 4200), (12, 50, 4100)])
 def test_nothing_is_written_past_the_outputs(dev, M, N, K):
     from draftkv import _lib, ops
     q = ops.mx4_quantize(torch.randn(N, K, device=dev))
     x = torch.randn(M, K, device=dev)
     y = torch.full((M * N + 4096,), 5.0, device=dev)
+    n = _lib.lib().dkv_gemm_mx4_workspace(x.data_ptr(), 0, M, N, K)
+    ws = torch.full((n + 4096,), 7, dtype=torch.uint8, device=dev)
     _lib.check(_lib.lib().dkv_gemm_mx4(x.data_ptr(), 0, None, q.codes.data_ptr(), q.scales.data_ptr(), None, 0, M, N, K, y.data_ptr(),
-                                       0, 0, torch.cuda.current_stream().cuda_stream), "dkv_gemm_mx4")
+                                       0, 0, ws.data_ptr(), n, torch.cuda.current_stream().cuda_stream), "dkv_gemm_mx4")
+    assert (ws[n:] == 7).all()
     assert (y[M * N:] == 5.0).all() and torch.equal(y[: M * N].view(M, N), ops.gemm_mx4(x, q, out_dtype=F32))
     codes = torch.full((q.codes.numel() + 4096,), 9, dtype=torch.uint8, device=dev)
     scales = torch.full((q.scales.numel() + 4096,), 9, dtype=torch.uint8, device=dev)
