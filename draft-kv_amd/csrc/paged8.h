@@ -99,8 +99,6 @@ __device__ __forceinline__ float p8_value(const dkv_paged8_t& c, int s, int laye
     return bf16_to_f32(__builtin_bit_cast(uint32_t, v) & 0xffff);
 }
 
-__device__ __forceinline__ float p8_load(const float* p, int64_t i) { return p[i]; }
-__device__ __forceinline__ float p8_load(const uint16_t* p, int64_t i) { return bf16_to_f32(p[i]); }
 
 int p8_check(const dkv_paged8_t* c, int layer, const char* fn);
 int p8_check_hot(const dkv_paged8_t& c, int T, const char* fn);

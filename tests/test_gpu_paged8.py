@@ -114,6 +114,30 @@ def test_append_codes_full_blocks(dev, bs, D, H, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("bs,tail,D", [(64, 96, 40), (16, 32, 64), (32, 112, 24)])
+def test_long_appends_wrap_around_the_tail(dev, bs, tail, D):
+    """An append of more rows than the tail holds, begun inside a block: its codes come from the rows that were there and
+    the new ones, and the tail then holds the last rows, those of the block before the last one too."""
+    g = torch.Generator(device=dev)
+    g.manual_seed(bs)
+    for s0 in (1, 5, bs - 1, bs, bs + 17, 2 * bs + 3):
+        for T in range(tail - bs + 2, tail + 2 * bs + 40, 11):
+            n = s0 + T
+            k, v = rows_of(g, 1, n, 2, D, dev)
+            c = new_cache(2, D, bs, n, tail_rows=tail)
+            for lo, hi in ((0, s0), (s0, n)):
+                c.reserve([hi - lo])
+                c.append_layer(0, k[:, lo:hi].contiguous(), v[:, lo:hi].contiguous(), i32([lo]))
+                c.commit([hi - lo])
+            for cut in (n, n - 1, n - n % bs - 1):
+                if cut < 1 or cut // bs * bs < -(-n // 16) * 16 - tail:
+                    continue
+                gk, gv = c.read_rows(0, i32([0]), i32([cut]), cut)
+                for got, x in ((gk, k), (gv, v)):
+                    assert torch.equal(got[0].double().cpu(), values(x[0, :cut].to(BF16).cpu(), bs)), (s0, T, cut)
+
+
+@pytest.mark.gpu
 def test_append_values_that_are_not_finite(dev):
     """NaN and infinities become NaN codes and do not count for the scale; the smallest and largest magnitudes hold."""
     bs, H, D = 16, 1, 32
