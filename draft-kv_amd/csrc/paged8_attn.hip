@@ -48,7 +48,7 @@ struct P8Args {
     float2* ml;              // (m, l) [row][n_chunks + 1]
     void* out;
     bool vec;                // rows of q and out in whole, 16-byte aligned runs of 8
-    bool direct;             // the walking kernel covers every key: it writes out itself
+    bool direct;             // each row's keys all lie in one workgroup, which writes out itself
 };
 
 // The rows of a workgroup's (sequence, KV head): row r is step r / G, query head h G + r % G.
@@ -556,7 +556,9 @@ __host__ __device__ constexpr size_t p8_chunk_lds(int dp, int nq, int ns) {
 }
 // Grid (KV head x sequence, q-group, run of chunks or own blocks). Eight waves, one unit of a chunk each, straight from
 // memory to registers; their states meet in LDS and leave as the chunk's.
-template <int DP, int NQ, int NS>
+// ONE: all keys lie in one chunk, and the workgroup takes the rows' own blocks too (its last wave, which few contexts
+// give a unit) and writes out: the merge would cost as much again as a short context's attention.
+template <int DP, int NQ, int NS, bool ONE>
 __global__ void __launch_bounds__(512) paged8_chunk_kernel(P8Args A) {
     constexpr int NDT = DP / 16, SETS = DP <= 64 || NQ == 1 ? 2 : 1;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), lane = threadIdx.x % WAVE;
@@ -569,9 +571,9 @@ __global__ void __launch_bounds__(512) paged8_chunk_kernel(P8Args A) {
     int lim0, lim1;
     R.pos(r0, bs, lim0);                                               // the least and the largest of the rows'
     const int last1 = R.pos(r0 + 16 * NQ - 1, bs, lim1);
-    const bool own = blockIdx.z == gridDim.z - 1;                      // this workgroup takes the rows' own blocks
+    const bool own = !ONE && blockIdx.z == gridDim.z - 1;              // this workgroup takes the rows' own blocks
     const int ch0 = blockIdx.z * A.per_slot;
-    const int ch1 = own ? ch0 + 1 : min(min(ch0 + A.per_slot, A.n_chunks), (lim1 + P8_CHUNK - 1) / P8_CHUNK);
+    const int ch1 = ONE || own ? ch0 + 1 : min(min(ch0 + A.per_slot, A.n_chunks), (lim1 + P8_CHUNK - 1) / P8_CHUNK);
     if (ch0 >= ch1) return;
     extern __shared__ __align__(16) char p8_lds[];
     constexpr bool QL = p8_query_in_lds(DP, NQ, NS);
@@ -591,6 +593,59 @@ __global__ void __launch_bounds__(512) paged8_chunk_kernel(P8Args A) {
     }
     st.load_limits(A, R, r0, lane);
     if (!own && k0 < lim1) u.template open<DP>(A, R, k0, min(k0 + P8_UNIT, lim1), lane);
+    auto leave = [&](int slot) {   // this wave's state
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+            if (lane < 16) sml[(slot * NQ + i) * 16 + lane] = make_float2(st.m[i], st.l[i]);
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt) so[((slot * NQ + i) * NDT + dt) * WAVE + lane] = st.acc[i][dt];
+        }
+    };
+    // d-tile x / 64 (of all q-tiles), lane x % 64 of the sums: slots 0 .. n - 1 in order behind (m, l, o)
+    auto fold = [&](int x, int n, float& m, float& l, p8_f32x4& o) {
+        for (int w = 0; w < n; ++w) {
+            const float2 ml = sml[(w * NQ + x / WAVE / NDT) * 16 + x % 16];
+            const p8_f32x4 ou = so[w * NQ * NDT * WAVE + x];
+            float a, b;
+            m = fold_max(m, ml.x, a, b);
+            l = fold_sum(l, a, ml.y, b);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = fold_sum(o[e], a, ou[e], b);
+        }
+    };
+    if constexpr (ONE) {
+        const int units = (lim1 + P8_UNIT - 1) / P8_UNIT;
+        if (wave < units) {
+            st.clear();
+            st.template unit<SETS>(A, u, k0, min(k0 + P8_UNIT, lim1), lim0, lane);
+            leave(wave);
+        }
+        if (wave == P8_UNITS - 1) {
+            st.clear();
+            st.own_blocks(A, R, lim0, last1, lane);
+        }
+        __syncthreads();
+        constexpr int NI = (NQ * NDT * WAVE + 511) / 512;
+        float m[NI], l[NI];
+        p8_f32x4 o[NI];
+#pragma unroll
+        for (int y = 0; y < NI; ++y) {
+            const int x = threadIdx.x + 512 * y;
+            m[y] = -INFINITY, l[y] = 0.0f, o[y] = p8_f32x4{0.f, 0.f, 0.f, 0.f};
+            if (x < NQ * NDT * WAVE) fold(x, units, m[y], l[y], o[y]);
+        }
+        __syncthreads();
+        if (wave == P8_UNITS - 1) leave(0);
+        __syncthreads();
+#pragma unroll
+        for (int y = 0; y < NI; ++y) {
+            const int x = threadIdx.x + 512 * y, r = r0 + 16 * (x / WAVE / NDT) + x % 16;
+            if (x >= NQ * NDT * WAVE || r >= R.n_rows) continue;
+            fold(x, 1, m[y], l[y], o[y]);
+            p8_store_out<NS>(A, R.row(r, A.Hq), x / WAVE % NDT * 16 + x % WAVE / 16 * 4, o[y], l[y]);
+        }
+        return;
+    }
     for (int ch = ch0; ch < ch1; ++ch, k0 += P8_CHUNK) {
         const int units = own ? 1 : min(P8_UNITS, (lim1 - ch * P8_CHUNK + P8_UNIT - 1) / P8_UNIT);
         if (wave < units) {
@@ -604,28 +659,15 @@ __global__ void __launch_bounds__(512) paged8_chunk_kernel(P8Args A) {
                 nu.template open<DP>(A, R, n0, n1, lane);
                 u = nu;
             }
-#pragma unroll
-            for (int i = 0; i < NQ; ++i) {
-                if (lane < 16) sml[(wave * NQ + i) * 16 + lane] = make_float2(st.m[i], st.l[i]);
-#pragma unroll
-                for (int dt = 0; dt < NDT; ++dt) so[((wave * NQ + i) * NDT + dt) * WAVE + lane] = st.acc[i][dt];
-            }
+            leave(wave);
         }
         __syncthreads();
-        for (int x = threadIdx.x; x < NQ * NDT * WAVE; x += 512) {   // d-tile x / 64 (of all q-tiles), lane x % 64 of the sums
-            const int ln = x % WAVE, col = ln % 16, i = x / WAVE / NDT, r = r0 + 16 * i + col;
+        for (int x = threadIdx.x; x < NQ * NDT * WAVE; x += 512) {
+            const int ln = x % WAVE, r = r0 + 16 * (x / WAVE / NDT) + ln % 16;
             if (r >= R.n_rows) continue;
             float m = -INFINITY, l = 0.0f;
             p8_f32x4 o = {0.f, 0.f, 0.f, 0.f};
-            for (int w = 0; w < units; ++w) {
-                const float2 ml = sml[(w * NQ + i) * 16 + col];
-                const p8_f32x4 ou = so[w * NQ * NDT * WAVE + x];
-                float a, b;
-                m = fold_max(m, ml.x, a, b);
-                l = fold_sum(l, a, ml.y, b);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = fold_sum(o[e], a, ou[e], b);
-            }
+            fold(x, units, m, l, o);
             const int64_t slot = R.row(r, A.Hq) * (A.n_chunks + 1) + (own ? A.n_chunks : ch);
             const int dt = x / WAVE % NDT;
             *reinterpret_cast<p8_f32x4*>(A.part + slot * DP + dt * 16 + ln / 16 * 4) = o;
@@ -918,8 +960,8 @@ static P8Plan p8_plan(const dkv_paged8_t& c, int T, int Hq, int max_len, int ns)
     p.n_chunks = (max_len + P8_CHUNK - 1) / P8_CHUNK;
     p.nq = tiles > 1 && dp <= 128 ? 2 : 1;
     p.walk = tiles > p.nq;
-    p.slots = 1, p.per_slot = p.n_chunks, p.direct = p.walk;
-    if (!p.walk) {
+    p.slots = 1, p.per_slot = p.n_chunks, p.direct = p.walk || p.n_chunks == 1;
+    if (!p.walk && !p.direct) {
         // a run of chunks per workgroup: about four workgroups per CU, as many as its chunks give
         const int64_t wgs = (tiles + p.nq - 1) / p.nq * c.n_kv_heads * c.batch;
         p.per_slot = (int)std::max<int64_t>(1, p.n_chunks * wgs / 1024);
@@ -955,24 +997,25 @@ static int p8_launch_walk(P8Args& a, const P8Plan& p, int64_t tiles, hipStream_t
     return DKV_OK;
 }
 
-template <int DP, int NQ, int NS>
+template <int DP, int NQ, int NS, bool ONE>
 static int p8_launch_chunk(P8Args& a, const P8Plan& p, int64_t tiles, hipStream_t st) {
     const size_t lds = p8_chunk_lds(DP, NQ, NS);
-    auto fn = paged8_chunk_kernel<DP, NQ, NS>;
+    auto fn = paged8_chunk_kernel<DP, NQ, NS, ONE>;
     static size_t done[16] = {};
     if (!reserve_lds(reinterpret_cast<const void*>(fn), lds, done))
         return fail(DKV_ELAUNCH, "dkv_paged8_attention: cannot reserve " + std::to_string(lds) + " B of LDS");
-    hipLaunchKernelGGL(fn, dim3(a.c.n_kv_heads * a.c.batch, (int)((tiles + NQ - 1) / NQ), p.slots + 1), dim3(512), lds, st, a);
+    hipLaunchKernelGGL(fn, dim3(a.c.n_kv_heads * a.c.batch, (int)((tiles + NQ - 1) / NQ), ONE ? 1 : p.slots + 1), dim3(512), lds, st, a);
     return DKV_OK;
 }
 
 template <int DP, int NS>
 static int p8_launch(P8Args& a, const P8Plan& p, hipStream_t st) {
     const int64_t tiles = ((int64_t)a.T * (a.Hq / a.c.n_kv_heads) + 15) / 16;
+    constexpr int NQ2 = DP <= 128 ? 2 : 1;   // (wider heads never have two)
     int rc;
     if (p.walk) rc = p8_launch_walk<DP, NS>(a, p, tiles, st);
-    else if (p.nq == 1) rc = p8_launch_chunk<DP, 1, NS>(a, p, tiles, st);
-    else rc = p8_launch_chunk<DP, DP <= 128 ? 2 : 1, NS>(a, p, tiles, st);
+    else if (p.nq == 1) rc = p.direct ? p8_launch_chunk<DP, 1, NS, true>(a, p, tiles, st) : p8_launch_chunk<DP, 1, NS, false>(a, p, tiles, st);
+    else rc = p.direct ? p8_launch_chunk<DP, NQ2, NS, true>(a, p, tiles, st) : p8_launch_chunk<DP, NQ2, NS, false>(a, p, tiles, st);
     if (rc || (rc = check_launch("dkv_paged8_attention")) || p.direct) return rc;
     const int64_t rows = (int64_t)a.c.batch * a.T * a.Hq;
     hipLaunchKernelGGL((paged8_merge_kernel<DP, NS>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);

@@ -174,6 +174,8 @@ class PagedKVCache:
 
     def _hot_room(self, T: int) -> None:
         """Room for an append of T rows that the tail does not hold beside an open block."""
+        if (self.block_size + T + 14) // 16 * 16 <= self.tail_rows:
+            return
         need = int(lib().dkv_paged8_hot_rows(self.desc(), T))
         if need > self.hot.shape[1]:
             if torch.cuda.is_current_stream_capturing():
@@ -275,6 +277,11 @@ class PagedKVCache:
     def append_attend(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, start: torch.Tensor,
                       max_len: int, count: Optional[torch.Tensor] = None) -> torch.Tensor:
         """append_layer, then attend: one layer's share of a forward."""
+        if self.fp8:
+            self._hot_room(k.shape[1])
+            d = self.desc()
+            ops.paged8_append(d, layer, k, v, start, count)
+            return ops.paged8_attention(d, layer, q, start, max_len, None, count)
         self.append_layer(layer, k, v, start, count)
         return self.attend(layer, q, start, max_len, count=count)
 
