@@ -953,13 +953,46 @@ struct P8Plan {
 __host__ constexpr int p8_walk_waves(int dp) { return dp > 128 ? 4 : 8; }
 __host__ constexpr int p8_walk_tiles(int dp, int ns) { return dp > 128 || ns > 1 ? 1 : 2; }
 
+// Which kernel, where either could take the rows: the one that a model of their times says is faster. A workgroup that
+// streams a chunk needs `full` us for its 2048 keys where every CU has one, and `base` however few keys it has (half of
+// that where CUs stay free); a walking one, of many more rows, 12 us and `step` per 32 keys. Measured, streaming against
+// walking, us: 32 / 8 heads of 128, bf16, one sequence: 400 rows on no context 21 / 33, 1600 rows 84 / 89; on 2000 keys
+// 100 rows 24 / 104, 400 rows 62 / 110, 1600 rows 215 / 174; four sequences, 400 rows on 2000 keys 202 / 137. 9 / 3
+// heads of 64, float32: 50 rows on 8000 keys 27 / 71, 800 rows 112 / 98.
+static bool p8_walks(const dkv_paged8_t& c, int64_t tiles, int T, int max_len, int nq, int slots, int per_slot, int ns) {
+    const int dp = p8_dp(c.head_dim), at = dp == 32 ? 0 : dp / 64;
+    static const float base[2][5] = {{9, 12, 13, 14, 20}, {14, 23, 20, 18, 33}}, full[2][5] = {{12, 16, 33, 24, 37}, {19, 30, 42, 24, 59}},
+                       step[2][5] = {{.8f, .9f, 1.45f, 1.f, 1.2f}, {.7f, .9f, 1.45f, 1.45f, 2.2f}};
+    const int64_t heads = (int64_t)c.n_kv_heads * c.batch, groups = (tiles + nq - 1) / nq;
+    if (groups > 65535) return true;
+    const float keys = (float)std::max(1, max_len - T / 2), chunks = keys / P8_CHUNK;   // of a row, on average
+    const float f = full[ns > 1][at] * chunks, b = base[ns > 1][at];
+    const float stream = std::max(std::min(std::max(f, b / 2), full[ns > 1][at]), groups * heads * std::max(f, b) / 256.0f);
+    const int per = p8_walk_waves(dp) * p8_walk_tiles(dp, ns);
+    const int64_t wgs = (tiles + per - 1) / per * heads * slots;
+    const float longest = (float)std::min<int64_t>(max_len, (int64_t)per_slot * P8_CHUNK);
+    const float walk = 12.0f + step[ns > 1][at] / 32.0f * std::max(longest, (float)((wgs + 255) / 256) * keys / slots);
+    return walk < stream;
+}
+
 static P8Plan p8_plan(const dkv_paged8_t& c, int T, int Hq, int max_len, int ns) {
     P8Plan p = {};
     const int dp = p8_dp(c.head_dim);
     const int64_t rows = (int64_t)T * (Hq / c.n_kv_heads), tiles = (rows + 15) / 16;
     p.n_chunks = (max_len + P8_CHUNK - 1) / P8_CHUNK;
     p.nq = tiles > 1 && dp <= 128 ? 2 : 1;
-    p.walk = tiles > p.nq;
+    // slots of a walk: where its workgroups are too few for 256 CUs, the chunks go to several, their states through memory
+    int slots = 1, per_slot = p.n_chunks;
+    {
+        const int per = p8_walk_waves(dp) * p8_walk_tiles(dp, ns);
+        const int64_t wgs = (tiles + per - 1) / per * c.n_kv_heads * c.batch;
+        if (wgs < 256 && p.n_chunks > 1) {
+            slots = (int)std::min<int64_t>(p.n_chunks, (512 + wgs - 1) / wgs);
+            per_slot = (p.n_chunks + slots - 1) / slots;
+            slots = (p.n_chunks + per_slot - 1) / per_slot;
+        }
+    }
+    p.walk = tiles > p.nq && p8_walks(c, tiles, T, max_len, p.nq, slots, per_slot, ns);
     p.slots = 1, p.per_slot = p.n_chunks, p.direct = p.walk || p.n_chunks == 1;
     if (!p.walk && !p.direct) {
         // a run of chunks per workgroup: about four workgroups per CU, as many as its chunks give
@@ -969,15 +1002,8 @@ static P8Plan p8_plan(const dkv_paged8_t& c, int T, int Hq, int max_len, int ns)
     }
     if (p.walk) {
         p.nq = p8_walk_tiles(dp, ns);
-        const int per = p8_walk_waves(dp) * p.nq;
-        const int64_t wgs = (tiles + per - 1) / per * c.n_kv_heads * c.batch;
-        // too few workgroups for 256 CUs: the chunks go to several, and their states through memory
-        if (wgs < 256 && p.n_chunks > 1) {
-            p.direct = false;
-            p.slots = (int)std::min<int64_t>(p.n_chunks, (512 + wgs - 1) / wgs);
-            p.per_slot = (p.n_chunks + p.slots - 1) / p.slots;
-            p.slots = (p.n_chunks + p.per_slot - 1) / p.per_slot;
-        }
+        p.direct = slots == 1;
+        p.slots = slots, p.per_slot = per_slot;
     }
     if (!p.direct) p.bytes = (size_t)c.batch * T * Hq * (p.n_chunks + 1) * (dp + 2) * sizeof(float);
     return p;

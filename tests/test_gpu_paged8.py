@@ -239,6 +239,49 @@ def test_rows_do_not_depend_on_the_call(dev, D, H, G, bs, n, dtype):
         at, step = at + T, step + 1
 
 
+# D, KV heads, query heads per KV head, block, rows that are there, new rows: prompts enough to fill the chip, and long ones
+# of few sequences, whose keys several workgroups share
+PROMPTS = [
+    (128, 2, 8, 16, [0, 7, 30, 16, 100, 33], 300), (64, 2, 16, 32, [0, 7, 30, 16, 3, 2, 1, 31], 200), (16, 4, 16, 16, [20, 7, 1, 16, 3, 2, 0, 0], 300),
+    (192, 2, 8, 64, [0, 7, 70, 64, 3, 2, 1, 129], 300), (256, 2, 8, 16, [0, 7, 30, 16, 3, 15], 200), (16, 4, 16, 16, [1700, 0, 2000, 1999], 200),
+    (64, 2, 16, 16, [1700, 0, 3000, 2049], 200), (64, 1, 16, 128, [1700, 0, 3000, 2049], 200), (128, 2, 16, 16, [1700, 0, 2000, 1999], 200),
+    (128, 1, 16, 64, [3000], 800), (192, 1, 16, 16, [2000], 800), (256, 1, 16, 16, [3000], 400), (256, 1, 8, 32, [3001], 800),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shape", PROMPTS, ids=lambda s: f"d{s[0]}h{s[1]}x{s[2]}b{s[3]}t{s[5]}n{s[4][-1]}")
+def test_prompts_equal_calls_of_a_few_rows(dev, shape, dtype):
+    """Bit for bit, in every sequence, with values that are not finite in two of them; the last one's rows end early."""
+    D, H, G, bs, have, T = shape
+    b, m = len(have), max(have) + T
+    g = torch.Generator(device=dev)
+    g.manual_seed(D + T + b)
+    k, v = rows_of(g, b, m, H, D, dev)
+    for s, bad in ((0, have[0] + T // 2), (b // 2, have[b // 2] + T // 3)):
+        k[s, bad, 0, 3], v[s, bad + 20, H - 1, 5] = math.nan, math.inf
+    q = torch.randn(b, T, H * G, D, generator=g, device=dev).to(dtype)
+    cnt = [T] * (b - 1) + [T - 21]
+
+    def call(at, rows, count):
+        """Rows at[s] .. of the sequences in one call, over a cache that holds those before them."""
+        c = new_cache(H, D, bs, m, b=b)
+        c.reserve([m] * b)
+        fill(c, k, v, at)
+        pick = lambda x: torch.stack([torch.nn.functional.pad(x[s, at[s]:at[s] + rows], (0, 0, 0, 0, 0, rows - x[s, at[s]:at[s] + rows].shape[0]))
+                                      for s in range(b)])
+        off = [a - h for a, h in zip(at, have)]
+        qq = torch.stack([q[s, off[s]:off[s] + rows] for s in range(b)])
+        return c.append_attend(0, qq, pick(k), pick(v), i32(at), max(at) + rows, i32(count))
+
+    out = call(have, T, cnt)
+    for t in (0, 1, T // 3 - 1, T // 2 - 2, T // 2 + 18, 130, T - 23 - 3):
+        few = call([h + t for h in have], 3, [3] * b)
+        got = out[:, t:t + 3]
+        assert torch.equal(got.isnan(), few.isnan()) and torch.equal(got.nan_to_num(nan=0.0), few.nan_to_num(nan=0.0)), t
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("T", [3, 40, 200])
 def test_padding_rows_and_empty_sequences(dev, T):
