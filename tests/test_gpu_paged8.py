@@ -581,8 +581,8 @@ def test_bad_calls_are_refused():
     err(L.dkv_paged8_attention(r, 0, 16, 2, 1, 2, 16, None, 64, 16, 16, 1 << 30, None), -1, "dtype")
     err(L.dkv_paged8_attention(r, 0, 16, 0, 1, 3, 16, None, 64, 16, 16, 1 << 30, None), -1, "multiple")
     err(L.dkv_paged8_attention(r, 0, 16, 0, 1, 2, 16, None, 0, 16, 16, 1 << 30, None), -1, "max_len")
-    err(L.dkv_paged8_attention(r, 0, 16, 0, 1, 2, 16, None, 64, 16, 16, 64, None), -3, "workspace")
-    err(L.dkv_paged8_attention(r, 0, 16, 0, 1, 2, 16, None, 64, 16, None, 1 << 30, None), -3, "workspace")
+    err(L.dkv_paged8_attention(r, 0, 16, 0, 1, 2, 16, None, 4096, 16, 16, 64, None), -3, "workspace")
+    err(L.dkv_paged8_attention(r, 0, 16, 0, 1, 2, 16, None, 4096, 16, None, 1 << 30, None), -3, "workspace")
     err(L.dkv_paged8_attention(r, 0, 16, 0, 1, 2, None, None, 64, 16, 16, 1 << 30, None), -1, "NULL")
     err(L.dkv_paged8_read(r, 0, 16, None, 1, 16, 16, None), -1, "NULL")
     assert L.dkv_paged8_append(r, 0, 16, 16, 0, 0, 16, None, None) == 0
