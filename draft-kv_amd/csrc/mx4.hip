@@ -520,17 +520,29 @@ __global__ void __launch_bounds__(256, 2) mx4_tile_kernel(MxArgs A, int mtiles, 
             }
             fetch(t + PD, (b + PD) % 4);
             const char* xs = mx_smem + b % NS * STAGE + col * 256;
+            // the operands of step j + 1 are under way while step j multiplies, where registers hold both
+            constexpr int AHEAD = NF * MB <= 20 ? 2 : 1;
+            mx_bf16x8 wv[AHEAD][NF], xv[AHEAD][MB];
+            auto operands = [&](int j) {
+#pragma unroll
+                for (int m = 0; m < MB; ++m)
+                    xv[j % AHEAD][m] = *reinterpret_cast<const mx_bf16x8*>(xs + m * 4096 + ((4 * q + j) ^ col) * 16);
+#pragma unroll
+                for (int i = 0; i < NF; ++i)
+                    wv[j % AHEAD][i] = mx_operand(w[b % NS][i][j], __uint_as_float((sc[i] >> 8 * b & 0xff) << 23));
+            };
+            if (AHEAD == 2) operands(0);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                mx_bf16x8 wv[NF];
+                if (AHEAD == 1) operands(j);
+                else if (j < 3) operands(j + 1);
+                if (AHEAD == 2) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int i = 0; i < NF; ++i) wv[i] = mx_operand(w[b % NS][i][j], __uint_as_float((sc[i] >> 8 * b & 0xff) << 23));
+                for (int m = 0; m < MB; ++m)
 #pragma unroll
-                for (int m = 0; m < MB; ++m) {
-                    const mx_bf16x8 xv = *reinterpret_cast<const mx_bf16x8*>(xs + m * 4096 + ((4 * q + j) ^ col) * 16);
-#pragma unroll
-                    for (int i = 0; i < NF; ++i) acc[i][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv[i], xv, acc[i][m], 0, 0, 0);
-                }
+                    for (int i = 0; i < NF; ++i)
+                        acc[i][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv[j % AHEAD][i], xv[j % AHEAD][m], acc[i][m], 0, 0, 0);
+                if (AHEAD == 2) __builtin_amdgcn_sched_barrier(0);
             }
         }
         if constexpr (MULTI) {
@@ -757,7 +769,7 @@ static int mx_launch_rows(const MxArgs& a, hipStream_t st) {
     // two workgroups of 128 rows of W per CU where 256-row tiles leave less than that (their waves then wait for LDS and
     // the conversions one after another)
     if ((a.M + 79) / 80 * wide < 512) switch (mx_rows(a.M, narrow, {5, 4, 2})) {
-        case 5: return mx_launch_tile<2, 5, 1, MX_CHAIN>(a, st);
+        case 5: return mx_launch_tile<2, 5, 3, MX_CHAIN>(a, st);
         case 4: return mx_launch_tile<2, 4, 3, MX_CHAIN>(a, st);
         default: return mx_launch_tile<2, 2, 3, MX_CHAIN>(a, st);
     }
