@@ -169,22 +169,27 @@ __device__ __forceinline__ uint32_t mx_bf16_pair(float a, float b) {
     return (uint32_t)__builtin_bit_cast(uint16_t, x) | (uint32_t)__builtin_bit_cast(uint16_t, y) << 16;
 }
 
+__device__ __forceinline__ float mx_swiglu(float gate, float up) { return gate / (1.0f + __expf(-gate)) * up; }
+__device__ __forceinline__ mx_f32x4 mx_bias4(const MxArgs& A, int n) {
+    mx_f32x4 b;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) b[e] = n + e < A.N ? load_elem(A.bias, n + e, A.bias_f32 ? DKV_F32 : DKV_BF16) : 0.0f;
+    return b;
+}
 // outputs (m, n .. n + 3), n a multiple of 4
 __device__ __forceinline__ void mx_store(const MxArgs& A, int64_t m, int n, mx_f32x4 t) {
     if (n >= A.N) return;   // the last fragment's rows past N
     if (A.swiglu) {   // rows of W interleave (gate, up); N is even
         for (int e = 0; e < 4; e += 2)
             if (n + e < A.N) {
-                const float o = t[e] / (1.0f + __expf(-t[e])) * t[e + 1];
+                const float o = mx_swiglu(t[e], t[e + 1]);
                 const int64_t at = m * (A.N / 2) + (n + e) / 2;
                 if (A.y_f32) static_cast<float*>(A.y)[at] = o;
                 else static_cast<uint16_t*>(A.y)[at] = f32_to_bf16_rne(o);
             }
         return;
     }
-    if (A.bias)
-        for (int e = 0; e < 4; ++e)
-            if (n + e < A.N) t[e] += load_elem(A.bias, n + e, A.bias_f32 ? DKV_F32 : DKV_BF16);
+    if (A.bias) t += mx_bias4(A, n);
     const int64_t at = m * A.N + n;
     if (A.N % 4 == 0) {
         if (A.y_f32) *reinterpret_cast<mx_f32x4*>(static_cast<float*>(A.y) + at) = t;
@@ -196,6 +201,26 @@ __device__ __forceinline__ void mx_store(const MxArgs& A, int64_t m, int n, mx_f
             if (A.y_f32) static_cast<float*>(A.y)[at + e] = t[e];
             else static_cast<uint16_t*>(A.y)[at + e] = f32_to_bf16_rne(t[e]);
         }
+}
+
+// outputs (m, n .. n + 7), n and N multiples of 8
+__device__ __forceinline__ void mx_store8(const MxArgs& A, int64_t m, int n, mx_f32x4 a, mx_f32x4 b) {
+    if (A.swiglu) {
+        const mx_f32x4 o = {mx_swiglu(a[0], a[1]), mx_swiglu(a[2], a[3]), mx_swiglu(b[0], b[1]), mx_swiglu(b[2], b[3])};
+        const int64_t at = m * (A.N / 2) + n / 2;
+        if (A.y_f32) *reinterpret_cast<mx_f32x4*>(static_cast<float*>(A.y) + at) = o;
+        else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(A.y) + at) = make_uint2(mx_bf16_pair(o[0], o[1]), mx_bf16_pair(o[2], o[3]));
+        return;
+    }
+    if (A.bias) a += mx_bias4(A, n), b += mx_bias4(A, n + 4);
+    const int64_t at = m * A.N + n;
+    if (A.y_f32) {
+        *reinterpret_cast<mx_f32x4*>(static_cast<float*>(A.y) + at) = a;
+        *reinterpret_cast<mx_f32x4*>(static_cast<float*>(A.y) + at + 4) = b;
+    } else {
+        *reinterpret_cast<mx_u32x4*>(static_cast<uint16_t*>(A.y) + at) =
+            mx_u32x4{mx_bf16_pair(a[0], a[1]), mx_bf16_pair(a[2], a[3]), mx_bf16_pair(b[0], b[1]), mx_bf16_pair(b[2], b[3])};
+    }
 }
 
 enum { MX_XF32, MX_XBF16, MX_XMX4 };
@@ -382,15 +407,34 @@ __global__ void __launch_bounds__(512) mx4_stream_kernel(MxArgs A) {
     mx_join<NF, MB>(A, mx_lds, acc, f0, m0, wave, A.S, lane);
 }
 
-// A wave's outputs: fragments f0 .. of W by rows m0 .. of x, o[NF][MB] as the matrix instructions leave them. Where rows
-// of y are not aligned to four values, 16 of them at a time pass through LDS (the wave's own), and leave in runs of
-// 16 NF: four separate values per lane are four times the stores. (4-bit rows, 4096 x 50257 from 768: 409 us, separate
-// 462; bf16 rows, 160 x 50257: 24.6, separate 29.7; 4096: 522, separate 520.)
+// A wave's outputs: fragments f0 .. of W by rows m0 .. of x, o[NF][MB] as the matrix instructions leave them: a lane has
+// four outputs of each fragment, 32 bytes of a row where they are bf16. 16 rows at a time pass through LDS (the wave's
+// own) and leave in runs of 16 NF. 4096 x 28672 from 4096 in 4 bits: 256 us, with every lane's own stores 321 (a workgroup
+// alone on its CU has nothing else to do meanwhile); bf16 rows 657 and 685. Rows of odd length (50257) leave value by value.
 template <int NF, int MB>
 __device__ __forceinline__ void mx_store_tile(const MxArgs& A, float* lds, const mx_f32x4* o, int64_t f0, int64_t m0, int lane) {
     const int64_t frags = mx_frags(A.N);
     const int col = lane % 16, q = lane / 16;
-    if (A.swiglu || A.N % 4 == 0) {
+    if (A.N % 8 == 0) {   // 16 bytes per lane (SwiGLU: half)
+        constexpr int W = 16 * NF, LD = W + 4, ROWS = WAVE / (W / 8);
+        const int n = lane % (W / 8) * 8, rr = lane / (W / 8);
+        const int64_t gn = f0 * 16 + n;
+#pragma unroll
+        for (int m = 0; m < MB; ++m) {
+#pragma unroll
+            for (int i = 0; i < NF; ++i) *reinterpret_cast<mx_f32x4*>(lds + col * LD + 16 * i + 4 * q) = o[i * MB + m];
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int x = 0; x < 16; x += ROWS) {
+                const int64_t r = m0 + 16 * m + x + rr;
+                const mx_f32x4* v = reinterpret_cast<const mx_f32x4*>(lds + (x + rr) * LD + n);
+                if (r < A.M && gn < A.N) mx_store8(A, r, (int)gn, v[0], v[1]);
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+        return;
+    }
+    if (A.swiglu) {
 #pragma unroll
         for (int i = 0; i < NF; ++i)
 #pragma unroll
@@ -447,8 +491,8 @@ __host__ inline unsigned mx_grid(int mtiles, int ntiles) { return (unsigned)((mt
 // x by rows of 16 pieces (8 values), piece p of row r in slot p ^ (r % 16): a row's pieces arrive together, and the 16
 // rows that an operand read takes lie on different banks. One tile ahead is enough where two workgroups per CU multiply
 // a thousand cycles per tile; a few rows' tiles are shorter than W's way from memory.
-// 28672 x 4096: 32 rows 20 us, 160 rows 50 (753 TFLOP/s: matrix instructions and conversions in turn), 1100 rows 203,
-// 4096 rows 710 (1350 TFLOP/s, what a large bf16 product of the library reaches).
+// 28672 x 4096: 32 rows 16 us, 80 rows 27, 160 rows 40 (930 TFLOP/s; without the operands of a step ahead 50), 1100 rows
+// 190, 4096 rows 657 (1460 TFLOP/s, what a large bf16 product of the library reaches).
 enum { MX_CHAIN, MX_MULTI, MX_PART };   // one chunk; several, added here; one of several, to memory
 template <int NF, int MB, int PD, int MODE>
 __global__ void __launch_bounds__(256, 2) mx4_tile_kernel(MxArgs A, int mtiles, int ntiles) {
@@ -520,8 +564,9 @@ __global__ void __launch_bounds__(256, 2) mx4_tile_kernel(MxArgs A, int mtiles, 
             }
             fetch(t + PD, (b + PD) % 4);
             const char* xs = mx_smem + b % NS * STAGE + col * 256;
-            // the operands of step j + 1 are under way while step j multiplies, where registers hold both
-            constexpr int AHEAD = NF * MB <= 20 ? 2 : 1;
+            // the operands of step j + 1 are under way while step j multiplies, where registers hold both (and few
+            // workgroups share a CU)
+            constexpr int AHEAD = PD == 3 && NF * MB <= 20 ? 2 : 1;
             mx_bf16x8 wv[AHEAD][NF], xv[AHEAD][MB];
             auto operands = [&](int j) {
 #pragma unroll
@@ -576,7 +621,7 @@ __global__ void __launch_bounds__(256, 2) mx4_tile_kernel(MxArgs A, int mtiles, 
     mx_f32x4* o;
     if constexpr (MULTI) o = &tot[0][0];
     else o = &acc[0][0];
-    mx_store_tile<NF, MB>(A, reinterpret_cast<float*>(mx_smem) + wave * (16 * (16 * NF + 1)), o, f0, m0, lane);
+    mx_store_tile<NF, MB>(A, reinterpret_cast<float*>(mx_smem) + wave * (16 * (16 * NF + 4)), o, f0, m0, lane);
 }
 
 // The chunks' sums in order, and out: four outputs per thread.
@@ -614,7 +659,8 @@ __global__ void __launch_bounds__(256) mx4_pack_kernel(const X* __restrict__ x, 
 // 4-bit rows: eight waves, four along W by two along x, 4 x MB fragments each. Both operands' tiles go to LDS as they
 // are (1 KB, one load instruction each, four stages); the scale words straight to registers, once in four tiles. At
 // 4 x 8 a tile of 256 x 256 reads 32 KB per 1024 cycles of matrix instructions, half of what an XCD's L2 gives its CUs.
-// 28672 x 4096: 512 rows 43 us (2.8 PFLOP/s), 4096 rows 330 (2.9).
+// 28672 x 4096: 512 rows 42 us (2.8 PFLOP/s), 4096 rows 256 (3.8): without the matrix instructions 219, without the
+// loads 204, so neither alone bounds it; a tile's barrier and the stores at the end do the rest.
 template <int MB, bool MULTI>
 __global__ void __launch_bounds__(512, 2) mx4_tile4_kernel(MxArgs A, int mtiles, int ntiles) {
 #pragma clang fp contract(off)
@@ -712,7 +758,7 @@ __global__ void __launch_bounds__(512, 2) mx4_tile4_kernel(MxArgs A, int mtiles,
     mx_f32x4* o;
     if constexpr (MULTI) o = &tot[0][0];
     else o = &acc[0][0];
-    mx_store_tile<NF, MB>(A, reinterpret_cast<float*>(mx_smem) + wave * (16 * (16 * NF + 1)), o, f0 + wn * NF, (x0 + wm * MB) * 16, lane);
+    mx_store_tile<NF, MB>(A, reinterpret_cast<float*>(mx_smem) + wave * (16 * (16 * NF + 4)), o, f0 + wn * NF, (x0 + wm * MB) * 16, lane);
 }
 
 // 16-row tiles of x per workgroup, of the ones there are kernels for: the fewest rounds of 256 workgroups, by their
@@ -769,7 +815,10 @@ static int mx_launch_rows(const MxArgs& a, hipStream_t st) {
     // two workgroups of 128 rows of W per CU where 256-row tiles leave less than that (their waves then wait for LDS and
     // the conversions one after another)
     if ((a.M + 79) / 80 * wide < 512) switch (mx_rows(a.M, narrow, {5, 4, 2})) {
-        case 5: return mx_launch_tile<2, 5, 3, MX_CHAIN>(a, st);
+        // Four stages of 80 rows leave LDS for two workgroups per CU, two stages for four, which then cover each other's
+        // waits, beginnings and ends. 28672 x 4096: 160 rows (448 workgroups) 41.9 us with four stages, 50.7 with two;
+        // 20000 x 4096: 400 rows (785) 70.0 and 65.0; 50257 x 768: 160 rows (786) 31.5 and 24.3.
+        case 5: return (a.M + 79) / 80 * narrow <= 512 ? mx_launch_tile<2, 5, 3, MX_CHAIN>(a, st) : mx_launch_tile<2, 5, 1, MX_CHAIN>(a, st);
         case 4: return mx_launch_tile<2, 4, 3, MX_CHAIN>(a, st);
         default: return mx_launch_tile<2, 2, 3, MX_CHAIN>(a, st);
     }

@@ -81,7 +81,7 @@ def tol(x, w, dtype, want):
 SIZES = [(1, 16, 32), (1, 960, 576), (3, 17, 100), (16, 100, 128), (17, 64, 640), (33, 250, 1000), (64, 48, 4096), (65, 1030, 257),
          (160, 512, 512), (130, 33, 2304), (300, 768, 768), (2, 5, 1), (4096, 1021, 384), (200, 4099, 512), (90, 16390, 256), (700, 257, 128), (1, 20000, 96), (70, 9000, 160),
          (1, 64, 640), (12, 90, 200), (20, 100, 4224), (100, 130, 10112), (30, 8200, 256), (50, 8210, 130), (2100, 4099, 640), (330, 16402, 256),
-         (250, 33002, 384), (640, 33002, 256), (300, 49000, 128)]
+         (250, 33002, 384), (640, 33002, 256), (300, 49000, 128), (75, 33002, 640), (150, 50257, 128), (240, 40004, 128), (700, 8192, 256), (640, 33000, 128)]
 
 
 @pytest.mark.gpu
