@@ -614,7 +614,7 @@ __global__ void __launch_bounds__(512) paged8_chunk_kernel(P8Args A) {
         }
     };
     if constexpr (ONE) {
-        const int units = (lim1 + P8_UNIT - 1) / P8_UNIT;
+        const int units = min(P8_UNITS, (lim1 + P8_UNIT - 1) / P8_UNIT);   // (longer than max_len said: its first keys)
         if (wave < units) {
             st.clear();
             st.template unit<SETS>(A, u, k0, min(k0 + P8_UNIT, lim1), lim0, lane);

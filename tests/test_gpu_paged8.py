@@ -283,6 +283,25 @@ def test_prompts_equal_calls_of_a_few_rows(dev, shape, dtype):
 
 
 @pytest.mark.gpu
+def test_a_bound_that_is_too_short_drops_chunks_only(dev):
+    """max_len below what a sequence holds: its rows see the chunks of 2048 keys up to it and their own block."""
+    D, H, G, bs, n = 64, 2, 2, 16, 5000
+    g = torch.Generator(device=dev)
+    g.manual_seed(3)
+    k, v = rows_of(g, 1, n + 1, H, D, dev)
+    q = torch.randn(1, 1, H * G, D, generator=g, device=dev)
+    c = new_cache(H, D, bs, n + 1)
+    c.reserve([n + 1])
+    fill(c, k, v, [n])
+    out = c.append_attend(0, q, k[:, n:].contiguous(), v[:, n:].contiguous(), i32([n]), 100)
+    own = n // bs * bs
+    kk = torch.cat([k[0, :2048], k[0, own:n + 1]]).to(BF16).cpu()
+    vv = torch.cat([v[0, :2048], v[0, own:n + 1]]).to(BF16).cpu()
+    want, top = attention(q[0].cpu(), kk, vv, kk.shape[0] - 1, bs)
+    assert ((out[0].double().cpu() - want).abs() <= bound(F32, kk.shape[0], D, top, float(vv.float().abs().max()), want)).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("T", [3, 40, 200])
 def test_padding_rows_and_empty_sequences(dev, T):
     """Rows past count see what the last row does, a sequence without new rows gives zeros; no other block is touched."""
