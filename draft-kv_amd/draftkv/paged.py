@@ -169,18 +169,26 @@ class PagedKVCache:
         self.store = torch.empty((self.batch * self.n_blocks, int(lib().dkv_paged8_block_bytes(H, D, bs))), **kw)
         self.tail = torch.empty((self.batch, self.n_layers, self.tail_rows, self._row_bytes), **kw)
         self.hot = torch.empty((self.batch, 0, self._row_bytes), **kw)      # rows of long appends, grown by need
+        self._hot_of: Optional[tuple] = None       # (layer, T) of the append whose rows are there
+        self._hot_kept: list = []                  # buffers that captured graphs still write to
         # the first position whose bf16 row is still there, per (sequence, layer)
         self.tail_from = np.zeros((self.batch, self.n_layers), np.int64)
 
-    def _hot_room(self, T: int) -> None:
+    def _hot_room(self, layer: int, T: int) -> None:
         """Room for an append of T rows that the tail does not hold beside an open block."""
         if (self.block_size + T + 14) // 16 * 16 <= self.tail_rows:
             return
         need = int(lib().dkv_paged8_hot_rows(self.desc(), T))
+        capturing = torch.cuda.is_current_stream_capturing()
         if need > self.hot.shape[1]:
-            if torch.cuda.is_current_stream_capturing():
+            if capturing:
                 raise RuntimeError(f"append of {T} rows under graph capture: run one of that length before")
+            if self.hot.numel():
+                self.hot.record_stream(torch.cuda.current_stream(self.device))
             self.hot = torch.empty((self.batch, need, self._row_bytes), dtype=torch.uint8, device=self.device)
+        elif capturing and not any(t is self.hot for t in self._hot_kept):
+            self._hot_kept.append(self.hot)
+        self._hot_of = (layer, T)
 
     def _written(self, end: np.ndarray, layers) -> None:
         """Rows up to end [batch, ...] are in ``layers``: the tail holds the last tail_rows (whole 16s) of them."""
@@ -259,7 +267,7 @@ class PagedKVCache:
         """Write ``k, v`` [batch, T, heads, d_head] at positions start[s]..; blocks
         must have been reserved."""
         if self.fp8:
-            self._hot_room(k.shape[1])
+            self._hot_room(layer, k.shape[1])
             ops.paged8_append(self.desc(), layer, k, v, start, count)
             return
         ops.paged_append(self.desc(), layer, k, v, start, count)
@@ -271,6 +279,9 @@ class PagedKVCache:
         An 8-bit cache takes the queries of the rows that were just appended
         (the same T, start and count), float32 or bfloat16."""
         if self.fp8:
+            T = q.shape[1]
+            if (self.block_size + T + 14) // 16 * 16 > self.tail_rows and self._hot_of != (layer, T):
+                raise ValueError(f"attend() of {T} rows must follow their append_layer(): layer {layer}'s bf16 rows are not there")
             return ops.paged8_attention(self.desc(), layer, q, start, max_len, out, count)
         return ops.paged_attention(self.desc(), layer, q, start, max_len, self.chunk_keys, out, count)
 
@@ -278,7 +289,9 @@ class PagedKVCache:
                       max_len: int, count: Optional[torch.Tensor] = None) -> torch.Tensor:
         """append_layer, then attend: one layer's share of a forward."""
         if self.fp8:
-            self._hot_room(k.shape[1])
+            if q.shape[1] != k.shape[1]:
+                raise ValueError(f"append_attend(): {q.shape[1]} queries for {k.shape[1]} rows")
+            self._hot_room(layer, k.shape[1])
             d = self.desc()
             ops.paged8_append(d, layer, k, v, start, count)
             return ops.paged8_attention(d, layer, q, start, max_len, None, count)

@@ -460,6 +460,62 @@ def test_another_stream_and_graph_replays(dev):
 
 # ---------------------------------------------------------------- cache, mirror, engine
 @pytest.mark.gpu
+def test_long_rows_of_another_append_are_refused(dev):
+    """The bf16 rows of a long append are there until the next one; short ones are in the tail."""
+    T = 150
+    c = new_cache(1, 32, 16, 400, layers=2)
+    k = torch.randn(1, T, 1, 32, device=dev)
+    c.reserve([T + 2])
+    st = i32([0])
+    with pytest.raises(ValueError, match="append_layer"):
+        c.attend(0, k, st, T)
+    # each within bound() of the same exact result, which -v negates; |score| <= |k|^2 / sqrt(D)
+    tol = 2 * bound(F32, T, 32, float(k.norm(dim=-1).max()) ** 2 / math.sqrt(32), float(k.abs().max()), None)
+    c.append_layer(0, k, k, st)
+    a = c.attend(0, k, st, T)
+    c.append_layer(1, k, -k, st)
+    with pytest.raises(ValueError, match="append_layer"):
+        c.attend(0, k, st, T)
+    b = c.attend(1, k, st, T)
+    one = new_cache(1, 32, 16, 400)       # (a matrix instruction need not round -x as it rounds x)
+    one.reserve([T])
+    assert torch.equal(b, one.append_attend(0, k, k, -k, st, T)) and ((a + b).abs() <= tol).all()
+    with pytest.raises(ValueError, match="queries"):
+        c.append_attend(0, k[:, :3].contiguous(), k, k, st, T)
+    for L in range(2):     # short ones: any order
+        c.append_layer(L, k[:, :2].contiguous(), (1 - 2 * L) * k[:, :2], i32([T]))
+    x, y = (c.attend(L, k[:, :2].contiguous(), i32([T]), T + 2) for L in range(2))
+    assert ((x + y).abs() <= tol).all()
+
+
+@pytest.mark.gpu
+def test_a_captured_long_append_keeps_its_rows(dev):
+    """A longer append after the capture moves the bf16 rows; the graph still has its own."""
+    T, D = 150, 32
+    g = torch.Generator(device=dev)
+    g.manual_seed(9)
+    k, v = rows_of(g, 1, 700, 2, D, dev)
+    q = torch.randn(1, T, 4, D, generator=g, device=dev)
+    c, other = (new_cache(2, D, 16, 1000) for _ in range(2))
+    for x in (c, other):
+        x.reserve([700])
+    kb, vb, st = k[:, :T].clone(), v[:, :T].clone(), i32([0])
+    want = c.append_attend(0, q, kb, vb, st, T)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = c.append_attend(0, q, kb, vb, st, T)
+    c.append_layer(0, k, v, st)                                     # moves them
+    junk = [torch.full((1 << 20,), math.nan, device=dev) for _ in range(8)]   # takes what was freed
+    for i in range(3):
+        kb.copy_(k[:, T * i:T * i + T])
+        vb.copy_(v[:, T * i:T * i + T])
+        want = other.append_attend(0, q, kb, vb, st, T)
+        graph.replay()
+        assert torch.equal(out, want)
+    assert all(x.isnan().all() for x in junk)
+
+
+@pytest.mark.gpu
 def test_truncate_keeps_what_the_tail_holds(dev):
     c = new_cache(2, 16, 16, 400, tail_rows=64)
     g = torch.Generator(device=dev)
