@@ -60,14 +60,23 @@ def _dt(t: torch.Tensor) -> int:
     raise ValueError(f"unsupported dtype {t.dtype} (float32 or bfloat16)")
 
 
-class Workspace:
-    """Grow-only scratch buffer per device (allocates only when a call needs more)."""
+_is_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
 
-    def __init__(self) -> None:
+
+class Workspace:
+    """Grow-only scratch buffer per device and stream (allocates only when a
+    call needs more): calls on two streams may run at once. ``shared``: not
+    owned by one captured graph; a call that is being captured then takes a
+    buffer from the graph's own memory, which no other graph writes to."""
+
+    def __init__(self, shared: bool = False) -> None:
         self._buf: dict = {}
+        self._shared = shared
 
     def get(self, device: torch.device, nbytes: int) -> torch.Tensor:
-        key = (device.type, device.index)
+        if self._shared and _is_capturing():
+            return torch.empty(max(nbytes, 1), dtype=torch.uint8, device=device)
+        key = (device.type, device.index, _stream())
         b = self._buf.get(key)
         if b is None or b.numel() < nbytes:
             b = torch.empty(max(nbytes, 1 << 16), dtype=torch.uint8, device=device)
@@ -75,7 +84,7 @@ class Workspace:
         return b
 
 
-_WS = Workspace()
+_WS = Workspace(shared=True)
 
 
 class Stager:

@@ -194,6 +194,62 @@ def test_stream_and_graph_replays(dev):
         assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
+@pytest.mark.gpu
+def test_graphs_and_streams_do_not_share_scratch(dev):
+    """Two graphs recorded one after another and two streams, at once, each with products that pack their rows and add
+    chunks through memory; a larger call in between."""
+    from draftkv import ops
+    g = torch.Generator(device=dev)
+    g.manual_seed(2)
+    w = ops.mx4_quantize(torch.randn(1000, 8192, generator=g, device=dev))
+    xs = [torch.randn(24, 8192, generator=g, device=dev) for _ in range(2)]
+    want = [ops.gemm_mx4(x, w, out_dtype=F32) for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    graphs, outs = [], []
+    for x in xs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append([ops.gemm_mx4(x, w, out_dtype=F32) for _ in range(8)])
+        graphs.append(graph)
+    ops.gemm_mx4(torch.randn(900, 8192, generator=g, device=dev), w)      # more scratch than before
+    junk = [torch.full((1 << 22,), math.nan, device=dev) for _ in range(4)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for o, ref in zip(outs, want):
+            assert all(torch.equal(t, ref) for t in o)
+        eager = []
+        for i in range(16):
+            with torch.cuda.stream(streams[i % 2]):
+                eager.append(ops.gemm_mx4(xs[i % 2], w, out_dtype=F32))
+        torch.cuda.synchronize()
+        assert all(torch.equal(t, want[i % 2]) for i, t in enumerate(eager))
+    assert all(t.isnan().all() for t in junk)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("xk", ["bf16", "f32", "mx4"])
+def test_rows_past_32_bits_of_bytes(dev, xk):
+    from draftkv import ops
+    g = torch.Generator(device=dev)
+    g.manual_seed(5)
+    M, N, K = 150000, 48, 16384          # x: 4.9 GB of bf16
+    x = torch.empty(M, K, device=dev, dtype=F32 if xk == "f32" else BF16).normal_(generator=g)
+    w = ops.mx4_quantize(torch.randn(N, K, generator=g, device=dev))
+    q = ops.mx4_quantize(x) if xk == "mx4" else x
+    out = ops.gemm_mx4(q, w, out_dtype=F32)
+    for lo in (0, 65536, 131071, 149984):
+        part = x[lo:lo + 16].contiguous()
+        pq = ops.mx4_quantize(part) if xk == "mx4" else part
+        assert torch.equal(ops.gemm_mx4(pq, w, out_dtype=F32), out[lo:lo + 16]), lo
+    if xk == "mx4":
+        v = ops.MX4(q.codes, q.scales, (M, K)).values()
+        assert torch.equal(v[-16:], pq.values())
+
+
 # ---------------------------------------------------------------- models
 @pytest.mark.gpu
 @pytest.mark.parametrize("family,dtype", [("llama", F32), ("llama", BF16), ("bias", F32), ("gpt2", F32), ("gpt2", BF16), ("tiny", F32)])
