@@ -72,6 +72,7 @@ class Decoder:
             raise ValueError("dtype must be torch.float32 or torch.bfloat16")
         self.act_dtype = dtype           # dtype of GEMM inputs
         self.kv_dtype = dtype            # dtype of the full cache; torch.float8_e4m3fn holds it in 8 bits
+        self.weights_version = 0         # recorded graphs hold the weights they were recorded with
         self._cs: Optional[torch.Tensor] = None
         self._cs_len = 0
 
@@ -195,6 +196,7 @@ class Decoder:
         biases and the head stay. The activations of a product are rounded to
         bf16; verify rows and one-token rows still agree bit for bit."""
         inter = getattr(self, "gate_up_interleaved", False)
+        self.weights_version += 1
         for p in self.layers:
             for name in ("wqkv", "wo", "w1", "w2"):
                 w = getattr(p, name)

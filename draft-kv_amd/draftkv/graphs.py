@@ -42,7 +42,7 @@ from . import ops
 
 def graph_key(model, comp, b: int, temperature: float) -> tuple:
     cs = getattr(model, "_cs", None)
-    return (b, float(temperature), tuple(comp.cfgs), comp.cap, comp.page_stride, comp.pages.data_ptr(),
+    return (getattr(model, "weights_version", 0), b, float(temperature), tuple(comp.cfgs), comp.cap, comp.page_stride, comp.pages.data_ptr(),
             comp.pos.data_ptr(), comp.score.data_ptr(), comp.n_rows.data_ptr(),
             None if cs is None else (cs.data_ptr(), model._cs_len))
 
@@ -131,7 +131,7 @@ class DraftStepGraph:
 
 def full_graph_key(model, full, b: int, temperature: float, max_len: int) -> tuple:
     cs = getattr(model, "_cs", None)
-    return (b, float(temperature), full.store.data_ptr(), full.d_tables.data_ptr(), int(max_len),
+    return (getattr(model, "weights_version", 0), b, float(temperature), full.store.data_ptr(), full.d_tables.data_ptr(), int(max_len),
             full.chunk_keys, full.tail.data_ptr() if full.fp8 else None, None if cs is None else (cs.data_ptr(), model._cs_len))
 
 

@@ -291,6 +291,35 @@ def test_model_with_4_bit_weights(dev, family, dtype):
         assert got == DraftKVEngine(model).generate_baseline_batch(prompts, 30)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("gamma", [0, 4])
+def test_weights_quantized_while_decoding(dev, gamma):
+    """Recorded steps hold the weights that they were recorded with: after quantize_weights() they are recorded anew."""
+    from draftkv import CompressionConfig, DraftKVEngine, FixedPolicy
+    from draftkv.engine import DecodeBatch
+    from draftkv.llama import demo_llama
+    prompts = [np.random.default_rng(s).integers(0, 128, size=n).tolist() for s, n in ((0, 30), (1, 40))]
+    runs, graphs = [], 0
+    for use in (True, False):
+        m = demo_llama(dtype=F32, device=dev)
+        eng = DraftKVEngine(m, FixedPolicy(CompressionConfig(4, 0.5), gamma))
+        eng.draft_graphs = use
+        full = eng._new_full(2, 200)
+        eng._prefill(prompts, full)
+        batch = DecodeBatch(eng, prompts, full, 60, 0.0)
+        for _ in range(6):
+            batch.step()
+        old = [w for p in m.layers for w in (p.wqkv, p.wo, p.w1, p.w2)]
+        m.quantize_weights()
+        for w in old:
+            w.fill_(math.nan)     # (nothing reads them any more)
+        while batch.step():
+            pass
+        runs.append([r.tokens for r in batch.results()])
+        graphs = max(graphs, len(batch._graphs))
+    assert runs[0] == runs[1] and graphs >= 2
+
+
 # ---------------------------------------------------------------- refusals (no GPU)
 @pytest.mark.skipif(torch.cuda.is_available(), reason="made-up pointers: host checks only")
 def test_bad_calls_are_refused():
