@@ -745,7 +745,11 @@ class MX4:
     __slots__ = ("codes", "scales", "shape")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape: tuple) -> None:
-        self.codes, self.scales, self.shape = codes, scales, shape
+        rows, k = shape
+        for t, name, n in ((codes, "codes", lib().dkv_mx4_code_bytes(rows, k)), (scales, "scales", lib().dkv_mx4_scale_bytes(rows, k))):
+            if t.dtype != torch.uint8 or t.numel() != n or not t.is_contiguous() or t.device != codes.device:
+                raise ValueError(f"MX4: {name} of {tuple(shape)} must be {n} contiguous bytes on {codes.device}")
+        self.codes, self.scales, self.shape = codes, scales, (rows, k)
 
     @property
     def device(self):

@@ -174,6 +174,11 @@ class PagedKVCache:
         # the first position whose bf16 row is still there, per (sequence, layer)
         self.tail_from = np.zeros((self.batch, self.n_layers), np.int64)
 
+    def _here(self, *tensors: Optional[torch.Tensor]) -> None:
+        for t in tensors:
+            if t is not None and t.device != self.store.device:
+                raise ValueError(f"a tensor on {t.device} for a cache on {self.store.device}")
+
     def _hot_room(self, layer: int, T: int) -> None:
         """Room for an append of T rows that the tail does not hold beside an open block."""
         if (self.block_size + T + 14) // 16 * 16 <= self.tail_rows:
@@ -267,6 +272,7 @@ class PagedKVCache:
         """Write ``k, v`` [batch, T, heads, d_head] at positions start[s]..; blocks
         must have been reserved."""
         if self.fp8:
+            self._here(k)
             self._hot_room(layer, k.shape[1])
             ops.paged8_append(self.desc(), layer, k, v, start, count)
             return
@@ -279,6 +285,7 @@ class PagedKVCache:
         An 8-bit cache takes the queries of the rows that were just appended
         (the same T, start and count), float32 or bfloat16."""
         if self.fp8:
+            self._here(q)
             T = q.shape[1]
             if (self.block_size + T + 14) // 16 * 16 > self.tail_rows and self._hot_of != (layer, T):
                 raise ValueError(f"attend() of {T} rows must follow their append_layer(): layer {layer}'s bf16 rows are not there")
@@ -289,6 +296,7 @@ class PagedKVCache:
                       max_len: int, count: Optional[torch.Tensor] = None) -> torch.Tensor:
         """append_layer, then attend: one layer's share of a forward."""
         if self.fp8:
+            self._here(k, q)
             if q.shape[1] != k.shape[1]:
                 raise ValueError(f"append_attend(): {q.shape[1]} queries for {k.shape[1]} rows")
             self._hot_room(layer, k.shape[1])
@@ -304,6 +312,7 @@ class PagedKVCache:
         the device); rows past length[s], the rows the sequence holds, are zero."""
         if not self.fp8:
             raise ValueError("read_rows() is the 8-bit cache's; use read()")
+        self._here(first)
         return ops.paged8_read(self.desc(), layer, first, length, T)
 
     def commit(self, counts: Sequence[int]) -> None:

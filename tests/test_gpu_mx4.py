@@ -368,6 +368,15 @@ def test_bad_tensors_are_refused():
         ops.gemm_mx4(w, ops.MX4(w.codes, w.scales, (15, 32)), swiglu=True)
 
 
+def test_matrices_of_other_sizes_are_refused():
+    from draftkv import ops
+    b = lambda n: torch.zeros(n, dtype=torch.uint8)
+    ops.MX4(b(2048), b(512), (17, 128))
+    for codes, scales in ((b(1024), b(512)), (b(2048), b(256)), (b(4096)[::2], b(512)), (torch.zeros(2048), b(512))):
+        with pytest.raises(ValueError, match="contiguous bytes"):
+            ops.MX4(codes, scales, (17, 128))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("M,N,K", [(16, 100, 128), (3, 17, 100), (130, 36, 64), (40, 1028, 256), (50, 260, 2048), (20, 102, 4200), (12, 50, 4100)])
 def test_nothing_is_written_past_the_outputs(dev, M, N, K):

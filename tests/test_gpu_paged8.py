@@ -664,6 +664,16 @@ def test_bad_calls_are_refused():
     assert L.dkv_paged8_hot_rows(r, 113) == 0 and L.dkv_paged8_hot_rows(r, 114) == 144
 
 
+def test_tensors_on_another_device_are_refused():
+    from draftkv.paged import PagedKVCache
+    c = PagedKVCache(1, 2, 64, 16, 4, F8, device="cpu")
+    k, st = torch.zeros(1, 1, 2, 64, device="meta"), torch.zeros(1, dtype=torch.int32)
+    for call in (lambda: c.append_layer(0, k, k, st), lambda: c.attend(0, k, st, 16), lambda: c.append_attend(0, k, k, k, st, 16),
+                 lambda: c.read_rows(0, st.to("meta"), st, 1)):
+        with pytest.raises(ValueError, match="for a cache on"):
+            call()
+
+
 def test_bad_constructions_are_refused():
     from draftkv.paged import PagedKVCache
     for kw, word in ((dict(block_size=48), "block_size"), (dict(d_head=300), "d_head"), (dict(tail_rows=20), "tail_rows")):
