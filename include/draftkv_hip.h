@@ -134,10 +134,10 @@ int dkv_paged_attention(const dkv_paged_t* cache, int32_t layer, const float* q,
  * float32, paged.py:76-176). A block of block_size (16, 32, 64 or 128) tokens
  * is coded in e4m3 once all its rows are there; e is the least integer with
  * max |x| <= 448 * 2^e over the block's finite K (V) values of the head,
- * within -126 .. 119; NaN and infinities become NaN. A query at position p reads the blocks before
- * its own in 8 bits and its own block's rows up to p in bf16, so its result
- * is a function of rows 0..p alone, whatever rows share a call and however
- * they were appended or rolled back.
+ * within -126 .. 119; NaN and infinities become NaN. A query at position p
+ * reads the blocks before its own in 8 bits and its own block's rows up to p
+ * in bf16, so its result is a function of rows 0..p alone, whatever rows share
+ * a call and however they were appended or rolled back.
  * pool: blocks of dkv_paged8_block_bytes(), 16-byte aligned; block_table as in
  * dkv_paged_t. tail: the last tail_rows rows in bf16 (a ring; a multiple of
  * 16, at least block_size + 16), batch * n_layers * tail_rows *
@@ -176,9 +176,10 @@ int dkv_paged8_append(const dkv_paged8_t* cache, int32_t layer, const void* k, c
  * at absolute positions into units of 256 and chunks of 2048 that fold in
  * order, the query's own block last: a row's result depends neither on T nor
  * on the launch. A padding row t >= count[s] sees what the last row does, and
- * is zero where count[s] is 0. max_len bounds start + count of
- * every sequence (it sizes the launch). work: dkv_paged8_attention_workspace()
- * bytes, 16-byte aligned. */
+ * is zero where count[s] is 0. max_len bounds start + count of every sequence
+ * (it sizes the launch; keys past the chunk that it ends in are not read, but
+ * for the own blocks). work: dkv_paged8_attention_workspace() bytes, 16-byte
+ * aligned; none (it may be NULL) where that is 0. */
 size_t dkv_paged8_attention_workspace(const dkv_paged8_t* cache, int32_t T, int32_t n_q_heads, int32_t max_len);
 int dkv_paged8_attention(const dkv_paged8_t* cache, int32_t layer, const void* q, int32_t q_dtype, int32_t T,
                          int32_t n_q_heads, const int32_t* start, const int32_t* count, int32_t max_len, void* out,
