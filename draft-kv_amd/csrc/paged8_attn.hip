@@ -547,9 +547,10 @@ __device__ __forceinline__ void p8_zero_rows(const P8Args& A, const P8Rows& R, i
 }
 
 // ---------------------------------------------------------------- few rows: a workgroup streams its chunks
-// Two float32 q-tiles' queries would take 96 registers of the 256 that two waves per SIMD have; the eight waves share
-// them in LDS instead.
-__host__ __device__ constexpr bool p8_query_in_lds(int dp, int nq, int ns) { return nq * (dp / 32) * ns > 16; }
+// Two float32 q-tiles' queries of 128 channels would take 96 registers of the 256 that two waves per SIMD have, bf16 ones
+// 32 that spill; the eight waves share them in LDS instead (5 rows of 4 heads each, batch 32, context 32k, bf16: 502 us
+// with registers, 465 so).
+__host__ __device__ constexpr bool p8_query_in_lds(int dp, int nq, int ns) { return nq * (dp / 32) * ns > 16 || nq * (dp / 32) >= 8; }
 __host__ __device__ constexpr size_t p8_chunk_lds(int dp, int nq, int ns) {
     return (size_t)P8_UNITS * nq * ((dp / 16) * 1024 + 16 * sizeof(float2)) +
            (p8_query_in_lds(dp, nq, ns) ? (size_t)nq * (dp / 32) * ns * 1024 : 0);
@@ -560,7 +561,9 @@ __host__ __device__ constexpr size_t p8_chunk_lds(int dp, int nq, int ns) {
 // give a unit) and writes out: the merge would cost as much again as a short context's attention.
 template <int DP, int NQ, int NS, bool ONE>
 __global__ void __launch_bounds__(512) paged8_chunk_kernel(P8Args A) {
-    constexpr int NDT = DP / 16, SETS = DP <= 64 || NQ == 1 ? 2 : 1;
+    // (two sets of codes where they do not spill: 16 / 8 heads of 256, 16 x 16000 keys, float32, 5 rows 420 us with two, 247
+    // with one; of 192 bf16 200 and 157)
+    constexpr int NDT = DP / 16, SETS = DP <= 64 || (NQ == 1 && DP <= 128) ? 2 : 1;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), lane = threadIdx.x % WAVE;
     const P8Rows R = p8_rows(A, blockIdx.x);
     const int r0 = blockIdx.y * 16 * NQ, bs = A.c.block_size;
@@ -956,12 +959,12 @@ __host__ constexpr int p8_walk_tiles(int dp, int ns) { return dp > 128 || ns > 1
 // Which kernel, where either could take the rows: the one that a model of their times says is faster. A workgroup that
 // streams a chunk needs `full` us for its 2048 keys where every CU has one, and `base` however few keys it has (half of
 // that where CUs stay free); a walking one, of many more rows, 12 us and `step` per 32 keys. Measured, streaming against
-// walking, us: 32 / 8 heads of 128, bf16, one sequence: 400 rows on no context 21 / 33, 1600 rows 84 / 89; on 2000 keys
-// 100 rows 24 / 104, 400 rows 62 / 110, 1600 rows 215 / 174; four sequences, 400 rows on 2000 keys 202 / 137. 9 / 3
+// walking, us: 32 / 8 heads of 128, bf16, one sequence: 400 rows on no context 20 / 33, 1600 rows 78 / 89; on 2000 keys
+// 100 rows 22 / 104, 400 rows 56 / 110, 1600 rows 205 / 174; four sequences, 400 rows on 2000 keys 186 / 137. 9 / 3
 // heads of 64, float32: 50 rows on 8000 keys 27 / 71, 800 rows 112 / 98.
 static bool p8_walks(const dkv_paged8_t& c, int64_t tiles, int T, int max_len, int nq, int slots, int per_slot, int ns) {
     const int dp = p8_dp(c.head_dim), at = dp == 32 ? 0 : dp / 64;
-    static const float base[2][5] = {{9, 12, 13, 14, 20}, {14, 23, 20, 18, 33}}, full[2][5] = {{12, 16, 33, 24, 37}, {19, 30, 42, 24, 59}},
+    static const float base[2][5] = {{9, 12, 13, 13, 15}, {14, 23, 20, 18, 25}}, full[2][5] = {{12, 16, 26, 19, 24}, {19, 30, 40, 27, 36}},
                        step[2][5] = {{.8f, .9f, 1.45f, 1.f, 1.2f}, {.7f, .9f, 1.45f, 1.45f, 2.2f}};
     const int64_t heads = (int64_t)c.n_kv_heads * c.batch, groups = (tiles + nq - 1) / nq;
     if (groups > 65535) return true;
