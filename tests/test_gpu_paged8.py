@@ -245,7 +245,8 @@ PROMPTS = [
     (128, 2, 8, 16, [0, 7, 30, 16, 100, 33], 300), (64, 2, 16, 32, [0, 7, 30, 16, 3, 2, 1, 31], 200), (16, 4, 16, 16, [20, 7, 1, 16, 3, 2, 0, 0], 300),
     (192, 2, 8, 64, [0, 7, 70, 64, 3, 2, 1, 129], 300), (256, 2, 8, 16, [0, 7, 30, 16, 3, 15], 200), (16, 4, 16, 16, [1700, 0, 2000, 1999], 200),
     (64, 2, 16, 16, [1700, 0, 3000, 2049], 200), (64, 1, 16, 128, [1700, 0, 3000, 2049], 200), (128, 2, 16, 16, [1700, 0, 2000, 1999], 200),
-    (128, 1, 16, 64, [3000], 800), (192, 1, 16, 16, [2000], 800), (256, 1, 16, 16, [3000], 400), (256, 1, 8, 32, [3001], 800),    (128, 1, 16, 16, [3000], 1200), (192, 1, 1, 16, [3000, 2990], 4000), (256, 1, 1, 64, [3000, 2990], 4000),
+    (128, 1, 16, 64, [3000], 800), (192, 1, 16, 16, [2000], 800), (256, 1, 16, 16, [3000], 400), (256, 1, 8, 32, [3001], 800),
+    (128, 1, 16, 16, [3000], 1200), (192, 1, 1, 16, [3000, 2990], 4000), (256, 1, 1, 64, [3000, 2990], 4000),
 ]
 
 
