@@ -641,18 +641,30 @@ __global__ void __launch_bounds__(256) mx4_reduce_kernel(MxArgs A) {
     mx_store(A, i / quads, (int)(i % quads) * 4, t);
 }
 
-// Rows of any type and width as bf16 rows of whole tiles, zeros past K.
-template <class X>
+// Rows of any type and width as bf16 rows of whole tiles, zeros past K. VEC: rows of x in whole, 16-byte aligned runs of
+// 8. Bound by the traffic (4096 x 14336 float32, 352 MB: 62 us, value by value 125).
+template <class X, bool VEC>
 __global__ void __launch_bounds__(256) mx4_pack_kernel(const X* __restrict__ x, int64_t M, int K, int Kp, uint32_t* __restrict__ out) {
     const int64_t n = M * (Kp / 8);
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
         const int64_t r = i / (Kp / 8);
         const int k = (int)(i % (Kp / 8)) * 8;
-        float v[8];
+        const X* p = x + r * K + k;
+        mx_u32x4 o = {0, 0, 0, 0};
+        if constexpr (VEC && sizeof(X) == 4) {
+            if (k < K) {
+                const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+                o = mx_u32x4{mx_bf16_pair(a.x, a.y), mx_bf16_pair(a.z, a.w), mx_bf16_pair(b.x, b.y), mx_bf16_pair(b.z, b.w)};
+            }
+        } else if constexpr (VEC) {
+            if (k < K) o = *reinterpret_cast<const mx_u32x4*>(p);
+        } else {
+            float v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = k + e < K ? mx_load(x + r * K + k + e) : 0.0f;
-        *reinterpret_cast<mx_u32x4*>(out + i * 4) =
-            mx_u32x4{mx_bf16_pair(v[0], v[1]), mx_bf16_pair(v[2], v[3]), mx_bf16_pair(v[4], v[5]), mx_bf16_pair(v[6], v[7])};
+            for (int e = 0; e < 8; ++e) v[e] = k + e < K ? mx_load(p + e) : 0.0f;
+            o = mx_u32x4{mx_bf16_pair(v[0], v[1]), mx_bf16_pair(v[2], v[3]), mx_bf16_pair(v[4], v[5]), mx_bf16_pair(v[6], v[7])};
+        }
+        *reinterpret_cast<mx_u32x4*>(out + i * 4) = o;
     }
 }
 
@@ -967,10 +979,13 @@ extern "C" int dkv_gemm_mx4(const void* x, int32_t x_dtype, const uint8_t* x_sca
             return fail(DKV_EWORKSPACE, "dkv_gemm_mx4: workspace too small or not 16-byte aligned (need " + std::to_string(need) + ")");
         const dim3 grid((unsigned)std::min<int64_t>(8192, ((int64_t)M * (kp / 8) + 255) / 256)), blk(256);
         uint32_t* out = static_cast<uint32_t*>(work);
-        if (x_dtype == DKV_F32)
-            hipLaunchKernelGGL((mx4_pack_kernel<float>), grid, blk, 0, st, static_cast<const float*>(x), (int64_t)M, K, kp, out);
-        else
-            hipLaunchKernelGGL((mx4_pack_kernel<uint16_t>), grid, blk, 0, st, static_cast<const uint16_t*>(x), (int64_t)M, K, kp, out);
+        const bool vec = K % 8 == 0 && aligned(x, 16);
+#define DKV_MXP(XX, VV) hipLaunchKernelGGL((mx4_pack_kernel<XX, VV>), grid, blk, 0, st, static_cast<const XX*>(x), (int64_t)M, K, kp, out)
+        if (x_dtype == DKV_F32 && vec) DKV_MXP(float, true);
+        else if (x_dtype == DKV_F32) DKV_MXP(float, false);
+        else if (vec) DKV_MXP(uint16_t, true);
+        else DKV_MXP(uint16_t, false);
+#undef DKV_MXP
         if ((rc = check_launch("dkv_gemm_mx4(pack)"))) return rc;
         a.x = work, a.ldx = kp;
     }

@@ -30,10 +30,13 @@ def _stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _device(dev: torch.device):
     """The launch's device made current, where it is not (the stream is then that device's current one)."""
     if dev.index is None or _get_device is not None and _get_device() == dev.index:
-        return contextlib.nullcontext()
+        return _HERE
     return torch.cuda.device(dev)
 
 
@@ -785,7 +788,8 @@ def mx4_quantize(x: torch.Tensor, values: bool = False):
         with _device(x.device):
             check(lib().dkv_mx4_quantize(x.data_ptr(), dt, rows, k, codes.data_ptr(), scales.data_ptr(), _ptr(out),
                                          _stream()), "dkv_mx4_quantize")
-    q = MX4(codes, scales, (rows, k))
+    q = MX4.__new__(MX4)   # (of the right sizes by construction)
+    q.codes, q.scales, q.shape = codes, scales, (rows, k)
     return (q, out) if values else q
 
 
