@@ -269,8 +269,8 @@ __device__ __forceinline__ void mx_join(const MxArgs& A, mx_f32x4* lds, const mx
 // instruction as they are. More fragments per wave halve and quarter the reads of x, which at 64 rows are 16 times a
 // fragment's bytes. Grid (group of fragments, group of rows), one wave per chunk; the sums meet in LDS.
 // RAG: K is no multiple of 128 (but of 8): x is zero from there on.
-// 28672 x 4096 (62 MB, 13.1 us at the rate of a copy): 4-bit rows 11.4 us for one, 13.7 for 32, 17.8 for 64; bf16 rows
-// 16.4 for one, 21.8 for 16. The bf16 rows pay for the conversions of W (36.7 with W in bf16).
+// 28672 x 4096 (62 MB, 13.1 us at the rate of a copy): 4-bit rows 11.4 us for one, 13.7 for 32, 17.8 for 64. 4096 x 4096
+// (8.9 MB): 5.0 for one, 8.1 for 64; bf16 rows 6.1 for one, 11.7 for 16: each wave converts its W and waits for its x.
 template <int XM, int MB, int NF, bool RAG>
 __global__ void __launch_bounds__(512) mx4_stream_kernel(MxArgs A) {
 #pragma clang fp contract(off)
@@ -491,7 +491,7 @@ __host__ inline unsigned mx_grid(int mtiles, int ntiles) { return (unsigned)((mt
 // x by rows of 16 pieces (8 values), piece p of row r in slot p ^ (r % 16): a row's pieces arrive together, and the 16
 // rows that an operand read takes lie on different banks. One tile ahead is enough where two workgroups per CU multiply
 // a thousand cycles per tile; a few rows' tiles are shorter than W's way from memory.
-// 28672 x 4096: 32 rows 16 us, 80 rows 27, 160 rows 40 (930 TFLOP/s; without the operands of a step ahead 50), 1100 rows
+// 28672 x 4096: one row 15 us, 32 rows 16, 80 rows 27, 160 rows 40 (930 TFLOP/s; without the operands of a step ahead 50), 1100 rows
 // 190, 4096 rows 657 (1460 TFLOP/s, what a large bf16 product of the library reaches).
 enum { MX_CHAIN, MX_MULTI, MX_PART };   // one chunk; several, added here; one of several, to memory
 template <int NF, int MB, int PD, int MODE>
@@ -851,16 +851,27 @@ static int mx_launch_stream(const MxArgs& a, hipStream_t st) {
     hipLaunchKernelGGL(fn, grid, blk, lds, st, a);
     return check_launch("dkv_gemm_mx4");
 }
-// Up to MX_ONE rows cost a wave next to nothing beside its W; float rows past MX_FEW go through LDS.
-// Packed first are: rows that no 16-byte loads can read (value by value 2048 x 515 took 13 us at 4 rows, packed 5.5;
-// 4096 x 4097 27 and 9); past MX_FEW, rows of K % 128 != 0; float32 rows past MX_ONE, or of a W that is long enough for
-// its waves' conversions of the same x to cost more than a launch (28672 x 4096, one row: 26.8 us, packed 19.1; 4096 x
-// 14336 16.1 and 12.7; 4096 x 4096 8.6 and 8.6).
+// Float rows that a wave takes beside its W from L2; more go through LDS. Of a weight in one chunk (wide) all do: its
+// workgroups fill the CUs, and their x comes in time (28672 x 4096 bf16: one row 14.8 us, by the waves themselves 16.5, 16
+// rows 15.5 and 21.5; 50257 x 768: 8.0 and 9.6, 9.1 and 13.7), unless K % 128 asks for another launch first. Of the others
+// up to MX_ONE rows, which cost a wave next to nothing, or MX_FEW where the chunks are short (6144 x 4096: 16 rows 9.7,
+// through LDS 10.4; 4096 x 14336: 22.1 and 14.8, one row 10.7 and 14.0).
 constexpr int MX_ONE = 4, MX_FEW = 16;
+static int mx_few(int N, int K) {
+    int S, CT;
+    mx_chunks(N, K, S, CT);
+    if (S == 1 && N >= 16384) return K % 128 ? MX_ONE : 0;
+    return mx_tiles(K) - CT >= 64 ? MX_ONE : MX_FEW;
+}
+// Packed first are: rows that no 16-byte loads can read (value by value 2048 x 515 took 13 us at 4 rows, packed 5.5;
+// 4096 x 4097 27 and 9); of those that go through LDS, rows of K % 128 != 0 and float32 ones; float32 rows past MX_ONE,
+// or of a W that is long enough for its waves' conversions of the same x to cost more than a launch (4096 x 14336, one
+// row: 16.1 us, packed 12.7; 4096 x 4096 8.6 and 8.6).
 static bool mx_packs(const void* x, int x_dtype, int M, int N, int K) {
     if (x_dtype == DKV_MX4) return false;
     if (K % 8 || reinterpret_cast<uintptr_t>(x) % 16) return true;
-    return x_dtype == DKV_F32 ? M > MX_ONE || mx_frags(N) * mx_tiles(K) > 8192 : M > MX_FEW && K % 128;
+    const int few = mx_few(N, K);
+    return x_dtype == DKV_F32 ? M > std::min(few, MX_ONE) || mx_frags(N) * mx_tiles(K) > 8192 : M > few && K % 128;
 }
 template <int MB, bool MULTI>
 static int mx_launch_tile4(const MxArgs& a, hipStream_t st) {
@@ -962,7 +973,8 @@ extern "C" int dkv_gemm_mx4(const void* x, int32_t x_dtype, const uint8_t* x_sca
         return rc ? rc : check_launch("dkv_gemm_mx4");
     }
     const bool packs = mx_packs(x, x_dtype, M, N, K);
-    if (M <= MX_FEW && !packs) {
+    const int few = mx_few(N, K);
+    if (M <= few && !packs) {
         const bool rag = K % 128;
         if (x_dtype == DKV_F32) return rag ? mx_launch_stream<MX_XF32, 1, 1, true>(a, st) : mx_launch_stream<MX_XF32, 1, 1, false>(a, st);
         if (M <= MX_ONE) return rag ? mx_launch_stream<MX_XBF16, 1, 1, true>(a, st) : mx_launch_stream<MX_XBF16, 1, 1, false>(a, st);
@@ -989,7 +1001,7 @@ extern "C" int dkv_gemm_mx4(const void* x, int32_t x_dtype, const uint8_t* x_sca
         if ((rc = check_launch("dkv_gemm_mx4(pack)"))) return rc;
         a.x = work, a.ldx = kp;
     }
-    if (M <= MX_FEW) return M <= MX_ONE ? mx_launch_stream<MX_XBF16, 1, 1, false>(a, st) : mx_launch_stream<MX_XBF16, 1, 2, false>(a, st);
+    if (M <= few) return M <= MX_ONE ? mx_launch_stream<MX_XBF16, 1, 1, false>(a, st) : mx_launch_stream<MX_XBF16, 1, 2, false>(a, st);
     if (mx_parts(M, N, K)) {
         const size_t xb = packs ? (size_t)M * kp * 2 : 0, need = xb + mx_part_bytes(M, N, K);
         if (!work || work_bytes < need || !aligned(work, 16))
@@ -1011,5 +1023,5 @@ extern "C" size_t dkv_gemm_mx4_workspace(const void* x, int32_t x_dtype, int32_t
     using namespace dkv;
     if (M < 1 || N < 1 || K < 1 || x_dtype == DKV_MX4) return 0;
     // (a multiple of 16: the partial sums follow the packed rows)
-    return (mx_packs(x, x_dtype, M, N, K) ? (size_t)M * 128 * mx_tiles(K) * 2 : 0) + (M > MX_FEW ? mx_part_bytes(M, N, K) : 0);
+    return (mx_packs(x, x_dtype, M, N, K) ? (size_t)M * 128 * mx_tiles(K) * 2 : 0) + (M > mx_few(N, K) ? mx_part_bytes(M, N, K) : 0);
 }

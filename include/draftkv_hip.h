@@ -475,9 +475,9 @@ int dkv_mx4_values(const uint8_t* codes, const uint8_t* scales, int32_t rows, in
  * * up of the float32 outputs, [M][N/2] (N even, no bias). K is cut into
  * chunks fixed by (N, K) whose sums are added in order, so a row's result is
  * the same for any M. work: dkv_gemm_mx4_workspace() bytes, 16-byte
- * aligned (for float rows that are packed first: those of K % 8 != 0 or not
- * 16-byte aligned, float32 ones past a few rows of a small w, more than 16 of
- * K % 128 != 0; and for the chunks' sums of some narrow products)  -- the x @ W (+ b) products of the model forwards
+ * aligned (for float rows that are packed to bf16 first and for the chunks'
+ * sums of some narrow products; none, and NULL will do, where that is 0)  --
+ * the x @ W (+ b) products of the model forwards
  * (model.py:113-133, gpt2.py:191-213, llama.py:187-225) */
 size_t dkv_gemm_mx4_workspace(const void* x, int32_t x_dtype, int32_t M, int32_t N, int32_t K);
 int dkv_gemm_mx4(const void* x, int32_t x_dtype, const uint8_t* x_scales, const uint8_t* w,
