@@ -10,8 +10,9 @@
 // A code is exact in bf16 and the conversion instruction applies the block's scale, so the products see the values the
 // cache stands for. In the S^T accumulator a lane holds keys 4 q + r of two tiles for one row; taking the k-slots of
 // the second product in that order, the probabilities never leave their lane. float32 queries and probabilities are
-// split into three bf16 parts (NS = 3: 24 bits, as much as float32 has); bf16 queries are whole, and their
-// probabilities are rounded once to bf16 (NS = 1), an error of at most 2^-8 of each, as much as the output's own rounding.
+// split into three bf16 parts (NS = 3: 24 bits, as much as float32 has); bf16 queries are whole (NS = 1), and their
+// probabilities two parts (PS = 2): 2^-16 of each, far below the rounding of a bf16 output. (One part, 2^-8 of each,
+// put 40 % on the error of a result: 0.0023 of its norm where the output's own rounding is 0.0017.)
 //
 // Order of the sums, the same for every launch: units of 256 keys at absolute positions, each with a softmax of its
 // own in steps of 32; a chunk's eight units fold in order; chunks of 2048 keys fold in order; the query's own block
@@ -30,6 +31,9 @@ typedef __bf16 p8_bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 p8_bf16x2 __attribute__((ext_vector_type(2)));
 typedef float p8_f32x2 __attribute__((ext_vector_type(2)));
 typedef float p8_f32x4 __attribute__((ext_vector_type(4)));
+
+// bf16 parts of a probability, by those of a query
+__host__ __device__ constexpr int p8_prob_parts(int ns) { return ns == 1 ? 2 : ns; }
 
 constexpr int P8_UNIT = 256, P8_CHUNK = 2048, P8_UNITS = P8_CHUNK / P8_UNIT;
 
@@ -216,7 +220,7 @@ struct P8Query<NQ, NSTEP, NS, true> {
 // NQ q-tiles of 16 rows (row r0 + 16 i + lane % 16) and their softmax state.
 template <int DP, int NQ, int NS, bool QL>
 struct P8State {
-    static constexpr int NSTEP = DP / 32, NDT = DP / 16;
+    static constexpr int NSTEP = DP / 32, NDT = DP / 16, PS = p8_prob_parts(NS);
     P8Query<NQ, NSTEP, NS, QL> q;
     p8_f32x4 acc[NQ][NDT];
     float m[NQ], l[NQ];      // l: the lane's own keys
@@ -304,7 +308,7 @@ struct P8State {
     // sums with it) only when a score is more than 2^8 times as likely: a maximum that moves with every record would
     // have the 16 rows rescale their sums in almost every one of a unit's eight steps. The reference is a function of
     // the row's own scores, and a probability of up to 256 is as exact as one of up to 1.
-    __device__ __forceinline__ void softmax(float (&p)[NQ][8], p8_bf16x8 (&ph)[NQ][NS], float qscale) {
+    __device__ __forceinline__ void softmax(float (&p)[NQ][8], p8_bf16x8 (&ph)[NQ][PS], float qscale) {
 #pragma unroll
         for (int i = 0; i < NQ; ++i) {
             float mx = p[i][0];
@@ -332,14 +336,14 @@ struct P8State {
             }
             l[i] += sum;
 #pragma unroll
-            for (int k = 0; k < 8; k += 2) p8_split<NS>(p[i][k], p[i][k + 1], ph[i], k);
+            for (int k = 0; k < 8; k += 2) p8_split<PS>(p[i][k], p[i][k + 1], ph[i], k);
         }
     }
     // O^T += V^T . P^T of keys that some rows do not see (their P is 0, and 0 * NaN is NaN): what is not finite in V
     // stays out of the product, and then, rarely, marks the channels of the rows that do see it. vis: the lane's keys'
     // bits of its row.
     template <class Keys>
-    __device__ __forceinline__ void values_masked(const Keys& x, const p8_bf16x8 (&ph)[NQ][NS], const uint32_t (&vis)[NQ]) {
+    __device__ __forceinline__ void values_masked(const Keys& x, const p8_bf16x8 (&ph)[NQ][PS], const uint32_t (&vis)[NQ]) {
         auto odd = [](uint32_t u) {   // a mask of the halves that are no finite bf16
             return ((u & 0x7f80) == 0x7f80 ? 0xffffu : 0u) | ((u & 0x7f800000) == 0x7f800000 ? 0xffff0000u : 0u);
         };
@@ -353,7 +357,7 @@ struct P8State {
 #pragma unroll
             for (int i = 0; i < NQ; ++i)
 #pragma unroll
-                for (int j = 0; j < NS; ++j)
+                for (int j = 0; j < PS; ++j)
                     acc[i][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(p8_bf16x8, w), ph[i][j], acc[i][dt], 0, 0, 0);
         }
         if (!__any(any != 0)) return;
@@ -393,7 +397,7 @@ struct P8State {
     template <bool MASK, class Keys, class Next>
     __device__ __forceinline__ void step(const Keys& x, int kb, float qscale, Next next_k) {
         float p[NQ][8];
-        p8_bf16x8 ph[NQ][NS];
+        p8_bf16x8 ph[NQ][PS];
         scores(x, p);
         next_k();
         uint32_t vis[NQ];
@@ -414,7 +418,7 @@ struct P8State {
 #pragma unroll
             for (int i = 0; i < NQ; ++i)
 #pragma unroll
-                for (int j = 0; j < NS; ++j) acc[i][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, ph[i][j], acc[i][dt], 0, 0, 0);
+                for (int j = 0; j < PS; ++j) acc[i][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, ph[i][j], acc[i][dt], 0, 0, 0);
         }
     }
     // The rows' own blocks: keys lim <= k <= last. past: the first position that holds no row (stale memory from there).
@@ -422,7 +426,7 @@ struct P8State {
         constexpr int NW = P8Bf16<DP>::NW, NP = P8Bf16<DP>::NP;
         const int g = lane / 16;
         float p[NQ][8];
-        p8_bf16x8 ph[NQ][NS];
+        p8_bf16x8 ph[NQ][PS];
         scores(x, p);
         uint32_t vis[NQ];
 #pragma unroll
@@ -548,8 +552,8 @@ __device__ __forceinline__ void p8_zero_rows(const P8Args& A, const P8Rows& R, i
 
 // ---------------------------------------------------------------- few rows: a workgroup streams its chunks
 // Two float32 q-tiles' queries of 128 channels would take 96 registers of the 256 that two waves per SIMD have, bf16 ones
-// 32 that spill; the eight waves share them in LDS instead (5 rows of 4 heads each, batch 32, context 32k, bf16: 502 us
-// with registers, 465 so).
+// 32 that spill; the eight waves share them in LDS instead (5 rows of 4 heads each, batch 32, context 32k, bf16, with one
+// part of the probabilities: 502 us with registers, 465 so).
 __host__ __device__ constexpr bool p8_query_in_lds(int dp, int nq, int ns) { return nq * (dp / 32) * ns > 16 || nq * (dp / 32) >= 8; }
 __host__ __device__ constexpr size_t p8_chunk_lds(int dp, int nq, int ns) {
     return (size_t)P8_UNITS * nq * ((dp / 16) * 1024 + 16 * sizeof(float2)) +
@@ -557,8 +561,8 @@ __host__ __device__ constexpr size_t p8_chunk_lds(int dp, int nq, int ns) {
 }
 // Grid (KV head x sequence, q-group, run of chunks or own blocks). Eight waves, one unit of a chunk each, straight from
 // memory to registers; their states meet in LDS and leave as the chunk's. Bound by memory: 32 sequences of 32700 tokens, 8
-// KV heads of 128, one token each, bf16, 373 us (5.8 TB/s); 5 rows of 4 heads each, bf16, 465, float32 (three products
-// for one, on 32 rows for 20: 295 us of matrix instructions) 505 to 540.
+// KV heads of 128, one token each, bf16, 383 us (5.6 TB/s), float32 403; 5 rows of 4 heads each, bf16, 472, float32 (three
+// products for one, on 32 rows for 20: 295 us of matrix instructions) 505 to 540.
 // ONE: all keys lie in one chunk, and the workgroup takes the rows' own blocks too (its last wave, which few contexts
 // give a unit) and writes out: the merge would cost as much again as a short context's attention.
 template <int DP, int NQ, int NS, bool ONE>
@@ -687,8 +691,9 @@ __global__ void __launch_bounds__(512) paged8_chunk_kernel(P8Args A) {
 // workgroup, into LDS in operand order, two stages deep with the next step's codes in registers: a wave's own
 // conversion (64 instructions a step) would cost as much as half its softmax, and its loads 8 KB of L1 each. Of a
 // wave's state the unit's and the chunk's sums are registers, the sums over the chunks before lie in LDS (touched once
-// in 2048 keys). A prompt of 4096 tokens, 32 / 8 heads of 128: bf16 230 to 245 us (580 TFLOP/s), float32 420. A step of
-// 32 keys takes 1.3 us where its products alone take 0.4: the eight waves come to their products, their exponentials and
+// in 2048 keys). A prompt of 4096 tokens, 32 / 8 heads of 128: bf16 266 us (517 TFLOP/s; with one part of the
+// probabilities, a third fewer products, 225), float32 425 to 443. A step of 32 keys takes 1.5 us in bf16 where its
+// products alone take 0.6: the eight waves come to their products, their exponentials and
 // their LDS reads together, and registers leave no room to run one step's products under another's softmax.
 template <int DP>
 struct P8Staged {
@@ -964,13 +969,13 @@ __host__ constexpr int p8_walk_tiles(int dp, int ns) { return dp > 128 || ns > 1
 // Which kernel, where either could take the rows: the one that a model of their times says is faster. A workgroup that
 // streams a chunk needs `full` us for its 2048 keys where every CU has one, and `base` however few keys it has (half of
 // that where CUs stay free); a walking one, of many more rows, 12 us and `step` per 32 keys. Measured, streaming against
-// walking, us: 32 / 8 heads of 128, bf16, one sequence: 400 rows on no context 20 / 33, 1600 rows 78 / 89; on 2000 keys
-// 100 rows 22 / 104, 400 rows 56 / 110, 1600 rows 205 / 174; four sequences, 400 rows on 2000 keys 186 / 137. 9 / 3
-// heads of 64, float32: 50 rows on 8000 keys 27 / 71, 800 rows 112 / 98.
+// walking, us: 32 / 8 heads of 128, bf16, one sequence: 400 rows on no context 22 / 36, 1600 rows 91 / 105; on 2000 keys
+// 100 rows 25 / 121, 400 rows 63 / 129, 1600 rows 231 / 206; four sequences, 400 rows on 2000 keys 202 / 163. 9 / 3
+// heads of 64, float32: 400 rows on 8000 keys 60 / 84, 1600 rows 183 / 167.
 static bool p8_walks(const dkv_paged8_t& c, int64_t tiles, int T, int max_len, int nq, int slots, int per_slot, int ns) {
     const int dp = p8_dp(c.head_dim), at = dp == 32 ? 0 : dp / 64;
     static const float base[2][5] = {{9, 12, 13, 13, 15}, {14, 23, 20, 18, 25}}, full[2][5] = {{12, 16, 26, 19, 24}, {19, 30, 40, 27, 36}},
-                       step[2][5] = {{.8f, .9f, 1.45f, 1.f, 1.2f}, {.7f, .9f, 1.45f, 1.45f, 2.2f}};
+                       step[2][5] = {{.9f, 1.1f, 1.75f, 1.2f, 1.5f}, {.7f, .9f, 1.45f, 1.45f, 2.2f}};
     const int64_t heads = (int64_t)c.n_kv_heads * c.batch, groups = (tiles + nq - 1) / nq;
     if (groups > 65535) return true;
     const float keys = (float)std::max(1, max_len - T / 2), chunks = keys / P8_CHUNK;   // of a row, on average

@@ -172,7 +172,7 @@ int dkv_paged8_append(const dkv_paged8_t* cache, int32_t layer, const void* k, c
  * append before it wrote (same T, start and count). q and out: DKV_F32 or
  * DKV_BF16 (q_dtype both), [batch][T][Hq][D]. float32 queries and
  * probabilities enter the products in three bf16 parts, bf16 queries whole
- * and their probabilities rounded to bf16; sums are float32. Keys are cut
+ * and their probabilities in two; sums are float32. Keys are cut
  * at absolute positions into units of 256 and chunks of 2048 that fold in
  * order, the query's own block last: a row's result depends neither on T nor
  * on the launch. A padding row t >= count[s] sees what the last row does, and

@@ -213,6 +213,29 @@ def test_attention_against_64_bits(dev, shape, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(64, 1, 4, 16, 700, 1), (128, 1, 4, 16, 2500, 5), (128, 2, 4, 64, 300, 40), (256, 1, 2, 32, 400, 3),
+                                   (192, 1, 1, 16, 2100, 9), (24, 1, 3, 128, 900, 30)], ids=lambda s: f"d{s[0]}n{s[4]}t{s[5]}")
+def test_bf16_queries_are_off_by_the_outputs_rounding(dev, shape):
+    """The probabilities of bf16 queries hold 16 bits: half a step of the bf16 output (2^-8 of it) is all that may show.
+    Scores near each other, so that many keys take part and their values cancel."""
+    D, H, G, bs, have, T = shape
+    g = torch.Generator(device=dev)
+    g.manual_seed(D + have)
+    n = have + T
+    k, v = (torch.randn(1, n, H, D, generator=g, device=dev) for _ in range(2))
+    q = (0.2 * torch.randn(1, T, H * G, D, generator=g, device=dev)).to(BF16)
+    c = new_cache(H, D, bs, n)
+    c.reserve([n])
+    fill(c, k, v, [have])
+    out = c.append_attend(0, q, k[:, have:].contiguous(), v[:, have:].contiguous(), i32([have]), n)[0].double().cpu()
+    k16, v16 = k[0].to(BF16).cpu(), v[0].to(BF16).cpu()
+    want, top = attention(q[0].cpu(), k16, v16, have, bs)
+    size, _ = attention(q[0].cpu(), k16, v16.abs(), have, bs)       # sum of p |v|
+    # two bf16 parts of a probability leave 2^-8 of 2^-8 of it; float32 sums and scores as in bound()
+    assert ((out - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -16 * size + bound(F32, n, D, top, size, None)).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("D,H,G,bs,n", [(128, 2, 4, 16, 2300), (64, 3, 3, 64, 700), (8, 1, 4, 16, 100), (256, 1, 1, 128, 520)])
 def test_rows_do_not_depend_on_the_call(dev, D, H, G, bs, n, dtype):
