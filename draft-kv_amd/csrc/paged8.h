@@ -11,7 +11,10 @@
 // or of rejected rows that were there in between (their block's codes are written again when it fills again). That is
 // what keeps greedy speculative decoding over this cache equal to plain decoding over it. The bf16 rows live in a ring
 // per (sequence, layer), the last tail_rows rows; an append of more rows than fit beside the open block also leaves
-// all its rows in `hot`, which the attention that follows reads instead.
+// all its rows in `hot`, which the attention that follows reads instead. Its last rows then take the places of the open
+// block's in the ring: those go to `held`, tile by tile with their position as a tag, so that the same append can be made
+// again (a forward that failed, a state that is run again). A tag says that held has the tile's newest rows; whoever
+// puts the tile's rows elsewhere takes it back.
 //
 // Tiles. 16 tokens of one (KV head, K or V), channels padded with zeros to DP = 32, 64, 128, 192 or 256, in panels of
 // PW = min(64, DP) channels. A panel holds PW / 4 values per lane, lane-major, in the order of the matrix
@@ -71,6 +74,24 @@ __device__ __forceinline__ uint16_t* p8_hot_tile(const dkv_paged8_t& c, int s, i
            (((int64_t)s * c.n_kv_heads + h) * tiles + (pos - base) / 16) * 32 * p8_dp(c.head_dim);
 }
 
+// A tile of the open block in held [batch][layer][head][block_size / 16], and behind it a tag for each (K or V, panel):
+// every one belongs to the one wave of an append that has that panel.
+__host__ __device__ inline int p8_panels(int dp) { return dp < 64 ? 1 : dp / 64; }
+__host__ __device__ inline int p8_held_stride(int dp) { return 64 * dp + (8 * p8_panels(dp) + 15) / 16 * 16; }
+__device__ __forceinline__ uint16_t* p8_held_tile(const dkv_paged8_t& c, int s, int layer, int h, int pos) {
+    const int64_t tile = (((int64_t)s * c.n_layers + layer) * c.n_kv_heads + h) * (c.block_size / 16) + pos % c.block_size / 16;
+    return reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(c.held) + tile * p8_held_stride(p8_dp(c.head_dim)));
+}
+__device__ __forceinline__ int32_t* p8_held_tag(const dkv_paged8_t& c, int s, int layer, int h, int pos, int kv, int panel) {
+    const int dp = p8_dp(c.head_dim);
+    return reinterpret_cast<int32_t*>(p8_held_tile(c, s, layer, h, pos) + 32 * dp) + kv * p8_panels(dp) + panel;
+}
+// bf16 tile at pos of the open block (outside an append all panels' tags agree)
+__device__ __forceinline__ const uint16_t* p8_open_tile(const dkv_paged8_t& c, int s, int layer, int h, int pos) {
+    return c.held && *p8_held_tag(c, s, layer, h, pos, 0, 0) == pos ? p8_held_tile(c, s, layer, h, pos)
+                                                                     : p8_ring_tile(c, s, layer, h, pos);
+}
+
 __device__ __forceinline__ const uint8_t* p8_block(const dkv_paged8_t& c, int s, int layer, int pos) {
     return static_cast<const uint8_t*>(c.pool) +
            c.block_table[((int64_t)s * c.n_layers + layer) * c.max_blocks + pos / c.block_size] *
@@ -91,14 +112,13 @@ __device__ __forceinline__ float p8_scale(uint32_t biased) { return __uint_as_fl
 __device__ __forceinline__ float p8_value(const dkv_paged8_t& c, int s, int layer, int pos, int len, int h, int d, int kv) {
     const int dp = p8_dp(c.head_dim);
     const int o = (kv ? p8_v_off(dp, pos % 16, d) : p8_k_off(dp, pos % 16, d)) + kv * 16 * dp;
-    if (pos >= len / c.block_size * c.block_size) return bf16_to_f32(p8_ring_tile(c, s, layer, h, pos / 16 * 16)[o]);
+    if (pos >= len / c.block_size * c.block_size) return bf16_to_f32(p8_open_tile(c, s, layer, h, pos / 16 * 16)[o]);
     const uint8_t* b = p8_block(c, s, layer, pos);
     const uint32_t code = b[p8_tile_off(c, h, pos % c.block_size) + o];
     // (the conversion yields a pair; a code is exact in bf16, and so is its product with the scale)
     const auto v = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(code, p8_scale(b[p8_scale_off(c, h) + kv]), false);
     return bf16_to_f32(__builtin_bit_cast(uint32_t, v) & 0xffff);
 }
-
 
 int p8_check(const dkv_paged8_t* c, int layer, const char* fn);
 int p8_check_hot(const dkv_paged8_t& c, int T, const char* fn);

@@ -19,8 +19,8 @@ int p8_check(const dkv_paged8_t* c, int layer, const char* fn) {
     if (layer < 0 || layer >= c->n_layers) return fail(DKV_EINVAL, f + ": layer out of range");
     if (c->n_kv_heads > 32767 || c->batch > 65535) return fail(DKV_EINVAL, f + ": too many heads or sequences");
     if (reinterpret_cast<uintptr_t>(c->pool) % 16 || reinterpret_cast<uintptr_t>(c->tail) % 16 ||
-        reinterpret_cast<uintptr_t>(c->hot) % 16)
-        return fail(DKV_EINVAL, f + ": pool, tail and hot must be 16-byte aligned");
+        reinterpret_cast<uintptr_t>(c->hot) % 16 || reinterpret_cast<uintptr_t>(c->held) % 16)
+        return fail(DKV_EINVAL, f + ": pool, tail, hot and held must be 16-byte aligned");
     return DKV_OK;
 }
 
@@ -38,8 +38,9 @@ int p8_check_hot(const dkv_paged8_t& c, int T, const char* fn) {
 // values that it stores (K: PB channels of a token; V: four tokens of PB / 4 channels), so nothing is transposed and the
 // rows stay in registers from the load to the codes. They go to the ring or to hot as bf16 and, where the block is now
 // full, into codes: one maximum over the block, then a conversion per pair. The inputs are read once; rows that the
-// block held before come from the ring. Bound by that traffic for a prompt (4096 tokens, 8 heads of 128, float32 in, 59
-// MB: 19 us, 3.1 TB/s), by the latency of a load and a store for single tokens.
+// block held before come from the ring, or from held, and go back to the ring where this append leaves them room. Bound
+// by that traffic for a prompt (4096 tokens, 8 heads of 128, float32 in, 59 MB: 19 us, 3.1 TB/s), by the latency of a
+// load and a store for single tokens.
 constexpr int AP_WAVES = 8;
 
 __device__ __forceinline__ uint32_t p8_biased_exponent(uint32_t amax_bits) {
@@ -122,12 +123,19 @@ struct ApRows {
 };
 
 template <class X, bool VEC, int PB>
-__global__ void __launch_bounds__(64 * AP_WAVES) paged8_append_kernel(dkv_paged8_t c, int layer, const X* __restrict__ k,
+__global__ void __launch_bounds__(64 * AP_WAVES, 8) paged8_append_kernel(dkv_paged8_t c, int layer, const X* __restrict__ k,
                                                                       const X* __restrict__ v, int T, bool in_ring,
                                                                       const int32_t* __restrict__ start,
                                                                       const int32_t* __restrict__ count) {
     constexpr int PW = 4 * PB, UNITS = 4;   // panels per wave: 8 tiles of 4 panels over 8 waves
     const int h = blockIdx.y >> 1, kv = blockIdx.y & 1, s = blockIdx.z, D = c.head_dim, DP = p8_dp(D), bs = c.block_size;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), lane = threadIdx.x % WAVE, waves = blockDim.x / WAVE;
+    const int panels = DP / PW;   // unit u: panel u % panels of tile u / panels; a wave has the units wave + x * waves
+    int tag = -1;                 // lane x: the first block's tag of unit x
+    if (c.held && blockIdx.x == 0 && lane < UNITS && wave + lane * waves < bs / 16 * panels) {
+        const int u = wave + lane * waves;
+        tag = *p8_held_tag(c, s, layer, h, u / panels * 16, kv, u % panels);
+    }
     const int s0 = start[s], n = p8_new_rows(c, T, s0, count, s), end = s0 + n;
     const int base = s0 / bs * bs, p0 = base + blockIdx.x * bs;   // the block's first position
     if (n <= 0 || p0 >= end) return;
@@ -135,8 +143,6 @@ __global__ void __launch_bounds__(64 * AP_WAVES) paged8_append_kernel(dkv_paged8
     const int new0 = max(p0, s0), new1 = min(p0 + bs, end);
     // tiles to put together: all of the block where it is coded or moves to hot, else those with new rows
     const int t0 = sealed || !in_ring ? 0 : (new0 - p0) / 16, t1 = (new1 - p0 + 15) / 16;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), lane = threadIdx.x % WAVE, waves = blockDim.x / WAVE;
-    const int panels = DP / PW;
     // (looked up here: beside the loads of the rows, not behind them)
     uint8_t* block = sealed ? const_cast<uint8_t*>(p8_block(c, s, layer, p0)) : nullptr;
     const ApRows<X, VEC, PB> rows{(kv ? v : k) + ((int64_t)s * T * c.n_kv_heads + h) * D, (int64_t)c.n_kv_heads * D,
@@ -148,16 +154,33 @@ __global__ void __launch_bounds__(64 * AP_WAVES) paged8_append_kernel(dkv_paged8
     };
     const int last = (end - 1) / 16 * 16;                       // the last tile
     const int held = (s0 - base + 15) / 16 * 16;                // rows of the tiles that the first block reads in the ring
+    // Where held has a tile of the first block (rarely), it goes back to the ring, whose place nothing else touches. A tag
+    // of a later block is void, the sequence was cut before it: an append that goes on from here to that block has all
+    // the tiles of its first block here.
+    if (__any(tag >= base + bs || (tag >= base && tag < p0 + 16 * t1))) {
+        for (int x = 0; x < UNITS; ++x) {
+            const int u = wave + x * waves, i = u % panels, pos = p0 + 16 * (u / panels), was = __shfl(tag, x);
+            if (u >= t1 * panels) break;
+            if (was != pos && was < base + bs) continue;
+            if (lane == 0) *p8_held_tag(c, s, layer, h, pos, kv, i) = -1;
+            if (was != pos || pos >= s0) continue;
+            const uint16_t* from = at(p8_held_tile(c, s, layer, h, pos), i) + lane * PB;
+            uint16_t* to = at(p8_ring_tile(c, s, layer, h, pos), i) + lane * PB;
+#pragma unroll
+            for (int e = 0; e < PB / 8; ++e) reinterpret_cast<uint4*>(to)[e] = reinterpret_cast<const uint4*>(from)[e];
+        }
+    }
     __align__(16) uint32_t r[UNITS][PB / 2];
 #pragma unroll
     for (int x = 0; x < UNITS; ++x) {
-        const int u = wave + x * waves, t = t0 + u / panels, i = u % panels, pos = p0 + 16 * t;
-        if (t < t1) rows.load(pos, i, at(p8_ring_tile(c, s, layer, h, pos), i), r[x]);
+        const int u = wave + x * waves, t = u / panels, i = u % panels, pos = p0 + 16 * t;
+        if (t >= t0 && t < t1) rows.load(pos, i, at(p8_ring_tile(c, s, layer, h, pos), i), r[x]);
     }
 #pragma unroll
     for (int x = 0; x < UNITS; ++x) {
-        const int u = wave + x * waves, t = t0 + u / panels, i = u % panels, pos = p0 + 16 * t;
+        const int u = wave + x * waves, t = u / panels, i = u % panels, pos = p0 + 16 * t;
         if (t >= t1) break;
+        if (t < t0) continue;
         if (!in_ring) put(at(p8_hot_tile(c, s, h, pos, base), i), r[x]);
         // the ring keeps the last tail_rows rows. A tile whose place there holds rows that the first block still
         // reads is left to the wave that reads them
@@ -169,6 +192,10 @@ __global__ void __launch_bounds__(64 * AP_WAVES) paged8_append_kernel(dkv_paged8
                 __align__(16) uint32_t y[PB / 2];
                 rows.load(later, i, nullptr, y);
                 put(at(p8_ring_tile(c, s, layer, h, later), i), y);
+                if (c.held) {
+                    put(at(p8_held_tile(c, s, layer, h, pos), i), r[x]);
+                    if (lane == 0) *p8_held_tag(c, s, layer, h, pos, kv, i) = pos;
+                }
             }
         }
     }
@@ -231,7 +258,7 @@ __global__ void __launch_bounds__(256) paged8_read_kernel(dkv_paged8_t c, int la
     const uint16_t* tail = nullptr;
     const uint8_t* code = nullptr;
     float scale = 0.0f;
-    if (ring) tail = p8_ring_tile(c, s, layer, h, (int)p0) + kv * 16 * DP;
+    if (ring) tail = p8_open_tile(c, s, layer, h, (int)p0) + kv * 16 * DP;
     else if (any) {
         const uint8_t* b = p8_block(c, s, layer, (int)p0);
         code = b + p8_tile_off(c, h, (int)(p0 % c.block_size)) + kv * 16 * DP;
@@ -282,6 +309,12 @@ extern "C" int64_t dkv_paged8_row_bytes(int32_t n_kv_heads, int32_t head_dim) {
 
 extern "C" int32_t dkv_paged8_hot_rows(const dkv_paged8_t* cache, int32_t T) {
     return !cache || T < 1 ? 0 : dkv::p8_hot_rows(*cache, T);
+}
+
+extern "C" int64_t dkv_paged8_held_bytes(const dkv_paged8_t* cache) {
+    using namespace dkv;
+    if (!cache || cache->batch < 1 || cache->n_layers < 1 || cache->n_kv_heads < 1 || cache->head_dim < 1 || cache->block_size < 16) return 0;
+    return (int64_t)cache->batch * cache->n_layers * cache->n_kv_heads * (cache->block_size / 16) * p8_held_stride(p8_dp(cache->head_dim));
 }
 
 extern "C" int dkv_paged8_append(const dkv_paged8_t* cache, int32_t layer, const void* k, const void* v,

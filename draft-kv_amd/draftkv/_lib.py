@@ -30,7 +30,7 @@ class Paged8(C.Structure):
     _fields_ = [("pool", C.c_void_p), ("block_table", C.c_void_p), ("tail", C.c_void_p), ("hot", C.c_void_p),
                 ("batch", C.c_int32), ("n_layers", C.c_int32), ("n_kv_heads", C.c_int32),
                 ("head_dim", C.c_int32), ("block_size", C.c_int32), ("max_blocks", C.c_int32),
-                ("tail_rows", C.c_int32), ("hot_rows", C.c_int32)]
+                ("tail_rows", C.c_int32), ("hot_rows", C.c_int32), ("held", C.c_void_p)]
 
 
 class Drafter(C.Structure):
@@ -55,6 +55,7 @@ _SIGS = {
     "dkv_paged8_block_bytes": (I64, [I32, I32, I32]),
     "dkv_paged8_row_bytes": (I64, [I32, I32]),
     "dkv_paged8_hot_rows": (I32, [PPaged8, I32]),
+    "dkv_paged8_held_bytes": (I64, [PPaged8]),
     "dkv_paged8_append": (C.c_int, [PPaged8, I32, P, P, I32, I32, P, P, P]),
     "dkv_paged8_attention_workspace": (SZ, [PPaged8, I32, I32, I32]),
     "dkv_paged8_attention": (C.c_int, [PPaged8, I32, P, I32, I32, I32, P, P, I32, P, P, SZ, P]),

@@ -303,6 +303,8 @@ class Decoder:
                 raise ValueError(f"sequence {s}: rows must be appended at the cache end "
                                  f"(start {st[s]}, cache holds {have[s]})")
         cache.reserve(ct)
+        if cache.fp8:
+            cache._writing(ct[:, None], slice(None))
         start_d = ops.to_device(st.astype(np.int32), self.device)
         count_d = None if np.all(ct == T) else ops.to_device(ct.astype(np.int32), self.device)
         attn = self.paged_attn(cache, start_d, count_d, max_pos)

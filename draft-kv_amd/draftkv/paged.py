@@ -171,6 +171,9 @@ class PagedKVCache:
         self.hot = torch.empty((self.batch, 0, self._row_bytes), **kw)      # rows of long appends, grown by need
         self._hot_of: Optional[tuple] = None       # (layer, T) of the append whose rows are there
         self._hot_kept: list = []                  # buffers that captured graphs still write to
+        # an open block's rows whose places in the tail a long append took (0xff: none)
+        shape = Paged8(batch=self.batch, n_layers=self.n_layers, n_kv_heads=H, head_dim=D, block_size=bs)
+        self.held = torch.full((int(lib().dkv_paged8_held_bytes(shape)),), 255, **kw)
         # the first position whose bf16 row is still there, per (sequence, layer)
         self.tail_from = np.zeros((self.batch, self.n_layers), np.int64)
 
@@ -195,6 +198,13 @@ class PagedKVCache:
             self._hot_kept.append(self.hot)
         self._hot_of = (layer, T)
 
+    def _writing(self, counts: np.ndarray, layers) -> None:
+        """counts [batch, ...] rows are about to be written to ``layers``: what the tail then lacks is gone whether they
+        are committed or not (a forward that fails), but for the open block, which a long append keeps."""
+        n = self.n_tokens[:, layers]
+        gone = np.minimum(-(-(n + counts) // 16) * 16 - self.tail_rows, n // self.block_size * self.block_size)
+        self.tail_from[:, layers] = np.maximum(self.tail_from[:, layers], np.where(counts > 0, gone, 0))
+
     def _written(self, end: np.ndarray, layers) -> None:
         """Rows up to end [batch, ...] are in ``layers``: the tail holds the last tail_rows (whole 16s) of them."""
         self.tail_from[:, layers] = np.maximum(self.tail_from[:, layers], -(-end // 16) * 16 - self.tail_rows)
@@ -204,7 +214,7 @@ class PagedKVCache:
         if self.fp8:
             return Paged8(self.store.data_ptr(), self.d_tables.data_ptr(), self.tail.data_ptr(), self.hot.data_ptr(),
                           self.batch, self.n_layers, self.n_heads, self.d_head, self.block_size, self.max_blocks,
-                          self.tail_rows, self.hot.shape[1])
+                          self.tail_rows, self.hot.shape[1], self.held.data_ptr())
         return Paged(self.store.data_ptr(), self.d_tables.data_ptr(), self.batch, self.n_layers, self.n_heads,
                      self.d_head, self.block_size, self.max_blocks,
                      DKV_BF16 if self.dtype == torch.bfloat16 else DKV_F32)
@@ -339,6 +349,8 @@ class PagedKVCache:
         self._ensure_capacity(0, layer, T)
         self._upload()
         st = torch.tensor([start], dtype=torch.int32, device=self.device)
+        if self.fp8:
+            self._writing(np.array([T]), layer)
         self.append_layer(layer, k.float().contiguous()[None], v.float().contiguous()[None], st)
         self.n_tokens[0, layer] += T
         if self.fp8:
@@ -355,6 +367,7 @@ class PagedKVCache:
             d.batch = 1
             d.block_table += 4 * seq * self.n_layers * self.max_blocks
             d.tail += seq * self.tail[0].numel()
+            d.held += seq * (self.held.numel() // self.batch)
             at = torch.tensor([0, n], dtype=torch.int32, device=self.device)
             k, v = ops.paged8_read(d, layer, at[:1], at[1:], n)
             return k[0].cpu().numpy(), v[0].cpu().numpy(), np.arange(n, dtype=np.int64)

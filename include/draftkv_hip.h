@@ -145,22 +145,28 @@ int dkv_paged_attention(const dkv_paged_t* cache, int32_t layer, const float* q,
  * calls whose rows do not fit the ring beside an open block
  * (dkv_paged8_hot_rows(cache, T) > 0: hot_rows must be at least that); it is
  * written by the append and read by the attention of the same layer that
- * follows it on the stream. Rolling back: an append may start at any earlier
+ * follows it on the stream. held: the rows of the open block that such an
+ * append found in the ring and whose places its last rows took, so that an
+ * append may start there again (a forward that is run again);
+ * dkv_paged8_held_bytes() bytes, 16-byte aligned, filled with 0xff at first;
+ * or NULL: none kept. Rolling back: an append may start at any earlier
  * position p that is a multiple of block_size, or whose block's rows are
  * still in the ring (block start >= the rows ever written, rounded up to 16,
- * minus tail_rows). head_dim 1..256. The layout inside blocks and rows is
- * described in draft-kv_amd/csrc/paged8.h. */
+ * minus tail_rows) or in held. head_dim 1..256. The layout inside blocks and
+ * rows is described in draft-kv_amd/csrc/paged8.h. */
 typedef struct {
     void* pool;
     const int32_t* block_table;
     void* tail;
     void* hot;
     int32_t batch, n_layers, n_kv_heads, head_dim, block_size, max_blocks, tail_rows, hot_rows;
+    void* held;
 } dkv_paged8_t;
 
 int64_t dkv_paged8_block_bytes(int32_t n_kv_heads, int32_t head_dim, int32_t block_size);
 int64_t dkv_paged8_row_bytes(int32_t n_kv_heads, int32_t head_dim);
 int32_t dkv_paged8_hot_rows(const dkv_paged8_t* cache, int32_t T);
+int64_t dkv_paged8_held_bytes(const dkv_paged8_t* cache);
 
 /* dkv_paged_append for this cache: same arguments. A sequence whose rows would
  * lie outside its block table gets none (and no result from the attention:

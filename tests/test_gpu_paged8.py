@@ -638,6 +638,100 @@ def test_engine_over_it_is_lossless(dev, family, dtype, temperature):
             assert all(len(t) == len(p) + 40 for t, p in zip(got, prompts))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("bs,tail,D,H", [(16, 32, 64, 2), (16, 128, 24, 1), (64, 96, 128, 1), (128, 144, 256, 1), (32, 64, 192, 1)])
+def test_appends_made_again(dev, bs, tail, D, H):
+    """An append that is not committed may be made again from the same start, or another one in its place, however long:
+    the rows before it are there (its open block's, whose places in the tail a long append takes, too)."""
+    g = torch.Generator(device=dev)
+    g.manual_seed(bs + D)
+    rng = np.random.default_rng(bs + tail + D)
+    size = 900
+    c = new_cache(H, D, bs, size, tail_rows=tail)
+    c.reserve([size])
+    k, v = rows_of(g, 1, size, H, D, dev)      # the rows that are there, [0, n)
+    n, left = 0, 0                              # left: the first row that the tail still holds
+
+    def check(n):
+        gk, gv = c.read_rows(0, i32([0]), i32([n]), n + 1)
+        for got, x in ((gk, k), (gv, v)):
+            assert torch.equal(got[0, :n].double().cpu(), values(x[0, :n].to(BF16).cpu(), bs)), n
+
+    def append(T, fresh):
+        nonlocal k, v
+        if fresh:                               # other rows from n on
+            k2, v2 = rows_of(g, 1, T, H, D, dev)
+            k[:, n:n + T], v[:, n:n + T] = k2, v2
+        q = torch.randn(1, T, H, D, generator=g, device=dev)
+        return [c.append_attend(0, q, k[:, n:n + T].contiguous(), v[:, n:n + T].contiguous(), i32([n]), n + T) for _ in range(2)]
+
+    for _ in range(40):
+        if n > 500:                             # another sequence in this one's place
+            n = left = 0
+        for again in range(int(rng.integers(1, 4))):
+            T = int(rng.choice([1, 3, 17, tail - bs + 2, tail + 5, tail + 2 * bs + 9]))
+            a, b = append(T, again > 0)
+            assert torch.equal(a, b), (n, T)
+            check(n)
+            left = max(left, min(-(-(n + T) // 16) * 16 - tail, n // bs * bs))
+        n += T
+        left = max(left, -(-n // 16) * 16 - tail)
+        check(n)
+        if rng.random() < 0.4:                  # a rollback, within the rows that are left or to a block's end
+            cut = int(rng.integers(max(n - 20, 0), n + 1))
+            n = cut if cut // bs * bs >= left else cut // bs * bs
+            left = min(left, n)
+            check(n)
+
+
+@pytest.mark.gpu
+def test_a_forward_that_fails_leaves_the_cache_as_it_was(dev, monkeypatch):
+    """A long forward that fails after some layers took its rows: what the cache holds, the mirror from it and the forward
+    that follows are those of a cache that never saw it; rollbacks past the open block are refused, its rows are gone."""
+    from draftkv import CompressionConfig
+    from draftkv.compress import CompressedKVCache
+    from draftkv.llama import demo_llama
+    model = demo_llama(dtype=F32, device=dev)
+    model.kv_dtype = F8
+    toks = np.random.default_rng(5).integers(0, 128, size=500)
+    full, ref = model.new_cache(max_tokens=1000), model.new_cache(max_tokens=1000)
+    for c in (full, ref):
+        model.forward(toks[:100], c, 0)
+        model.forward(toks[100:150], c, 100)
+    calls = 0
+    real = model._mlp_inner
+
+    def fails(x, p):
+        nonlocal calls
+        calls += 1
+        if calls == 2:
+            raise MemoryError("out of memory")
+        return real(x, p)
+
+    monkeypatch.setattr(model, "_mlp_inner", fails)
+    with pytest.raises(MemoryError):
+        model.forward(toks[150:450], full, 150)
+    monkeypatch.undo()
+    assert full.length == 150
+    for L in range(model.n_layers):
+        for a, b in zip(full.read(L), ref.read(L)):
+            assert np.array_equal(a, b)
+    mirrors = [CompressedKVCache(model.n_layers, CompressionConfig(8, 1.0), device=dev) for _ in range(2)]
+    for start in (0, 130):
+        for m, c in zip(mirrors, (full, ref)):
+            m.sync_from(c, start)
+        for L in range(model.n_layers):
+            for a, b in zip(mirrors[0].read(L), mirrors[1].read(L)):
+                assert np.array_equal(a, b)
+    with pytest.raises(ValueError, match="gone"):
+        full.truncate(143)                  # rows 128 .. 143 were in the tail before, 144 on are the open block
+    for lo, hi in ((150, 155), (155, 450)):
+        assert np.array_equal(model.forward(toks[lo:hi], full, lo), model.forward(toks[lo:hi], ref, lo))
+    full.truncate(445)
+    ref.truncate(445)
+    assert np.array_equal(model.forward(toks[445:446], full, 445), model.forward(toks[445:446], ref, 445))
+
+
 # ---------------------------------------------------------------- refusals (no GPU)
 def _desc(**kw):
     from draftkv import _lib
@@ -686,6 +780,18 @@ def test_bad_calls_are_refused():
     err(L.dkv_paged8_read(r, 0, 16, None, 1, 16, 16, None), -1, "NULL")
     assert L.dkv_paged8_append(r, 0, 16, 16, 0, 0, 16, None, None) == 0
     assert L.dkv_paged8_hot_rows(r, 113) == 0 and L.dkv_paged8_hot_rows(r, 114) == 144
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="made-up pointers: host checks only")
+def test_held_rows_are_checked():
+    import ctypes as C
+    from draftkv import _lib
+    L, d = _lib.lib(), _desc(held=24)
+    assert L.dkv_paged8_append(C.byref(d), 0, 16, 16, 0, 1, 16, None, None) == -1 and "held" in L.dkv_last_error().decode()
+    for kw, tile in ((dict(head_dim=64), 4096 + 16), (dict(head_dim=8), 2048 + 16), (dict(head_dim=200, block_size=32), 16384 + 32)):
+        d = _desc(batch=3, n_layers=5, **kw)
+        assert L.dkv_paged8_held_bytes(C.byref(d)) == 3 * 5 * 2 * d.block_size // 16 * tile
+    assert L.dkv_paged8_held_bytes(None) == 0 and L.dkv_paged8_held_bytes(C.byref(_desc(head_dim=0))) == 0
 
 
 def test_tensors_on_another_device_are_refused():
