@@ -97,6 +97,11 @@ def _torch_dtype(dtype) -> torch.dtype:
     raise ValueError(f"unsupported cache dtype {dtype!r} (float32, bfloat16 or float8_e4m3fn)")
 
 
+def _version(t: Optional[torch.Tensor]) -> int:
+    """Counts the changes of a tensor in place (0 where torch does not: none, or an inference tensor)."""
+    return 0 if t is None or t.is_inference() else t._version
+
+
 def auto_chunk_keys(batch: int, n_heads: int, max_tokens: int) -> int:
     """Keys per chunk of the verify/decode attention kernel: about 1024
     chunks (four per CU) over the cache's capacity, a power of two in
@@ -168,9 +173,10 @@ class PagedKVCache:
         kw = dict(dtype=torch.uint8, device=self.device)
         self.store = torch.empty((self.batch * self.n_blocks, int(lib().dkv_paged8_block_bytes(H, D, bs))), **kw)
         self.tail = torch.empty((self.batch, self.n_layers, self.tail_rows, self._row_bytes), **kw)
-        self.hot = torch.empty((self.batch, 0, self._row_bytes), **kw)      # rows of long appends, grown by need
-        self._hot_of: Optional[tuple] = None       # (layer, T) of the append whose rows are there
-        self._hot_kept: list = []                  # buffers that captured graphs still write to
+        # rows of long appends, grown by need: of eager calls, and of captured ones, whose graphs keep theirs
+        self.hot = torch.empty((self.batch, 0, self._row_bytes), **kw)
+        self._graph_hot: list = []
+        self._hot_of: dict = {}                    # captured or not: the append whose rows are there
         # an open block's rows whose places in the tail a long append took (0xff: none)
         shape = Paged8(batch=self.batch, n_layers=self.n_layers, n_kv_heads=H, head_dim=D, block_size=bs)
         self.held = torch.full((int(lib().dkv_paged8_held_bytes(shape)),), 255, **kw)
@@ -182,21 +188,55 @@ class PagedKVCache:
             if t is not None and t.device != self.store.device:
                 raise ValueError(f"a tensor on {t.device} for a cache on {self.store.device}")
 
-    def _hot_room(self, layer: int, T: int) -> None:
-        """Room for an append of T rows that the tail does not hold beside an open block."""
-        if (self.block_size + T + 14) // 16 * 16 <= self.tail_rows:
-            return
-        need = int(lib().dkv_paged8_hot_rows(self.desc(), T))
+    def _long(self, T: int) -> bool:
+        """Whether an append of T rows is more than the tail holds beside an open block."""
+        return (self.block_size + T + 14) // 16 * 16 > self.tail_rows
+
+    def _append8(self, layer: int, k: torch.Tensor, v: torch.Tensor, start: torch.Tensor, count: Optional[torch.Tensor]) -> Paged8:
+        """The append, with its rows in a buffer too where it is long; the descriptor for their attention. Captured
+        appends have a buffer of their own: a replay must not change what an eager attend() reads."""
+        T = k.shape[1]
+        if not self._long(T):
+            if self._hot_of:      # (its rows may lie over those of the long one)
+                capturing = torch.cuda.is_current_stream_capturing()
+                if self._hot_of.get(capturing, (None,))[0] == layer:
+                    del self._hot_of[capturing]
+            d = self.desc()
+            ops.paged8_append(d, layer, k, v, start, count)
+            return d
         capturing = torch.cuda.is_current_stream_capturing()
-        if need > self.hot.shape[1]:
+        self._hot_of.pop(capturing, None)
+        need = int(lib().dkv_paged8_hot_rows(self.desc(), T))
+        hot = self.hot if not capturing else self._graph_hot[-1] if self._graph_hot else None
+        if hot is None or need > hot.shape[1]:
+            if hot is not None and hot.numel() and not capturing:
+                hot.record_stream(torch.cuda.current_stream(self.device))
+            hot = torch.empty((self.batch, need, self._row_bytes), dtype=torch.uint8, device=self.device)
             if capturing:
-                raise RuntimeError(f"append of {T} rows under graph capture: run one of that length before")
-            if self.hot.numel():
-                self.hot.record_stream(torch.cuda.current_stream(self.device))
-            self.hot = torch.empty((self.batch, need, self._row_bytes), dtype=torch.uint8, device=self.device)
-        elif capturing and not any(t is self.hot for t in self._hot_kept):
-            self._hot_kept.append(self.hot)
-        self._hot_of = (layer, T)
+                self._graph_hot.append(hot)
+            else:
+                self.hot = hot
+        d = self.desc(hot)
+        ops.paged8_append(d, layer, k, v, start, count)
+        self._hot_of[capturing] = (layer, T, *((t, _version(t)) for t in (start, count)))
+        return d
+
+    def _hot_rows_of(self, layer: int, T: int, start: torch.Tensor, count: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+        """The buffer with the rows of that append, or None where it is not the one whose rows are there."""
+        capturing = torch.cuda.is_current_stream_capturing()
+        of = self._hot_of.get(capturing)
+        if of is None or of[:2] != (layer, T):
+            return None
+        for (was, version), t in zip(of[2:], (start, count)):
+            if was is None and t is None:
+                continue
+            if _version(was) != version or capturing and t is not was:
+                return None
+            if t is not was:      # another tensor with the same values (the host waits for them)
+                a, b = (x if x is not None else torch.full_like(y, T) for x, y in ((was, t), (t, was)))
+                if (a.shape, a.dtype, a.device) != (b.shape, b.dtype, b.device) or not torch.equal(a, b):
+                    return None
+        return self.hot if not capturing else self._graph_hot[-1]
 
     def _writing(self, counts: np.ndarray, layers) -> None:
         """counts [batch, ...] rows are about to be written to ``layers``: what the tail then lacks is gone whether they
@@ -210,11 +250,12 @@ class PagedKVCache:
         self.tail_from[:, layers] = np.maximum(self.tail_from[:, layers], -(-end // 16) * 16 - self.tail_rows)
 
     # ------------------------------------------------------------ descriptor
-    def desc(self):
+    def desc(self, hot: Optional[torch.Tensor] = None):
         if self.fp8:
-            return Paged8(self.store.data_ptr(), self.d_tables.data_ptr(), self.tail.data_ptr(), self.hot.data_ptr(),
+            hot = self.hot if hot is None else hot
+            return Paged8(self.store.data_ptr(), self.d_tables.data_ptr(), self.tail.data_ptr(), hot.data_ptr(),
                           self.batch, self.n_layers, self.n_heads, self.d_head, self.block_size, self.max_blocks,
-                          self.tail_rows, self.hot.shape[1], self.held.data_ptr())
+                          self.tail_rows, hot.shape[1], self.held.data_ptr())
         return Paged(self.store.data_ptr(), self.d_tables.data_ptr(), self.batch, self.n_layers, self.n_heads,
                      self.d_head, self.block_size, self.max_blocks,
                      DKV_BF16 if self.dtype == torch.bfloat16 else DKV_F32)
@@ -283,8 +324,7 @@ class PagedKVCache:
         must have been reserved."""
         if self.fp8:
             self._here(k)
-            self._hot_room(layer, k.shape[1])
-            ops.paged8_append(self.desc(), layer, k, v, start, count)
+            self._append8(layer, k, v, start, count)
             return
         ops.paged_append(self.desc(), layer, k, v, start, count)
 
@@ -293,13 +333,18 @@ class PagedKVCache:
         """Causal attention of q [batch, T, heads, d_head] at positions start[s]..;
         count: the rows appended this forward when not all T (see append_layer).
         An 8-bit cache takes the queries of the rows that were just appended
-        (the same T, start and count), float32 or bfloat16."""
+        (the same T, start and count), float32 or bfloat16; of more rows than
+        its tail holds, only right after their append_layer(), both eager or
+        both captured, with start and count unchanged (a captured pair with
+        the same tensors)."""
         if self.fp8:
             self._here(q)
             T = q.shape[1]
-            if (self.block_size + T + 14) // 16 * 16 > self.tail_rows and self._hot_of != (layer, T):
-                raise ValueError(f"attend() of {T} rows must follow their append_layer(): layer {layer}'s bf16 rows are not there")
-            return ops.paged8_attention(self.desc(), layer, q, start, max_len, out, count)
+            hot = self._hot_rows_of(layer, T, start, count) if self._long(T) else None
+            if hot is None and self._long(T):
+                raise ValueError(f"attend() of {T} rows must follow their append_layer(): layer {layer}'s bf16 rows from "
+                                 "that start are not there")
+            return ops.paged8_attention(self.desc(hot), layer, q, start, max_len, out, count)
         return ops.paged_attention(self.desc(), layer, q, start, max_len, self.chunk_keys, out, count)
 
     def append_attend(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, start: torch.Tensor,
@@ -309,9 +354,7 @@ class PagedKVCache:
             self._here(k, q)
             if q.shape[1] != k.shape[1]:
                 raise ValueError(f"append_attend(): {q.shape[1]} queries for {k.shape[1]} rows")
-            self._hot_room(layer, k.shape[1])
-            d = self.desc()
-            ops.paged8_append(d, layer, k, v, start, count)
+            d = self._append8(layer, k, v, start, count)
             return ops.paged8_attention(d, layer, q, start, max_len, None, count)
         self.append_layer(layer, k, v, start, count)
         return self.attend(layer, q, start, max_len, count=count)
@@ -396,6 +439,7 @@ class PagedKVCache:
                                  f"bf16 rows of that block are gone (kept from {int(self.tail_from[s, L])} on; a multiple "
                                  f"of block_size {self.block_size}, or a larger tail_rows, can)")
             self.tail_from = np.where(changed, np.minimum(self.tail_from, keep), self.tail_from)
+            self._hot_of.pop(False, None)
         self.n_tokens = np.where(changed, keep, self.n_tokens)
         need = np.where(changed, -(-keep // self.block_size), self.table_len)
         # emptied tail blocks go back per sequence, layer by layer, last first

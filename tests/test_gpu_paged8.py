@@ -513,6 +513,78 @@ def test_long_rows_of_another_append_are_refused(dev):
 
 
 @pytest.mark.gpu
+def test_long_rows_from_another_start_are_refused(dev):
+    """attend() of a long append's rows: the same layer, T, start and count, and nothing on that layer in between."""
+    T, D = 150, 32
+    g = torch.Generator(device=dev)
+    g.manual_seed(3)
+    k, v = rows_of(g, 1, 3 * T, 1, D, dev)
+    q = torch.randn(1, T, 2, D, generator=g, device=dev)
+    part = lambda x, i: x[:, T * i:T * i + T].contiguous()
+    c, ref = (new_cache(1, D, 16, 4 * T) for _ in range(2))
+    for x in (c, ref):
+        x.reserve([3 * T])
+    st = [i32([0]), i32([T])]
+    for i in range(2):
+        c.append_layer(0, part(k, i), part(v, i), st[i])
+        want = ref.append_attend(0, q, part(k, i), part(v, i), st[i], 2 * T)
+    with pytest.raises(ValueError, match="append_layer"):
+        c.attend(0, q, st[0], 2 * T)
+    with pytest.raises(ValueError, match="append_layer"):
+        c.attend(0, q, st[1], 2 * T, count=i32([T - 1]))
+    for start, count in ((st[1], None), (st[1].clone(), None), (st[1], i32([T]))):
+        assert torch.equal(c.attend(0, q, start, 2 * T, count=count), want)
+    with pytest.raises(ValueError, match="must match"):
+        c.append_layer(0, part(k, 1), part(v, 1)[..., :8].contiguous(), st[1])
+    with pytest.raises(ValueError, match="append_layer"):
+        c.attend(0, q, st[1], 2 * T)
+    c.append_layer(0, part(k, 1), part(v, 1), st[1])
+    st[1].add_(1)
+    for start in (st[1], i32([T]), i32([T + 1])):
+        with pytest.raises(ValueError, match="append_layer"):
+            c.attend(0, q, start, 2 * T)
+    with torch.inference_mode():
+        a, b = i32([T]), i32([T])
+        c.append_layer(0, part(k, 1), part(v, 1), a)
+        assert torch.equal(c.attend(0, q, b, 2 * T), want)
+    for change in (lambda: c.append_layer(0, part(k, 2)[:, :1].contiguous(), part(v, 2)[:, :1].contiguous(), i32([T])),
+                   lambda: (c.commit([T + 3]), c.truncate([T]))):
+        s = i32([T])
+        c.append_layer(0, part(k, 1), part(v, 1), s)
+        change()
+        with pytest.raises(ValueError, match="append_layer"):
+            c.attend(0, q, s, 2 * T)
+
+
+@pytest.mark.gpu
+def test_a_replayed_long_append_leaves_the_eager_rows(dev):
+    """A graph's long append to one layer, replayed between an eager one to another layer and its attend()."""
+    T, D = 150, 32
+    g = torch.Generator(device=dev)
+    g.manual_seed(8)
+    k, v = rows_of(g, 1, 2 * T, 1, D, dev)
+    q = torch.randn(1, T, 2, D, generator=g, device=dev)
+    a, b = (tuple(x[:, lo:lo + T].contiguous() for x in (k, v)) for lo in (0, T))
+    c, ref = (new_cache(1, D, 16, 2 * T, layers=2) for _ in range(2))
+    for x in (c, ref):
+        x.reserve([T])
+    st = i32([0])
+    c.append_attend(0, q, *a, st, T)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.append_layer(0, *a, st)
+        out = c.attend(0, q, st, T)
+        with pytest.raises(ValueError, match="append_layer"):
+            c.attend(1, q, st, T)
+    want = [ref.append_attend(0, q, *a, st, T), ref.append_attend(1, q, *b, st, T)]
+    for _ in range(3):
+        c.append_layer(1, *b, st)
+        graph.replay()
+        assert torch.equal(c.attend(1, q, st, T), want[1])
+        assert torch.equal(out, want[0])
+
+
+@pytest.mark.gpu
 def test_a_captured_long_append_keeps_its_rows(dev):
     """A longer append after the capture moves the bf16 rows; the graph still has its own."""
     T, D = 150, 32
