@@ -70,7 +70,12 @@ class Workspace:
     """Grow-only scratch buffer per device and stream (allocates only when a
     call needs more): calls on two streams may run at once. ``shared``: not
     owned by one captured graph; a call that is being captured then takes a
-    buffer from the graph's own memory, which no other graph writes to."""
+    buffer from the graph's own memory, which no other graph writes to, and
+    the buffers of MAX_STREAMS streams are kept at most, the last that were
+    made (memory that goes back to the allocator is reused on its own stream
+    only, behind the calls that used it)."""
+
+    MAX_STREAMS = 8
 
     def __init__(self, shared: bool = False) -> None:
         self._buf: dict = {}
@@ -82,8 +87,11 @@ class Workspace:
         key = (device.type, device.index, _stream())
         b = self._buf.get(key)
         if b is None or b.numel() < nbytes:
+            self._buf.pop(key, None)
             b = torch.empty(max(nbytes, 1 << 16), dtype=torch.uint8, device=device)
             self._buf[key] = b
+            if self._shared and len(self._buf) > self.MAX_STREAMS:
+                del self._buf[next(iter(self._buf))]
         return b
 
 

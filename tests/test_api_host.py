@@ -257,3 +257,20 @@ def test_baseline_and_speculative_caches_share_the_key_chunk(plen, n_new, gamma)
             call()
     base, spec = m.calls
     assert base["chunk_keys"] == spec["chunk_keys"] == auto_chunk_keys(32, 8, plen + n_new)
+
+
+def test_scratch_of_many_streams_is_bounded(monkeypatch):
+    """One buffer per stream, of the last few streams; a captured graph's own buffers all stay."""
+    import torch
+    from draftkv import ops
+    monkeypatch.setattr(ops, "_is_capturing", lambda: False)
+    dev, n = torch.device("cpu"), ops.Workspace.MAX_STREAMS
+    for shared in (True, False):
+        ws, seen = ops.Workspace(shared=shared), {}
+        for i in list(range(100)) + [99, 98]:
+            monkeypatch.setattr(ops, "_stream", lambda: i)
+            b = ws.get(dev, 1 << 16)
+            assert b.numel() >= 1 << 16 and seen.setdefault(i, b) is b and ws.get(dev, 100) is b
+        assert len(ws._buf) == (n if shared else 100)
+        monkeypatch.setattr(ops, "_stream", lambda: 95)
+        assert ws.get(dev, 1 << 17).numel() == 1 << 17 and ws.get(dev, 5) is not seen[95]
