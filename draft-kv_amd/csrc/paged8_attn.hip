@@ -35,6 +35,7 @@ typedef float p8_f32x4 __attribute__((ext_vector_type(4)));
 // bf16 parts of a probability, by those of a query
 __host__ __device__ constexpr int p8_prob_parts(int ns) { return ns == 1 ? 2 : ns; }
 
+constexpr int P8_MAX_LEN = 65534 * 2048;   // (chunks and the rows' own blocks are a grid's z)
 constexpr int P8_UNIT = 256, P8_CHUNK = 2048, P8_UNITS = P8_CHUNK / P8_UNIT;
 
 struct P8Args {
@@ -1076,8 +1077,8 @@ static int p8_launch_ns(P8Args& a, const P8Plan& p, hipStream_t st) {
 
 extern "C" size_t dkv_paged8_attention_workspace(const dkv_paged8_t* cache, int32_t T, int32_t n_q_heads,
                                                  int32_t max_len) {
-    if (!cache || T <= 0 || n_q_heads <= 0 || max_len <= 0 || cache->n_kv_heads <= 0 || cache->head_dim <= 0 ||
-        cache->batch <= 0 || n_q_heads % cache->n_kv_heads)
+    if (!cache || T <= 0 || n_q_heads <= 0 || max_len <= 0 || max_len > dkv::P8_MAX_LEN || cache->n_kv_heads <= 0 ||
+        cache->head_dim <= 0 || cache->head_dim > dkv::P8_MAXD || cache->batch <= 0 || n_q_heads % cache->n_kv_heads)
         return 0;
     // (whichever type the queries have)
     return std::max(dkv::p8_plan(*cache, T, n_q_heads, max_len, 1).bytes, dkv::p8_plan(*cache, T, n_q_heads, max_len, 3).bytes);
@@ -1095,10 +1096,10 @@ extern "C" int dkv_paged8_attention(const dkv_paged8_t* cache, int32_t layer, co
     DKV_REQUIRE(n_q_heads > 0 && n_q_heads % c.n_kv_heads == 0,
                 "dkv_paged8_attention: query heads must be a multiple of KV heads");
     DKV_REQUIRE(max_len > 0, "dkv_paged8_attention: max_len must be > 0");
+    DKV_REQUIRE(max_len <= P8_MAX_LEN, "dkv_paged8_attention: max_len too large");
     if (T <= 0) return DKV_OK;
     if ((rc = p8_check_hot(c, T, "dkv_paged8_attention"))) return rc;
     const P8Plan p = p8_plan(c, T, n_q_heads, max_len, q_dtype == DKV_BF16 ? 1 : 3);
-    DKV_REQUIRE(p.n_chunks < 65535, "dkv_paged8_attention: max_len too large");
     DKV_REQUIRE((int64_t)c.batch * T * n_q_heads < (1LL << 31), "dkv_paged8_attention: too many rows");
     if (p.bytes && (!work || work_bytes < p.bytes || reinterpret_cast<uintptr_t>(work) % 16))
         return fail(DKV_EWORKSPACE, "dkv_paged8_attention: workspace too small or not 16-byte aligned (need " +

@@ -866,6 +866,20 @@ def test_held_rows_are_checked():
     assert L.dkv_paged8_held_bytes(None) == 0 and L.dkv_paged8_held_bytes(C.byref(_desc(head_dim=0))) == 0
 
 
+@pytest.mark.skipif(torch.cuda.is_available(), reason="made-up pointers: host checks only")
+def test_sizes_past_the_plans_are_refused():
+    import ctypes as C
+    from draftkv import _lib
+    L, top = _lib.lib(), 65534 * 2048
+    for max_len in (top + 1, 2 ** 31 - 2048, 2 ** 31 - 1):
+        assert L.dkv_paged8_attention(C.byref(_desc()), 0, 16, 0, 1, 2, 16, None, max_len, 16, 16, 1 << 62, None) == -1
+        assert "max_len" in L.dkv_last_error().decode()
+        assert L.dkv_paged8_attention_workspace(C.byref(_desc()), 1, 2, max_len) == 0
+    assert L.dkv_paged8_attention_workspace(C.byref(_desc()), 1, 2, top) > 0
+    for D in (257, 500, 2 ** 31 - 1):
+        assert L.dkv_paged8_attention_workspace(C.byref(_desc(head_dim=D)), 300, 2, 9000) == 0
+
+
 def test_tensors_on_another_device_are_refused():
     from draftkv.paged import PagedKVCache
     c = PagedKVCache(1, 2, 64, 16, 4, F8, device="cpu")
