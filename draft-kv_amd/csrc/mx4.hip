@@ -974,6 +974,9 @@ extern "C" int dkv_gemm_mx4(const void* x, int32_t x_dtype, const uint8_t* x_sca
     }
     const bool packs = mx_packs(x, x_dtype, M, N, K);
     const int few = mx_few(N, K);
+    // byte offsets into the rows that a workgroup takes are 32 bits: all of few rows, 256 of many
+    DKV_REQUIRE(M <= few ? (int64_t)M * a.tiles * 128 * (packs || x_dtype == DKV_BF16 ? 2 : 4) < (1LL << 32) : a.tiles <= 1 << 16,
+                "dkv_gemm_mx4: K too large");
     if (M <= few && !packs) {
         const bool rag = K % 128;
         if (x_dtype == DKV_F32) return rag ? mx_launch_stream<MX_XF32, 1, 1, true>(a, st) : mx_launch_stream<MX_XF32, 1, 1, false>(a, st);
@@ -982,9 +985,7 @@ extern "C" int dkv_gemm_mx4(const void* x, int32_t x_dtype, const uint8_t* x_sca
     }
     int rc = DKV_OK;
     const int kp = 128 * a.tiles;
-    // 32-bit byte offsets into x: rows in parts
-    const int part = (int)std::min<int64_t>(M, ((1LL << 31) / kp) & ~255LL);
-    DKV_REQUIRE(part > 0, "dkv_gemm_mx4: K too large");
+    const int part = (int)std::min<int64_t>(M, ((1LL << 31) / kp) & ~255LL);   // rows in parts
     if (packs) {
         const size_t need = (size_t)M * kp * 2;
         if (!work || work_bytes < need || !aligned(work, 16))

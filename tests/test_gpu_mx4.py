@@ -350,6 +350,16 @@ def test_bad_calls_are_refused():
     assert L.dkv_mx4_code_bytes(17, 129) == 2 * 2 * 1024 and L.dkv_mx4_scale_bytes(17, 513) == 2 * 2 * 256
 
 
+@pytest.mark.skipif(torch.cuda.is_available(), reason="made-up pointers: host checks only")
+@pytest.mark.parametrize("xd,M,N,K", [(1, 4, 16, 1 << 30), (1, 2, 16, (1 << 30) + 8), (1, 2, 1, 2 ** 31 - 1), (0, 3, 16, 2 ** 31 - 8),
+                                      (0, 16, 65536, 1 << 24), (1, 400, 64, (1 << 23) + 1)])
+def test_widths_past_32_bit_offsets_are_refused(xd, M, N, K):
+    from draftkv import _lib
+    L = _lib.lib()
+    rc = L.dkv_gemm_mx4(16, xd, None, 16, 16, None, 0, M, N, K, 16, 0, 0, 16, 1 << 62, None)
+    assert rc == -1 and "K too large" in L.dkv_last_error().decode()
+
+
 def test_bad_tensors_are_refused():
     from draftkv import ops
     z = torch.zeros(4, 32)
