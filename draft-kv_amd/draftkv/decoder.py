@@ -90,13 +90,15 @@ class Decoder:
     def w_layout(self) -> int:
         return 1 if self.wdtype == torch.bfloat16 else self.layout
 
-    def new_cache(self, batch: int = 1, max_tokens: int = 1 << 20, chunk_keys: Optional[int] = None) -> FullKVCache:
+    def new_cache(self, batch: int = 1, max_tokens: int = 1 << 20, chunk_keys: Optional[int] = None,
+                  tail_rows: Optional[int] = None) -> FullKVCache:
         """The full cache for ``batch`` sequences of up to ``max_tokens`` rows;
         ``chunk_keys`` fixes the attention kernel's key chunk (by default
         chosen from the shape, ``paged.auto_chunk_keys``). Its type is
-        ``kv_dtype``: the model's, or torch.float8_e4m3fn when set so."""
+        ``kv_dtype``: the model's, or torch.float8_e4m3fn when set so;
+        ``tail_rows`` is then the cache's."""
         return FullKVCache(self.n_layers, self.n_kv_heads, self.d_head, dtype=self.kv_dtype, batch=batch,
-                           max_tokens=max_tokens, device=self.device, chunk_keys=chunk_keys)
+                           max_tokens=max_tokens, device=self.device, chunk_keys=chunk_keys, tail_rows=tail_rows)
 
     # ------------------------------------------------------------ RoPE table
     def _cos_sin(self, need: int):

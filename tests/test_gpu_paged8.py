@@ -711,6 +711,29 @@ def test_engine_over_it_is_lossless(dev, family, dtype, temperature):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tail,most", [(32, 1), (48, 17)])
+def test_the_engine_drafts_no_more_than_the_tail_takes_back(dev, tail, most):
+    from draftkv import CompressionConfig, DraftKVEngine, FixedPolicy
+    from draftkv.engine import DecodeBatch
+    from draftkv.llama import demo_llama
+    model = demo_llama(dtype=F32, device=dev)
+    model.kv_dtype = F8
+    prompts = [np.random.default_rng(s).integers(0, 128, size=n).tolist() for s, n in ((0, 30), (1, 49))]
+    want = DraftKVEngine(model).generate_baseline_batch([list(p) for p in prompts], 60)
+    eng = DraftKVEngine(model, FixedPolicy(CompressionConfig(2, 0.3), 20))
+    full = model.new_cache(2, 200, tail_rows=tail)
+    assert full.tail_rows == tail and full.max_rollback == most
+    eng._prefill(prompts, full)
+    batch = DecodeBatch(eng, prompts, full, 60, 0.0)
+    while batch.step():
+        pass
+    res = batch.results()
+    assert [r.tokens for r in res] == want
+    gammas = [r.gamma for r in res[0].rounds]
+    assert max(gammas) == most
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("bs,tail,D,H", [(16, 32, 64, 2), (16, 128, 24, 1), (64, 96, 128, 1), (128, 144, 256, 1), (32, 64, 192, 1)])
 def test_appends_made_again(dev, bs, tail, D, H):
     """An append that is not committed may be made again from the same start, or another one in its place, however long:
