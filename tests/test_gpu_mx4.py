@@ -292,6 +292,90 @@ def test_model_with_4_bit_weights(dev, family, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("family,dtype", [("llama", F32), ("llama", BF16), ("bias", F32), ("bias", BF16), ("gpt2", F32), ("gpt2", BF16), ("tiny", F32)])
+def test_model_with_4_bit_weights_step_by_step(dev, family, dtype, monkeypatch):
+    """The same model with the 4-bit weights' values, every projection's input rounded to bf16: the products' operands
+    are then equal, and the logits differ by the order of float32 sums alone."""
+    from draftkv import ops
+    from draftkv.gpt2 import GPT2
+    from draftkv.llama import demo_llama
+    from draftkv.model import demo_model
+
+    def make():
+        if family == "tiny":
+            return demo_model(dtype=dtype, device=dev)
+        if family == "gpt2":
+            return GPT2.random(dict(n_layer=2, n_head=4, n_embd=64, n_positions=256, vocab_size=128), seed=1, std=0.1, dtype=dtype, device=dev)
+        return demo_llama(attn_bias=family == "bias", dtype=dtype, device=dev)
+
+    model, plain = make(), make()
+    for m in (model, plain):                                   # (biases that a logit shows)
+        for i, p in enumerate(m.layers):
+            for name in ("bqkv", "bo", "b1", "b2"):
+                if getattr(p, name) is not None:
+                    getattr(p, name).normal_(0.0, 0.5, generator=torch.Generator(device=dev).manual_seed(i))
+    model.quantize_weights()
+    for p, q in zip(plain.layers, model.layers):
+        for name in ("wqkv", "wo", "w1", "w2"):
+            v = getattr(q, name).values().to(dtype)            # (exact)
+            if name == "w1" and plain.mlp == "swiglu" and not getattr(plain, "gate_up_interleaved", False):
+                v = torch.cat([v[0::2], v[1::2]])
+            setattr(p, name, v if plain.w_layout == 1 else v.t().contiguous())
+    if dtype == F32:
+        f, g = ops.gemm_f32, ops.gemm_f32_act
+        monkeypatch.setattr(ops, "gemm_f32", lambda x, w, *a, **k: f(x if w is plain.head else x.to(BF16).float(), w, *a, **k))
+        monkeypatch.setattr(ops, "gemm_f32_act", lambda x, *a, **k: g(x.to(BF16).float(), *a, **k))
+    elif plain.mlp == "swiglu":       # of the float32 gate and up, as the 4-bit product's is (the bf16 one rounds them first)
+        def mlp(x, p):
+            y = ops.gemm_bf16(x, p.w1, out_dtype=F32)
+            gate, up = (y[:, 0::2], y[:, 1::2]) if getattr(plain, "gate_up_interleaved", False) else y.chunk(2, 1)
+            return (torch.nn.functional.silu(gate) * up).to(BF16)
+        monkeypatch.setattr(plain, "_mlp_inner", mlp)
+    toks = np.random.default_rng(2).integers(0, 128, size=50)
+    want = plain.forward(toks, plain.new_cache(), 0)
+    monkeypatch.undo()
+    got = model.forward(toks, model.new_cache(), 0)
+    # Sums in another order differ by about 2^-22 of a value, which now and then (2^-22 / 2^-8) puts an activation on the
+    # other side of a bf16 step: one of 64 or more inputs of a product by 2^-8 of it, about 2^-11 of the output. A few
+    # such per token: 2^-8 of the largest logit. bf16 models round every output as well, a few more: 2^-7.
+    assert np.abs(got - want).max() <= (2.0 ** -8 if dtype == F32 else 2.0 ** -7) * np.abs(want).max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("xk", ["f32", "bf16", "mx4"])
+@pytest.mark.parametrize("M,N,K", [(1, 131072, 128), (2, 140001, 40), (70, 131090, 96)])
+def test_few_rows_of_very_wide_weights(dev, M, N, K, xk):
+    from draftkv import ops
+    g = torch.Generator(device=dev)
+    g.manual_seed(N)
+    x = torch.randn(M, K, generator=g, device=dev).to(BF16 if xk == "bf16" else F32)
+    w = ops.mx4_quantize(0.05 * torch.randn(N, K, generator=g, device=dev))
+    xin = ops.mx4_quantize(x) if xk == "mx4" else x
+    x64, w64 = xin.values().double() if xk == "mx4" else x.to(BF16).double(), w.values().double()
+    want = x64 @ w64.t()
+    assert ((ops.gemm_mx4(xin, w, out_dtype=F32).double() - want).abs() <= tol(x64, w64, F32, want)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("xk", ["f32", "bf16", "mx4"])
+@pytest.mark.parametrize("M", [1, 40, 300])
+@pytest.mark.parametrize("ew,ex", [(-128, 100), (-126, 120), (110, -120), (-124, 90)])
+def test_products_of_tiny_and_large_values(dev, M, ew, ex, xk):
+    """Weights whose values are no normal bf16 numbers, or near the largest, and rows that bring the products back."""
+    from draftkv import ops
+    g = torch.Generator(device=dev)
+    g.manual_seed(ew + 200)
+    N, K = 96, 256
+    x = (torch.randn(M, K, generator=g, device=dev) * 2.0 ** ex).to(BF16 if xk == "bf16" else F32)
+    w = ops.mx4_quantize(torch.randn(N, K, generator=g, device=dev) * 2.0 ** (ew / 2) * 2.0 ** (ew / 2))
+    xin = ops.mx4_quantize(x) if xk == "mx4" else x
+    x64, w64 = xin.values().double() if xk == "mx4" else x.to(BF16).double(), w.values().double()
+    assert w64.any() and torch.isfinite(w64).all()
+    want = x64 @ w64.t()
+    assert ((ops.gemm_mx4(xin, w, out_dtype=F32).double() - want).abs() <= tol(x64, w64, F32, want)).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("gamma", [0, 4])
 def test_weights_quantized_while_decoding(dev, gamma):
     """Recorded steps hold the weights that they were recorded with: after quantize_weights() they are recorded anew."""
