@@ -230,9 +230,11 @@ class PagedKVCache:
         for (was, version), t in zip(of[2:], (start, count)):
             if was is None and t is None:
                 continue
-            if _version(was) != version or capturing and t is not was:
+            view = was is not None and t is not None and (t.data_ptr(), t.shape, t.stride(), t.dtype) == \
+                (was.data_ptr(), was.shape, was.stride(), was.dtype)
+            if _version(was) != version or capturing and not view:
                 return None
-            if t is not was:      # another tensor with the same values (the host waits for them)
+            if not view:          # another tensor with the same values (the host waits for them)
                 a, b = (x if x is not None else torch.full_like(y, T) for x, y in ((was, t), (t, was)))
                 if (a.shape, a.dtype, a.device) != (b.shape, b.dtype, b.device) or not torch.equal(a, b):
                     return None

@@ -573,7 +573,7 @@ def test_a_replayed_long_append_leaves_the_eager_rows(dev):
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         c.append_layer(0, *a, st)
-        out = c.attend(0, q, st, T)
+        out = c.attend(0, q, st[:], T)      # (a view of it)
         with pytest.raises(ValueError, match="append_layer"):
             c.attend(1, q, st, T)
     want = [ref.append_attend(0, q, *a, st, T), ref.append_attend(1, q, *b, st, T)]
