@@ -1,0 +1,64 @@
+// Copying whole pages of a paged store: what copy-on-write and compaction of
+// shared pages do (no counterpart in the reference, whose sequences share
+// nothing, draftkv/paged.py:76-176).
+//
+// dst page <- src page, byte for byte. Bound: memory, each byte read and
+// written once.
+#include "dkv_common.h"
+
+namespace dkv {
+
+constexpr int COPY_THREADS = 256;
+
+// Grid x: pair * pieces + piece. V is the widest type that the pages' size and
+// address allow. A pair with an id outside the store is skipped.
+template <class V, int PER>
+__global__ void __launch_bounds__(COPY_THREADS) paged_copy_kernel(char* __restrict__ store, int64_t n_pages, int64_t page_bytes,
+                                                                  const int32_t* __restrict__ src,
+                                                                  const int32_t* __restrict__ dst, int64_t first, int pieces) {
+    const int64_t pair = first + blockIdx.x / pieces;
+    const int64_t a = src[pair], b = dst[pair];
+    if (a < 0 || a >= n_pages || b < 0 || b >= n_pages || a == b) return;
+    const V* from = reinterpret_cast<const V*>(store + a * page_bytes);
+    V* to = reinterpret_cast<V*>(store + b * page_bytes);
+    const int64_t n = page_bytes / sizeof(V);
+    const int64_t i0 = (int64_t)(blockIdx.x % pieces) * (COPY_THREADS * PER) + threadIdx.x;
+    V v[PER];
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+        if (i0 + k * COPY_THREADS < n) v[k] = from[i0 + k * COPY_THREADS];
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+        if (i0 + k * COPY_THREADS < n) to[i0 + k * COPY_THREADS] = v[k];
+}
+
+template <class V, int PER>
+static int copy_pages(char* store, int64_t n_pages, int64_t page_bytes, const int32_t* src, const int32_t* dst,
+                      int64_t n_pairs, hipStream_t st) {
+    const int64_t span = (int64_t)COPY_THREADS * PER * sizeof(V);
+    const int64_t pieces = (page_bytes + span - 1) / span;
+    DKV_REQUIRE(pieces < (1 << 24), "dkv_paged_copy: pages too large");
+    const int64_t most = ((1 << 30) / pieces);   // pairs per launch
+    for (int64_t i = 0; i < n_pairs; i += most) {
+        const int64_t n = n_pairs - i < most ? n_pairs - i : most;
+        hipLaunchKernelGGL((paged_copy_kernel<V, PER>), dim3((unsigned)(n * pieces)), dim3(COPY_THREADS), 0, st, store, n_pages,
+                           page_bytes, src, dst, i, (int)pieces);
+    }
+    return check_launch("dkv_paged_copy");
+}
+
+}  // namespace dkv
+
+extern "C" int dkv_paged_copy(void* store, int64_t n_pages, int64_t page_bytes, const int32_t* src, const int32_t* dst,
+                              int64_t n_pairs, dkv_stream_t stream) {
+    DKV_REQUIRE(n_pages >= 0 && page_bytes >= 0 && n_pairs >= 0, "dkv_paged_copy: negative size");
+    if (n_pairs == 0 || n_pages == 0 || page_bytes == 0) return DKV_OK;
+    DKV_REQUIRE(store && src && dst, "dkv_paged_copy: NULL argument");
+    hipStream_t st = dkv::as_stream(stream);
+    char* p = static_cast<char*>(store);
+    const int64_t at = reinterpret_cast<intptr_t>(store) | page_bytes;
+    if (at % 16 == 0) return dkv::copy_pages<uint4, 4>(p, n_pages, page_bytes, src, dst, n_pairs, st);
+    if (at % 4 == 0) return dkv::copy_pages<uint32_t, 8>(p, n_pages, page_bytes, src, dst, n_pairs, st);
+    if (at % 2 == 0) return dkv::copy_pages<uint16_t, 8>(p, n_pages, page_bytes, src, dst, n_pairs, st);
+    return dkv::copy_pages<uint8_t, 8>(p, n_pages, page_bytes, src, dst, n_pairs, st);
+}

@@ -33,6 +33,11 @@ class Paged8(C.Structure):
                 ("tail_rows", C.c_int32), ("hot_rows", C.c_int32), ("held", C.c_void_p)]
 
 
+class Groups(C.Structure):
+    _fields_ = [("first", C.c_void_p), ("shared", C.c_void_p), ("n_groups", C.c_int32), ("max_members", C.c_int32),
+                ("min_shared", C.c_int32), ("max_shared", C.c_int32)]
+
+
 class Drafter(C.Structure):
     _fields_ = [("pages", C.c_void_p), ("pos", C.c_void_p), ("score", C.c_void_p), ("n_rows", C.c_void_p),
                 ("batch", C.c_int32), ("n_layers", C.c_int32), ("n_kv_heads", C.c_int32),
@@ -46,6 +51,7 @@ class QCfg(C.Structure):
 
 P, I32, I64, F32, SZ = C.c_void_p, C.c_int32, C.c_int64, C.c_float, C.c_size_t
 PPaged, PPaged8, PDrafter, PQCfg = C.POINTER(Paged), C.POINTER(Paged8), C.POINTER(Drafter), C.POINTER(QCfg)
+PGroups = C.POINTER(Groups)
 
 _SIGS = {
     "dkv_quantize": (C.c_int, [P, I64, I32, I32, I32, I32, P, P, P, P, P]),
@@ -60,6 +66,9 @@ _SIGS = {
     "dkv_paged8_attention_workspace": (SZ, [PPaged8, I32, I32, I32]),
     "dkv_paged8_attention": (C.c_int, [PPaged8, I32, P, I32, I32, I32, P, P, I32, P, P, SZ, P]),
     "dkv_paged8_read": (C.c_int, [PPaged8, I32, P, P, I32, P, P, P]),
+    "dkv_paged_copy": (C.c_int, [P, I64, I64, P, P, I64, P]),
+    "dkv_shared_attention_workspace": (SZ, [PPaged, I32, I32, I32, I32]),
+    "dkv_shared_attention": (C.c_int, [PPaged, PGroups, I32, P, I32, I32, I32, P, P, I32, I32, P, P, SZ, P]),
     "dkv_page_bytes": (I64, [I32, I32, I32, I32]),
     "dkv_drafter_append": (C.c_int, [PDrafter, I32, QCfg, P, P, I32, I32, P, P, P, P]),
     "dkv_drafter_truncate": (C.c_int, [PDrafter, PQCfg, P, P]),
@@ -78,6 +87,8 @@ _SIGS = {
     "dkv_accept_workspace": (SZ, [I32, I32, I32]),
     "dkv_accept": (C.c_int, [P, P, P, I32, I32, I32, F32, P, P, P, P, P, P, SZ, P]),
     "dkv_accept_noalloc": (C.c_int, [P, P, P, I32, I32, I32, F32, P, P, P, P, P, P]),
+    "dkv_beam_select_workspace": (SZ, [I32, I32, I32, I32]),
+    "dkv_beam_select": (C.c_int, [P, I32, I64, I32, I32, I32, P, I32, P, P, P, P, SZ, P]),
     "dkv_embed": (C.c_int, [P, I32, P, I32, I32, P, P, P, P]),
     "dkv_rmsnorm": (C.c_int, [P, P, I32, I32, I32, F32, P, I32, P]),
     "dkv_layernorm": (C.c_int, [P, P, P, I32, I32, I32, F32, P, I32, P]),

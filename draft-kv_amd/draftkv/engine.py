@@ -33,6 +33,7 @@ import torch
 from . import ops
 from .compress import CompressedKVCache
 from .paged import PagedKVCache, auto_chunk_keys
+from .shared import SharedKVCache, auto_unit_keys
 from .graphs import DraftStepGraph, FullStepGraph, full_graph_key, graph_key
 from .config import CompressionConfig
 from .controller import Controller, FixedPolicy
@@ -72,6 +73,15 @@ class GenerationResult:                                             # engine.py:
     @property
     def tokens_per_verify(self) -> float:
         return self.new_tokens / self.verify_passes if self.verify_passes else float("nan")
+
+
+@dataclass
+class BeamHypothesis:
+    """One continuation of ``generate_beams``: the prompt and the new tokens (its last the end token, where it has one),
+    the sum of the new tokens' log probabilities, and that sum over (number of new tokens) ** length_penalty."""
+    tokens: list
+    logprob: float
+    score: float
 
 
 class DraftKVEngine:
@@ -190,6 +200,110 @@ class DraftKVEngine:
         while batch.step():
             pass
         return batch.results()
+
+    # ------------------------------------------------- many continuations of one prompt
+    def _new_shared(self, toks: list, n: int, own_rows: int, max_tokens: int, span: int) -> SharedKVCache:
+        """The full cache of the prompts, with pages for n continuations of each that write up to own_rows rows of their
+        own. ``span`` fixes the attention's unit, as ``_new_full`` does the chunk."""
+        m = self.model
+        bs = 16
+        if m.kv_dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError(f"continuations of one prompt share a float32 or bfloat16 cache, not {m.kv_dtype}")
+        # the prompt's whole pages once; of each continuation its own rows, from within an open page on
+        pages = sum(-(-len(t) // bs) for t in toks) + len(toks) * n * (-(-own_rows // bs) + 2)
+        return SharedKVCache(m.n_layers, m.n_kv_heads, m.d_head, bs, pages, m.kv_dtype, batch=len(toks),
+                             max_tokens=max_tokens, device=m.device,
+                             chunk_keys=auto_unit_keys(len(toks), m.n_kv_heads, span))
+
+    def generate_samples(self, prompts: Sequence, n: int, max_new_tokens: int, temperature: float = 1.0,
+                         context_key: Optional[str] = None) -> list:
+        """n continuations of every prompt, decoded by the same rounds as ``generate_batch`` in one batch: a list of n
+        GenerationResults per prompt. A prompt is computed and held once, its continuations share its pages, and
+        attention reads them once for all of them. Continuation i of prompt p draws from the random stream p * n + i."""
+        if n < 1:
+            raise ValueError(f"n must be at least 1, got {n}")
+        prompts = self._check_prompts(prompts, self.model.vocab_size)
+        if not prompts:
+            return []
+        plen = np.array([len(t) for t in prompts], np.int64)
+        need = rows_needed(plen, max_new_tokens, self.controller)
+        full = self._new_shared(prompts, n, need - int(plen.max()) + 1, need, int(plen.max()) + max_new_tokens)
+        self._prefill(prompts, full)
+        full.fork([p for p in range(len(prompts)) for _ in range(n)])
+        toks = [list(p) for p in prompts for _ in range(n)]
+        batch = DecodeBatch(self, toks, full, max_new_tokens, temperature, context_key)
+        while batch.step():
+            pass
+        res = batch.results()
+        return [res[p * n: (p + 1) * n] for p in range(len(prompts))]
+
+    def generate_beams(self, prompts: Sequence, n_beams: int, max_new_tokens: int, eos: Optional[int] = None,
+                       length_penalty: float = 1.0) -> list:
+        """Beam search over the full cache: per prompt, up to n_beams ``BeamHypothesis``, best score first. A beam ends with
+        the token ``eos`` (None: none does); a prompt is done when n_beams have ended and no living beam's score, at its
+        present length, is above the worst of them."""
+        if not 1 <= n_beams <= 64:
+            raise ValueError(f"n_beams must be 1..64, got {n_beams}")
+        model, B = self.model, int(n_beams)
+        prompts = self._check_prompts(prompts, model.vocab_size)
+        P = len(prompts)
+        if P == 0 or max_new_tokens <= 0:
+            return [[BeamHypothesis(p, 0.0, 0.0)] for p in prompts]
+        plen = np.array([len(t) for t in prompts], np.int64)
+        most = int(plen.max()) + max_new_tokens
+        full = self._new_shared(prompts, B, max_new_tokens + 1, most, most)
+        self.last_full = full
+        self._prefill(prompts, full)
+        full.fork([p for p in range(P) for _ in range(B)])
+        dev = model.device
+        k = 2 * B if eos is not None else B       # of 2 B continuations at most B end
+        start = np.repeat(plen - 1, B)
+        new = [[] for _ in range(P * B)]          # the beams' new tokens
+        cum = np.full((P, B), -np.inf)
+        cum[:, 0] = 0.0                           # at first the beams are one
+        last = np.array([p[-1] for p in prompts for _ in range(B)], np.int32)
+        ended: list = [[] for _ in range(P)]
+        open_ = np.ones(P, bool)
+
+        def hypothesis(p, tokens, logprob):
+            return BeamHypothesis(prompts[p] + tokens, float(logprob), float(logprob) / len(tokens) ** length_penalty)
+
+        for i in range(max_new_tokens):
+            act = np.repeat(open_, B).astype(np.int64)
+            x = ops.to_device(last, dev)
+            logits = model.forward_batch(x[:, None], full, start + i, act)[:, 0]
+            best, beam, tok = (t.cpu().numpy() for t in ops.beam_select(logits.view(P, B, -1), ops.to_device(cum, dev), k))
+            parents = np.arange(P * B)
+            fresh = [list(t) for t in new]
+            for p in np.flatnonzero(open_):
+                j, cum[p] = 0, -np.inf
+                for c in range(k):
+                    if j == B or tok[p, c] < 0:
+                        break
+                    s = p * B + int(beam[p, c])
+                    if eos is not None and int(tok[p, c]) == eos:
+                        if c < B:                 # (an end below the best B is no beam's)
+                            ended[p].append(hypothesis(p, new[s] + [eos], best[p, c]))
+                        continue
+                    d = p * B + j
+                    parents[d], cum[p, j], last[d] = s, best[p, c], tok[p, c]
+                    fresh[d] = new[s] + [int(tok[p, c])]
+                    j += 1
+                ended[p] = sorted(ended[p], key=lambda h: -h.score)[:B]
+                alive = float(cum[p, 0]) / (i + 1) ** length_penalty
+                if j == 0 or len(ended[p]) == B and alive <= ended[p][-1].score:
+                    open_[p] = False
+            new = fresh
+            if not open_.any() or i + 1 == max_new_tokens:
+                break
+            full.fork(parents)
+        out = []
+        for p in range(P):
+            hyps = ended[p]
+            if open_[p]:
+                hyps = hyps + [hypothesis(p, new[p * B + j], cum[p, j]) for j in range(B) if cum[p, j] > -np.inf]
+            out.append(sorted(hyps, key=lambda h: -h.score)[:B])
+        return out
 
 
 def gamma_bound(controller, max_new_tokens: int) -> int:

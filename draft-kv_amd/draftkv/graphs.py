@@ -132,7 +132,8 @@ class DraftStepGraph:
 def full_graph_key(model, full, b: int, temperature: float, max_len: int) -> tuple:
     cs = getattr(model, "_cs", None)
     return (getattr(model, "weights_version", 0), b, float(temperature), full.store.data_ptr(), full.d_tables.data_ptr(), int(max_len),
-            full.chunk_keys, full.tail.data_ptr() if full.fp8 else None, None if cs is None else (cs.data_ptr(), model._cs_len))
+            full.chunk_keys, full.tail.data_ptr() if full.fp8 else None, full.graph_key(),
+            None if cs is None else (cs.data_ptr(), model._cs_len))
 
 
 class FullStepGraph:

@@ -12,8 +12,8 @@ from typing import Optional, Sequence
 import torch
 
 from . import _lib
-from ._lib import (DKV_BF16, DKV_F32, DKV_GEMM_DEFER, DKV_GEMM_SWIGLU, DKV_GEMM_WTILED, DKV_MX4, Drafter, Paged, Paged8,
-                   QCfg, check, lib)
+from ._lib import (DKV_BF16, DKV_F32, DKV_GEMM_DEFER, DKV_GEMM_SWIGLU, DKV_GEMM_WTILED, DKV_MX4, Drafter, Groups, Paged,
+                   Paged8, QCfg, check, lib)
 
 
 _get_device = getattr(torch._C, "_cuda_getDevice", None)
@@ -292,6 +292,112 @@ def paged8_read(desc: Paged8, layer: int, first: torch.Tensor, length: torch.Ten
     return k, v
 
 
+# ------------------------------------------------------------------ pages that sequences share
+def paged_copy(store: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> torch.Tensor:
+    """Copy page src[i] of ``store`` [pages, ...] over page dst[i], in place; src and dst int32 on the device. A page may
+    be the source of several copies; no page may be the destination of two, or source and destination both (not
+    checked: the ids are on the device). Ids outside the store are skipped. Returns ``store``."""
+    _need(store, "store")
+    if store.dim() < 1:
+        raise ValueError("store must hold pages along its first axis")
+    for t, n in ((src, "src"), (dst, "dst")):
+        _need(t, n, torch.int32, 1)
+        if t.device != store.device:
+            raise ValueError(f"{n} must be on {store.device}")
+    if src.numel() != dst.numel():
+        raise ValueError(f"paged_copy: {src.numel()} sources for {dst.numel()} destinations")
+    pages = store.shape[0]
+    nbytes = store.numel() // pages * store.element_size() if pages else 0
+    with _device(store.device):
+        check(lib().dkv_paged_copy(store.data_ptr(), pages, nbytes, src.data_ptr(), dst.data_ptr(), src.numel(),
+                                   _stream()), "dkv_paged_copy")
+    return store
+
+
+class PrefixGroups:
+    """Groups of consecutive sequences with a common prefix, for ``shared_attention``: group g is sequences first[g] ..
+    first[g + 1] - 1, whose first shared[s] rows are the same pages (equal within a group; 0 for sequences of none).
+    Made from host lists; the device copies live as long as this. ``update`` writes other groups into the same device
+    memory (a recorded graph reads what is there when it is replayed; the bounds that sized its launch must hold)."""
+
+    def __init__(self, first: Sequence[int], shared: Sequence[int], device) -> None:
+        self.batch = len(shared)
+        self.mem = torch.zeros(2 * self.batch + 1, dtype=torch.int32, device=device)
+        self.device = self.mem.device
+        self._host: tuple = ()
+        self.update(first, shared)
+
+    def update(self, first: Sequence[int], shared: Sequence[int]) -> bool:
+        """Returns whether anything changed."""
+        first, shared = [int(x) for x in first], [int(x) for x in shared]
+        b = self.batch
+        if len(shared) != b:
+            raise ValueError(f"shared must hold one value per sequence ({b}), got {len(shared)}")
+        if len(first) == 1 or len(first) > b + 1 or any(y <= x for x, y in zip(first, first[1:])) or \
+                first and (first[0] < 0 or first[-1] > b):
+            raise ValueError(f"first must rise within 0..{b}, got {first}")
+        inside = [False] * b
+        for x, y in zip(first, first[1:]):
+            for s in range(x, y):
+                inside[s] = True
+                if shared[s] != shared[x]:
+                    raise ValueError(f"sequences {x} and {s} of one group share {shared[x]} and {shared[s]} rows")
+        if any(n < 0 or n >= 1 << 31 or n and not i for n, i in zip(shared, inside)):
+            raise ValueError("shared must not be negative, and 0 outside groups")
+        if (first, shared) == self._host:
+            return False
+        self._host = (first, shared)
+        self.n_groups = max(len(first) - 1, 0)
+        self.max_members = max((y - x for x, y in zip(first, first[1:])), default=0)
+        self.min_shared, self.max_shared = min(shared, default=0), max(shared, default=0)
+        import numpy as np
+        row = np.zeros(2 * b + 1, np.int32)
+        row[:b] = shared
+        row[b:b + len(first)] = first
+        if b:
+            with _device(self.device):
+                self.mem.copy_(to_device(row, self.device))
+        return True
+
+    def bounds(self) -> tuple:
+        """What sizes a launch."""
+        return (self.n_groups, self.max_members, self.min_shared, self.max_shared)
+
+    def desc(self) -> Groups:
+        return Groups(self.mem.data_ptr() + 4 * self.batch, self.mem.data_ptr(), *self.bounds())
+
+
+def shared_attention(desc: Paged, layer: int, q: torch.Tensor, start: torch.Tensor, max_len: int, unit_keys: int,
+                     groups: Optional[PrefixGroups] = None, out: Optional[torch.Tensor] = None,
+                     count: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention of q [batch, T, Hq, D] (float32 or bfloat16; the result has its type) over a paged cache whose
+    sequences share prefixes: what ``groups`` have in common is read once for all their rows. start, max_len and count
+    as for ``paged_attention``. Keys are summed in units of ``unit_keys`` (a multiple of 32) at absolute positions: a
+    row's bits depend on its keys and on that alone, neither on the groups nor on T."""
+    _need(q, "q", ndim=4)
+    b, T, Hq, D = q.shape
+    if b != desc.batch or D != desc.head_dim:
+        raise ValueError(f"q shape {tuple(q.shape)} does not match the cache")
+    _need_rows(start, "start", b, q.device)
+    _need_rows(count, "count", b, q.device)
+    if groups is not None and (groups.batch != b or groups.device != q.device):
+        raise ValueError(f"groups of {groups.batch} sequences on {groups.device} for {b} on {q.device}")
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        _need(out, "out", q.dtype, 4)
+        if out.shape != q.shape or out.device != q.device:
+            raise ValueError(f"out must have q's shape {tuple(q.shape)} and device")
+    g = Groups() if groups is None else groups.desc()
+    with _device(q.device):
+        nbytes = lib().dkv_shared_attention_workspace(C.byref(desc), T, Hq, max_len, unit_keys)
+        ws = _WS.get(q.device, nbytes) if nbytes else None
+        check(lib().dkv_shared_attention(C.byref(desc), C.byref(g), layer, q.data_ptr(), _dt(q), T, Hq, start.data_ptr(),
+                                         _ptr(count), max_len, unit_keys, out.data_ptr(), _ptr(ws),
+                                         0 if ws is None else ws.numel(), _stream()), "dkv_shared_attention")
+    return out
+
+
 # ------------------------------------------------------------------ mirror
 def _qarr(cfgs: Sequence[QCfg]):
     arr = (QCfg * len(cfgs))(*cfgs)
@@ -446,6 +552,32 @@ def accept(target: torch.Tensor, draft: Optional[torch.Tensor], draft_tokens: to
                            float(temperature), u.data_ptr(), _ptr(draft_stats), res[0].data_ptr(), res[1].data_ptr(),
                            res[2].data_ptr(), ws.data_ptr(), ws.numel(), _stream()), "dkv_accept")
     return res[0], res[1], res[2]
+
+
+# ------------------------------------------------------------------ beam search
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int):
+    """The k best continuations of each prompt's beams: of logits [prompts, beams, vocab] (float32 or bfloat16) and the
+    beams' scores float64 [prompts, beams], score = scores[p, b] + log_softmax(logits[p, b])[v] in float64, ordered by
+    score, then beam, then logit, then token. Returns (scores float64, beams int32, tokens int32), each [prompts, k], best
+    first; -inf, -1, -1 where there are fewer (tokens at -inf, rows with a NaN or +inf, beams at -inf or NaN have none)."""
+    _need(logits, "logits", ndim=3)
+    _need(scores, "scores", torch.float64, 2)
+    p, b, V = logits.shape
+    if scores.shape != (p, b) or scores.device != logits.device:
+        raise ValueError(f"scores must be [{p}, {b}] on {logits.device}, got {tuple(scores.shape)} on {scores.device}")
+    k = int(k)
+    dt = _dt(logits)
+    if b < 1 or V < 1 or not 1 <= k <= 128 or b * k > 4096:
+        raise ValueError(f"beam_select: bad sizes (logits {tuple(logits.shape)}, k {k}: k is 1..128, beams * k at most 4096)")
+    dev = logits.device
+    out = torch.empty((p, k), dtype=torch.float64, device=dev)
+    parents, tokens = (torch.empty((p, k), dtype=torch.int32, device=dev) for _ in range(2))
+    with _device(dev):
+        ws = _WS.get(dev, lib().dkv_beam_select_workspace(p, b, V, k))
+        check(lib().dkv_beam_select(logits.data_ptr(), dt, V, p, b, V, scores.data_ptr(), k, out.data_ptr(),
+                                    parents.data_ptr(), tokens.data_ptr(), ws.data_ptr(), ws.numel(), _stream()),
+              "dkv_beam_select")
+    return out, parents, tokens
 
 
 # ------------------------------------------------------------------ model forward ops

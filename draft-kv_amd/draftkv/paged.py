@@ -262,6 +262,10 @@ class PagedKVCache:
                      self.d_head, self.block_size, self.max_blocks,
                      DKV_BF16 if self.dtype == torch.bfloat16 else DKV_F32)
 
+    def graph_key(self) -> tuple:
+        """What a recorded forward over this cache depends on beside its buffers' addresses."""
+        return ()
+
     # ------------------------------------------------------------ allocation
     def _ensure_capacity(self, s: int, layer: int, extra: int) -> None:   # paged.py:112-117
         need = self.n_tokens[s, layer] + extra

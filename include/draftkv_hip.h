@@ -198,6 +198,52 @@ int dkv_paged8_attention(const dkv_paged8_t* cache, int32_t layer, const void* q
 int dkv_paged8_read(const dkv_paged8_t* cache, int32_t layer, const int32_t* first, const int32_t* length, int32_t T,
                     float* k, float* v, dkv_stream_t stream);
 
+/* ---------------------------------------------------------------- pages that sequences share */
+/* Sequences of one pool may have pages in common: their block tables then hold
+ * the same ids (no counterpart in the reference, whose sequences share
+ * nothing, paged.py:76-176). The calls above take such tables as they are. */
+
+/* Copies page src[i] of a store over page dst[i], i < n_pairs, byte for byte.
+ * Pages are page_bytes long and n_pages in number; a pair with an id outside
+ * 0 .. n_pages - 1 is skipped. A page may be the source of several pairs; no
+ * page is the destination of two, or source and destination both (what it then
+ * holds is undefined; the caller's to ensure). */
+int dkv_paged_copy(void* store, int64_t n_pages, int64_t page_bytes, const int32_t* src, const int32_t* dst,
+                   int64_t n_pairs, dkv_stream_t stream);
+
+/* Groups of consecutive sequences with a common prefix: group g is sequences
+ * first[g] .. first[g + 1] - 1 (first: int32 [n_groups + 1], rising, within
+ * 0..batch; sequences before first[0] or from first[n_groups] on are in none),
+ * and the first shared[s] keys (int32 [batch]; equal within a group, 0 outside
+ * groups) of its sequences are the same: those of the table of sequence
+ * first[g]. Both arrays are on the device. max_members, min_shared and
+ * max_shared bound group sizes and shared (0 outside groups counts too); they
+ * size the launch. n_groups 0: none (the arrays may be NULL). */
+typedef struct {
+    const int32_t* first;
+    const int32_t* shared;
+    int32_t n_groups, max_members, min_shared, max_shared;
+} dkv_groups_t;
+
+/* dkv_paged_attention of a batch whose sequences share prefixes: the same
+ * definition, arguments as there, with the keys that a group shares read once
+ * for all of its rows. q and out: DKV_F32 or DKV_BF16 (q_dtype both),
+ * [batch][T][Hq][D]. Against a bf16 cache float32 queries and probabilities
+ * enter the products in three bf16 parts, bf16 queries whole and their
+ * probabilities in two; against a float32 cache the products are float32. Keys
+ * are cut at absolute positions into units of unit_keys (a multiple of 32): a
+ * row's result depends on its keys and on unit_keys, not on T, the groups, the
+ * other rows or the launch. A row that sees no key is zero. head_dim 1..128,
+ * any block_size. max_len bounds start + count of every sequence; keys from the
+ * unit after it on are not seen. work: dkv_shared_attention_workspace() bytes,
+ * 16-byte aligned; none (it may be NULL) where that is 0. */
+size_t dkv_shared_attention_workspace(const dkv_paged_t* cache, int32_t T, int32_t n_q_heads, int32_t max_len,
+                                      int32_t unit_keys);
+int dkv_shared_attention(const dkv_paged_t* cache, const dkv_groups_t* groups, int32_t layer, const void* q,
+                         int32_t q_dtype, int32_t T, int32_t n_q_heads, const int32_t* start, const int32_t* count,
+                         int32_t max_len, int32_t unit_keys, void* out, void* work, size_t work_bytes,
+                         dkv_stream_t stream);
+
 /* ------------------------------------------------------------ mirror append / evict */
 /* Quantize and append T rows per sequence to one layer of the mirror, then
  * evict down to budget[s] -- replaces draftkv/compress.py:122-133 (`append`)
@@ -345,6 +391,23 @@ int dkv_accept_noalloc(const float* target, const float* draft, const int32_t* d
                        int32_t batch, int32_t gamma, int32_t vocab, float temperature,
                        const double* u, const dkv_row_stats_t* draft_stats, int32_t* accepted,
                        int32_t* next_token, int32_t* n_uniforms, dkv_stream_t stream);
+
+/* ---------------------------------------------------------------- beam search */
+/* The k best continuations of each prompt's beams (no counterpart in the
+ * reference, which decodes one sequence, engine.py:108-119):
+ * score(b, v) = scores[p][b] + (x - logsumexp(row)) in float64, x the logit of
+ * token v in row p * beams + b (DKV_F32 or DKV_BF16, rows row_stride elements
+ * apart), in the order (score, lowest beam, largest logit, lowest token).
+ * Outputs [prompts][k]: the score, its beam and its token, best first; -infinity,
+ * -1 and -1 where there are fewer. Tokens at -infinity, rows that hold NaN or
+ * +infinity and beams at -infinity or NaN have none. k 1..128, beams * k up to
+ * 4096, vocab up to 1048576, prompts * beams up to 65535. A row's scores do not
+ * depend on the other rows. work: dkv_beam_select_workspace() bytes, 8-byte
+ * aligned. */
+size_t dkv_beam_select_workspace(int32_t prompts, int32_t beams, int32_t vocab, int32_t k);
+int dkv_beam_select(const void* logits, int32_t dtype, int64_t row_stride, int32_t prompts, int32_t beams, int32_t vocab,
+                    const double* scores, int32_t k, double* out_scores, int32_t* out_parents, int32_t* out_tokens,
+                    void* work, size_t work_bytes, dkv_stream_t stream);
 
 /* ------------------------------------------------------ model forward ops */
 /* The non-attention pieces of the model forwards (reference
