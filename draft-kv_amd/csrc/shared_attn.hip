@@ -40,6 +40,9 @@ typedef __bf16 sa_bf16x2 __attribute__((ext_vector_type(2)));
 typedef float sa_f32x2 __attribute__((ext_vector_type(2)));
 typedef float sa_f32x4 __attribute__((ext_vector_type(4)));
 typedef float sa_f32x16 __attribute__((ext_vector_type(16)));
+// (callers' q and out need their elements' alignment only)
+typedef float sa_f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint16_t sa_u16x4u __attribute__((ext_vector_type(4), aligned(2)));
 
 constexpr int SA_ROWS = 32, SA_STEP = 32, SA_WAVES = 4;
 
@@ -51,7 +54,8 @@ struct SharedArgs {
     int n_groups;
     int units_p, tiles_p;    // prefix tasks: units and row tiles per (group, KV head)
     int unit_s, units_s, tiles_s;   // the sequences' own: first unit, units and row tiles per (sequence, KV head)
-    int64_t n_prefix, n_tasks;
+    bool wide_p, wide_s;     // a workgroup's waves share a unit's keys
+    int64_t blocks_p, tasks_p, tasks_s;   // prefix workgroups; tasks of waves, or of (unit, head) pairs where wide
     const int32_t* first;    // [n_groups + 1]
     const int32_t* shared;   // [batch]
     const void* q;
@@ -89,353 +93,644 @@ __device__ __forceinline__ void sa_split(float a, float b, sa_bf16x8 (&o)[NS], i
     }
 }
 
+// at most N of the wave's loads still in flight; its LDS reads and writes done
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// the key of row m of a K operand: bits 2 and 3 exchanged
+__device__ __forceinline__ int sa_key_of(int m) { return (m & 0x13) | (m & 4) << 1 | (m & 8) >> 1; }
+
 // rows a sequence has after this call, within its block table
 __device__ __forceinline__ int sa_len(const SharedArgs& A, int s) {
     return min(A.start[s] + (A.count ? A.count[s] : A.T), A.c.max_blocks * A.c.block_size);
 }
 
-// F32: float32 cache. NS: bf16 parts of a query. DP: head_dim rounded up to 32.
-// FAST: whole 16-token runs and aligned 16-byte loads.
-template <bool F32, bool QBF16, int DP, bool FAST>
-__global__ void __launch_bounds__(64 * SA_WAVES, 2) shared_attn_kernel(SharedArgs A) {
-    constexpr int NS = QBF16 ? 1 : 3, PS = QBF16 ? 2 : 3;   // bf16 parts of queries and probabilities
-    constexpr int DT = DP / 32;
+// Staging of the FAST path: 1 KB loads straight to LDS, 16 bytes per lane, into a step's 32 keys of K and V.
+//   K: of 16 keys, 64 bytes each (channels 64 B * piece ..): lane = 16 * (16-byte chunk) + key. A K operand of the
+//     product (16 bytes of channels of one key per lane) is one conflict-free 16-byte read.
+//   V^T: rows of 16 keys as they lie in the page, but for a swap of 16-byte chunks between rows (sa_v_chunk), so that
+//     an operand read covers all banks.
+template <bool F32, int DP>
+struct SharedStage {
+    static constexpr int ESIZE = F32 ? 4 : 2;
+    static constexpr int KPC = DP * ESIZE / 64;      // K loads per 16 keys
+    static constexpr int K_BYTES = 2 * KPC * 1024;
+    static constexpr int VROWS = 1024 / (16 * ESIZE);   // V^T rows per load
+    static constexpr int VPC = DP / VROWS;           // V loads per 16 keys
+    static constexpr int V_BYTES = 2 * VPC * 1024;
+    static constexpr int LOADS = 2 * KPC + 2 * VPC;
+    static constexpr int BYTES = K_BYTES + V_BYTES;
+    static constexpr int STAGES = 4;                 // of a block's waves together; a wave alone has one of them
+    static_assert(KPC == VPC && LOADS % SA_WAVES == 0, "loads split evenly");
+};
+// where the 16-byte chunk of a V^T row lies (its own inverse)
+template <bool F32>
+__device__ __forceinline__ int sa_v_chunk(int row, int chunk) {
+    return F32 ? chunk ^ (row >> 2 & 3) : chunk ^ (row >> 3 & 1);
+}
+
+// A wave's task: a tile of 32 rows of one KV head and a unit of keys. The lane's row, and what is the same in the wave.
+struct SharedTask {
+    int u, h, s0;            // unit, KV head, the sequence whose table is read
+    int k_begin, k_there;    // the unit's first key, and where the keys that are there end
+    int w_last, w_all;       // the last key that any row of the wave sees, and that all of them see
+    bool rvalid, live;       // the lane has a row; it sees a key
+    int last, row_last;      // the row's last key; the same, and no bound for rows that do not count
+    int64_t orow, prow;      // rows of q and out, and of the partials
+};
+
+// tile, u, h, s0: the same in the wave. False: no such task.
+__device__ __forceinline__ bool sa_task(const SharedArgs& A, bool prefix, int tile, int u, int h, int s0, int members, SharedTask& k) {
     const dkv_paged_t& c = A.c;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), lane = threadIdx.x % WAVE;
-    const int col = lane % 32, half = lane / 32;
-    const int D = c.head_dim, bs = c.block_size, G = A.G, H = c.n_kv_heads;
-
-    // ---- the wave's task: a tile of 32 rows of one KV head, and a unit of keys
-    int64_t task = (int64_t)blockIdx.x * SA_WAVES + wave;
-    if (task >= A.n_tasks) return;
-    const bool prefix = task < A.n_prefix;
-    int tile, u, h, s0, members;
-    if (prefix) {
-        tile = (int)(task % A.tiles_p), task /= A.tiles_p;
-        u = (int)(task % A.units_p), task /= A.units_p;
-        h = (int)(task % H);
-        const int g = (int)(task / H);
-        s0 = min(max(A.first[g], 0), c.batch), members = min(max(A.first[g + 1], s0), c.batch) - s0;
-    } else {
-        task -= A.n_prefix;
-        tile = (int)(task % A.tiles_s), task /= A.tiles_s;
-        u = A.unit_s + (int)(task % A.units_s), task /= A.units_s;
-        h = (int)(task % H), s0 = (int)(task / H), members = 1;
-    }
-    if (members <= 0) return;
-    const int per = A.Tn * G;                       // rows of one sequence
-    const int n_rows = members * per, r0 = tile * SA_ROWS;
-    if (r0 >= n_rows) return;
-    // units of the group's shared keys: the prefix tasks', the others' the sequences' own
-    const int shared_units = A.units_p ? min(max(min(A.shared[s0], c.max_blocks * bs), 0) / A.unit, A.units_p) : 0;
-    if (prefix != (u < shared_units)) return;
-    const int k_begin = u * A.unit;
-
-    // ---- the lane's row
+    const int lane = threadIdx.x % WAVE, col = lane % 32;
+    const int per = A.Tn * A.G, n_rows = members * per, r0 = tile * SA_ROWS;   // rows of one sequence, of all
+    k.u = u, k.h = h, k.s0 = s0;
+    k.k_begin = u * A.unit;
+    k.rvalid = r0 + col < n_rows;
     const int r = min(r0 + col, n_rows - 1);
-    const bool rvalid = r0 + col < n_rows;
-    const int s = s0 + r / per, t = A.t0 + r % per / G, hq = h * G + r % G;
-    const int len = sa_len(A, s), last = min(A.start[s] + t, len - 1);   // the row's last key
-    const bool live = rvalid && last >= 0;
-    const int64_t orow = ((int64_t)s * A.T + t) * A.Hq + hq;
-    const int64_t prow = (((int64_t)s * A.Tn + (t - A.t0)) * A.Hq + hq) * A.n_units;
-    // the last key that any row of the wave sees, and that all of them see (dead rows see what they like)
-    int w_last = live ? last : -1, w_all = live ? last : INT_MAX;
+    const int s = s0 + r / per, t = A.t0 + r % per / A.G, hq = h * A.G + r % A.G;
+    k.last = min(A.start[s] + t, sa_len(A, s) - 1);
+    k.live = k.rvalid && k.last >= 0;
+    k.orow = ((int64_t)s * A.T + t) * A.Hq + hq;
+    k.prow = (((int64_t)s * A.Tn + (t - A.t0)) * A.Hq + hq) * A.n_units;
+    int w_last = k.live ? k.last : -1, w_all = k.live ? k.last : INT_MAX;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         w_last = max(w_last, __shfl_xor(w_last, o));
         w_all = min(w_all, __shfl_xor(w_all, o));
     }
-    w_last = __builtin_amdgcn_readfirstlane(w_last), w_all = __builtin_amdgcn_readfirstlane(w_all);
-    const int row_last = live ? last : INT_MAX;
-    auto put = [&](int64_t i, float x) {
-        if constexpr (QBF16) static_cast<uint16_t*>(A.out)[i] = f32_to_bf16_rne(x);
-        else static_cast<float*>(A.out)[i] = x;
-    };
-    if (u == 0 && rvalid && !live)   // an empty sequence
-        for (int d = half; d < D; d += 2) put(orow * D + d, 0.0f);
-    if (w_last < k_begin) return;
-    // the keys that are there (a prefix unit lies whole in the shared keys)
-    const int k_there = prefix ? k_begin + A.unit : min(sa_len(A, s0), k_begin + A.unit);
-    const int k_end = min(k_there, w_last + 1);
+    k.w_last = __builtin_amdgcn_readfirstlane(w_last), k.w_all = __builtin_amdgcn_readfirstlane(w_all);
+    k.row_last = k.live ? k.last : INT_MAX;
+    // (a prefix unit lies whole in the shared keys)
+    const int len = __builtin_amdgcn_readfirstlane(sa_len(A, s0));
+    k.k_there = prefix ? k.k_begin + A.unit : min(len, k.k_begin + A.unit);
+    return r0 < n_rows;
+}
 
-    // ---- queries: B operands
-    constexpr int KS = F32 ? DP / 8 : DP / 16;
+// K and V^T operands: 16 (8) channels of a lane's key, 8 keys of a lane's channel; element by element from memory.
+template <bool F32>
+using sa_Kop = std::conditional_t<F32, sa_f32x4, sa_bf16x8>;
+template <bool F32>
+struct sa_Vop {
+    sa_Kop<F32> v[F32 ? 2 : 1];
+};
+template <bool F32>
+__device__ __forceinline__ sa_Kop<F32> sa_kop(const SharedArgs& A, const SharedTask& k, const int32_t* btab, int kb, int j) {
+    constexpr int N = F32 ? 4 : 8;
+    const dkv_paged_t& c = A.c;
+    const int lane = threadIdx.x % WAVE, bs = c.block_size, kp = min(kb + sa_key_of(lane % 32), k.k_there - 1);
+    const int32_t blk = btab[kp / bs];
+    sa_Kop<F32> o;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        const int d = N * (2 * j + lane / 32) + e;
+        const float x = d < c.head_dim ? load_elem(c.pool, paged_k_off(c, blk, kp % bs, k.h, d), c.dtype) : 0.0f;
+        if constexpr (F32) o[e] = x;
+        else o[e] = (__bf16)x;
+    }
+    return o;
+}
+// (past the cache's end zero: whatever the page holds, 0 * it could be NaN; FINITE: so are infinities and NaN)
+template <bool F32, bool FINITE>
+__device__ __forceinline__ sa_Vop<F32> sa_vop(const SharedArgs& A, const SharedTask& k, const int32_t* btab, int kb, int dt, int x) {
+    const dkv_paged_t& c = A.c;
+    const int lane = threadIdx.x % WAVE, bs = c.block_size, d = 32 * dt + lane % 32;
+    sa_Vop<F32> v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int vp = kb + 16 * x + 8 * (lane / 32) + e;
+        float w = d < c.head_dim && vp < k.k_there ? load_elem(c.pool, paged_v_off(c, btab[vp / bs], vp % bs, k.h, d), c.dtype) : 0.0f;
+        if (FINITE && !(fabsf(w) < INFINITY)) w = 0.0f;
+        if constexpr (F32) v.v[e / 4][e % 4] = w;
+        else v.v[0][e] = (__bf16)w;
+    }
+    return v;
+}
+
+// Scores to probabilities of a step's 16 keys of the lane, and the factor of what was summed before.
+__device__ __forceinline__ float sa_softmax(const SharedArgs& A, const SharedTask& k, int kb, float (&p)[16], float& m_run, float& l_run) {
+    if (kb + SA_STEP - 1 > k.w_all || kb + SA_STEP > k.k_there) {   // uniform: some row does not see the whole step
+        const int lim = min(k.row_last, k.k_there - 1) - kb - 8 * (int)(threadIdx.x % WAVE / 32);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (16 * (i / 8) + i % 8 > lim) p[i] = -INFINITY;
+    }
+    float mx = p[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, p[i]);
+    const float m_new = fmaxf(m_run, sa_max_halves(mx));
+    const float ms = m_new == -INFINITY ? 0.0f : m_new;   // a row that sees no key yet: p = 0
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        p[i] = sa_exp2(p[i] - ms);
+        sum += p[i];
+    }
+    const float alpha = m_new == m_run ? 1.0f : sa_exp2(m_run - m_new);
+    l_run = l_run * alpha + sum;
+    m_run = m_new;
+    return alpha;
+}
+
+// One wave's walk: queries, sums and a step of 32 keys.
+template <bool F32, bool QBF16, int DP>
+struct SharedWalk {
+    static constexpr int NS = QBF16 ? 1 : 3, PS = QBF16 ? 2 : 3;   // bf16 parts of queries and probabilities
+    static constexpr int DT = DP / 32, KS = F32 ? DP / 8 : DP / 16;
+    using Kop = sa_Kop<F32>;
+    using Vop = sa_Vop<F32>;
     sa_bf16x8 qp[F32 ? 1 : KS][NS];
     sa_f32x4 qf[F32 ? KS : 1];
-    {
-        auto at = [&](int d) -> float { return d < D ? load_elem(A.q, orow * D + d, QBF16 ? DKV_BF16 : DKV_F32) : 0.0f; };
-        if constexpr (F32) {
-#pragma unroll
-            for (int j = 0; j < KS; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) qf[j][e] = at(8 * j + 4 * half + e) * A.qscale;
-        } else {
-#pragma unroll
-            for (int j = 0; j < KS; ++j)
-#pragma unroll
-                for (int e = 0; e < 8; e += 2) {
-                    const float x = at(16 * j + 8 * half + e), y = at(16 * j + 8 * half + e + 1);
-                    // (bf16 queries stay whole: their scores are scaled)
-                    if constexpr (NS == 1) sa_split<NS>(x, y, qp[j], e);
-                    else sa_split<NS>(x * A.qscale, y * A.qscale, qp[j], e);
-                }
-        }
-    }
-
-    const int32_t* btab = c.block_table + ((int64_t)s0 * c.n_layers + A.layer) * c.max_blocks;
-    const int64_t bel = paged_block_elems(c);
-    const int key_of = (col & 0x13) | (col & 4) << 1 | (col & 8) >> 1;   // bits 2 and 3 exchanged
-
     sa_f32x16 acc[DT];
     float m_run, l_run;
-    auto clear = [&]() {
+
+    // channels 8 j + 4 half + e (float32 cache), 16 j + 8 half + e
+    __device__ __forceinline__ void set_query(int j, const float* x, float qscale) {
+        if constexpr (F32) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) qf[j][e] = x[e] * qscale;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {   // (bf16 queries stay whole: their scores are scaled)
+                if constexpr (NS == 1) sa_split<NS>(x[e], x[e + 1], qp[j], e);
+                else sa_split<NS>(x[e] * qscale, x[e + 1] * qscale, qp[j], e);
+            }
+        }
+    }
+    __device__ __forceinline__ void queries(const SharedArgs& A, const SharedTask& k) {   // any head_dim and alignment
+        constexpr int N = F32 ? 4 : 8;
+        const int half = threadIdx.x % WAVE / 32, D = A.c.head_dim;
+#pragma unroll
+        for (int j = 0; j < KS; ++j) {
+            float x[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const int d = N * (2 * j + half) + e;
+                x[e] = d < D ? load_elem(A.q, k.orow * D + d, QBF16 ? DKV_BF16 : DKV_F32) : 0.0f;
+            }
+            set_query(j, x, A.qscale);
+        }
+    }
+    __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int i = 0; i < DT; ++i)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][e] = 0.0f;
         m_run = -INFINITY, l_run = 0.0f;
-    };
-
-    // One walk over the unit, K and V straight from memory. Careful: values that are not finite, one by one.
-    auto walk = [&](auto careful) {
-      constexpr bool CAREFUL = decltype(careful)::value;
-      clear();
-      for (int kb = k_begin; kb < k_end; kb += SA_STEP) {
-        // ---- K and V operands of 32 keys
-        float kf[F32 ? KS : 1][4];
-        sa_bf16x8 kr[F32 ? 1 : KS];
-        float vf[F32 ? DT : 1][2][8];
-        sa_bf16x8 vr[F32 ? 1 : DT][2];
-        const int last_there = k_there - 1;
-        if constexpr (FAST) {
-            const int p0 = kb, p1 = min(kb + 16, last_there & ~15);   // two runs of 16 tokens
-            const int32_t b0 = __builtin_amdgcn_readfirstlane(btab[p0 / bs]), b1 = __builtin_amdgcn_readfirstlane(btab[p1 / bs]);
-            const int64_t g0 = b0 * bel, g1 = b1 * bel;
-            const int64_t kat = (key_of < 16 ? g0 : g1) + ((int64_t)h * bs + (key_of < 16 ? p0 : p1) % bs + key_of % 16) * DP;
-            const int64_t vrow = (int64_t)H * bs * DP + ((int64_t)h * DP + col) * bs + 8 * half;
-            if constexpr (F32) {
-                const float* pool = static_cast<const float*>(c.pool);
-#pragma unroll
-                for (int j = 0; j < KS; ++j) {
-                    const sa_f32x4 x = *reinterpret_cast<const sa_f32x4*>(pool + kat + 8 * j + 4 * half);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) kf[j][e] = x[e];
-                }
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                    for (int x = 0; x < 2; ++x)
-#pragma unroll
-                        for (int y = 0; y < 2; ++y) {
-                            const sa_f32x4 w = *reinterpret_cast<const sa_f32x4*>(
-                                pool + (x ? g1 : g0) + vrow + (int64_t)32 * dt * bs + (x ? p1 : p0) % bs + 4 * y);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) vf[dt][x][4 * y + e] = w[e];
-                        }
-            } else {
-                const uint16_t* pool = static_cast<const uint16_t*>(c.pool);
-#pragma unroll
-                for (int j = 0; j < KS; ++j) kr[j] = *reinterpret_cast<const sa_bf16x8*>(pool + kat + 16 * j + 8 * half);
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                    for (int x = 0; x < 2; ++x)
-                        vr[dt][x] = *reinterpret_cast<const sa_bf16x8*>(pool + (x ? g1 : g0) + vrow + (int64_t)32 * dt * bs +
-                                                                        (x ? p1 : p0) % bs);
-            }
-        } else {
-            const int kp = min(kb + key_of, last_there);
-            const int32_t kblk = btab[kp / bs];
-            auto kelem = [&](int d) { return d < D ? load_elem(c.pool, paged_k_off(c, kblk, kp % bs, h, d), c.dtype) : 0.0f; };
-            if constexpr (F32) {
-#pragma unroll
-                for (int j = 0; j < KS; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) kf[j][e] = kelem(8 * j + 4 * half + e);
-            } else {
-#pragma unroll
-                for (int j = 0; j < KS; ++j)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) kr[j][e] = (__bf16)kelem(16 * j + 8 * half + e);
-            }
-#pragma unroll
-            for (int x = 0; x < 2; ++x)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int vp = min(kb + 16 * x + 8 * half + e, last_there);
-                    const int32_t vblk = btab[vp / bs];
-#pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) {
-                        const int d = 32 * dt + col;
-                        const float w = d < D ? load_elem(c.pool, paged_v_off(c, vblk, vp % bs, h, d), c.dtype) : 0.0f;
-                        if constexpr (F32) vf[dt][x][e] = w;
-                        else vr[dt][x][e] = (__bf16)w;
-                    }
-                }
-        }
-        // ---- scores: lane holds keys kb + 16 x + 8 half + e of its row at 8 x + e
+    }
+    // Keys kb .. kb + 31. kop(j): the K operand of 16 (8) channels; between(): the scores are there, K is free; vop(dt, x):
+    // the V^T operand of 32 channels and 16 keys. The lane holds key kb + 16 x + 8 half + e at 8 x + e.
+    template <class K, class B, class V>
+    __device__ __forceinline__ void step(const SharedArgs& A, const SharedTask& k, int kb, K&& kop, B&& between, V&& vop) {
         sa_f32x16 sc;
 #pragma unroll
         for (int e = 0; e < 16; ++e) sc[e] = 0.0f;
-        if constexpr (F32) {
 #pragma unroll
-            for (int j = 0; j < KS; ++j)
+        for (int j = 0; j < KS; ++j) {
+            const Kop x = kop(j);
+            if constexpr (F32) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sc = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[j][e], qf[j][e], sc, 0, 0, 0);
-        } else {
+                for (int e = 0; e < 4; ++e) sc = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], qf[j][e], sc, 0, 0, 0);
+            } else {
 #pragma unroll
-            for (int j = 0; j < KS; ++j)
-#pragma unroll
-                for (int i = 0; i < NS; ++i) sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kr[j], qp[j][i], sc, 0, 0, 0);
-        }
-        float p[16];
-#pragma unroll
-        for (int k = 0; k < 16; ++k) p[k] = !F32 && NS == 1 ? sc[k] * A.qscale : sc[k];
-        const bool masked = kb + SA_STEP - 1 > w_all || kb + SA_STEP > k_there;   // uniform
-        const int k_lane = kb + 8 * half;
-        if constexpr (CAREFUL && !F32 && NS > 1) {
-            // An infinity times a query's parts is no number where they differ in sign or one is 0: its score again,
-            // channel by channel.
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                if (p[k] == p[k]) continue;
-                const int kp = min(k_lane + 16 * (k / 8) + k % 8, k_there - 1);
-                const int32_t blk = btab[kp / bs];
-                float x = 0.0f;
-                for (int d = 0; d < D; ++d)
-                    x += load_elem(A.q, orow * D + d, DKV_F32) * A.qscale * load_elem(c.pool, paged_k_off(c, blk, kp % bs, h, d), c.dtype);
-                p[k] = x;
+                for (int i = 0; i < NS; ++i) sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, qp[j][i], sc, 0, 0, 0);
             }
         }
-        if (masked) {
-            const int lim = min(row_last, k_there - 1);
+        between();
+        float p[16];
 #pragma unroll
-            for (int k = 0; k < 16; ++k)
-                if (k_lane + 16 * (k / 8) + k % 8 > lim) p[k] = -INFINITY;
-        }
-        float mx = p[0];
-#pragma unroll
-        for (int k = 1; k < 16; ++k) mx = fmaxf(mx, p[k]);
-        const float m_new = fmaxf(m_run, sa_max_halves(mx));
-        const float ms = m_new == -INFINITY ? 0.0f : m_new;   // a row that sees no key yet: p = 0
-        float sum = 0.0f;
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-            p[k] = sa_exp2(p[k] - ms);
-            sum += p[k];
-        }
-        const float alpha = m_new == m_run ? 1.0f : sa_exp2(m_run - m_new);
-        l_run = l_run * alpha + sum;
-        m_run = m_new;
+        for (int i = 0; i < 16; ++i) p[i] = !F32 && NS == 1 ? sc[i] * A.qscale : sc[i];
+        const float alpha = sa_softmax(A, k, kb, p, m_run, l_run);
         if (__any(alpha != 1.0f)) {
 #pragma unroll
             for (int i = 0; i < DT; ++i)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) acc[i][e] *= alpha;
         }
-        // ---- V past the cache's end: zero (whatever the page holds, 0 * it could be NaN)
-        if (kb + SA_STEP > k_there) {
 #pragma unroll
-            for (int x = 0; x < 2; ++x)
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (k_lane + 16 * x + e >= k_there)
-#pragma unroll
-                        for (int dt = 0; dt < DT; ++dt) {
-                            if constexpr (F32) vf[dt][x][e] = 0.0f;
-                            else vr[dt][x][e] = (__bf16)0.0f;
-                        }
-        }
-        if constexpr (CAREFUL) {   // infinities and NaN of V: out of the product, to the rows that see them by hand
-            for (int x = 0; x < 2; ++x)
-                for (int hh = 0; hh < 2; ++hh)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        float pk = 0.0f;
-#pragma unroll
-                        for (int y = 0; y < 2; ++y) {
-                            const float z = __shfl(p[8 * y + e], col + 32 * hh);
-                            pk = y == x ? z : pk;
-                        }
-                        const bool sees = kb + 16 * x + 8 * hh + e <= row_last;
-#pragma unroll
-                        for (int dt = 0; dt < DT; ++dt) {
-                            float w = 0.0f;
-#pragma unroll
-                            for (int y = 0; y < 2; ++y)
-                                if (y == x) {
-                                    if constexpr (F32) w = vf[dt][y][e];
-                                    else w = (float)vr[dt][y][e];
-                                }
-                            if (!__any(!(fabsf(w) < INFINITY))) continue;
-#pragma unroll
-                            for (int k = 0; k < 16; ++k) {   // the lane's channels of this tile
-                                const float v = __shfl(w, 8 * (k / 4) + 4 * half + k % 4 + 32 * hh);
-                                if (sees && !(fabsf(v) < INFINITY)) acc[dt][k] += pk * v;
-                            }
-                        }
-                    }
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                for (int x = 0; x < 2; ++x)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        if constexpr (F32) {
-                            if (!(fabsf(vf[dt][x][e]) < INFINITY)) vf[dt][x][e] = 0.0f;
-                        } else {
-                            if (!(fabsf((float)vr[dt][x][e]) < INFINITY)) vr[dt][x][e] = (__bf16)0.0f;
-                        }
-                    }
-        }
-        // ---- O^T += V^T . P^T
-        if constexpr (F32) {
-#pragma unroll
-            for (int x = 0; x < 2; ++x)
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-#pragma unroll
-                    for (int dt = 0; dt < DT; ++dt)
-                        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf[dt][x][e], p[8 * x + e], acc[dt], 0, 0, 0);
-        } else {
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                sa_bf16x8 pp[PS];
+        for (int x = 0; x < 2; ++x) {
+            sa_bf16x8 pp[F32 ? 1 : PS];
+            if constexpr (!F32)
 #pragma unroll
                 for (int e = 0; e < 8; e += 2) sa_split<PS>(p[8 * x + e], p[8 * x + e + 1], pp, e);
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt)
+            for (int dt = 0; dt < DT; ++dt) {
+                const Vop v = vop(dt, x);
+                if constexpr (F32) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(v.v[e / 4][e % 4], p[8 * x + e], acc[dt], 0, 0, 0);
+                } else {
 #pragma unroll
                     for (int i = 0; i < PS; ++i)
-                        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vr[dt][x], pp[i], acc[dt], 0, 0, 0);
+                        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v.v[0], pp[i], acc[dt], 0, 0, 0);
+                }
             }
         }
-      }
-    };
-    walk(std::false_type{});
-    // A NaN: of a key that its row sees, or 0 times what it does not. Again, and telling them apart.
-    bool odd = l_run != l_run;
+    }
+    // The whole unit with K and V element by element from memory.
+    __device__ __forceinline__ void unit(const SharedArgs& A, const SharedTask& k) {
+        const int32_t* btab = A.c.block_table + ((int64_t)k.s0 * A.c.n_layers + A.layer) * A.c.max_blocks;
+        clear();
+        const int k_end = min(k.k_there, k.w_last + 1);
+#pragma unroll 1
+        for (int kb = k.k_begin; kb < k_end; kb += SA_STEP)
+            step(A, k, kb, [&](int j) { return sa_kop<F32>(A, k, btab, kb, j); }, [] {},
+                 [&](int dt, int x) { return sa_vop<F32, false>(A, k, btab, kb, dt, x); });
+    }
+    // The walk met a NaN: of a key that its row sees, or 0 times one that it does not.
+    __device__ __forceinline__ bool odd() const {
+        bool o = l_run != l_run;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
+        for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int k = 0; k < 16; ++k) odd |= acc[dt][k] != acc[dt][k];
-    if (__any(odd)) walk(std::true_type{});
-    // ---- out: channels 32 dt + 8 (k / 4) + 4 half + k % 4 of the lane's row
-    const float l = sa_sum_halves(l_run);
-    if (!live) return;
-    const bool alone = last < A.unit || A.n_units == 1;   // the row sees one unit
-    if (alone && u > 0) return;
+            for (int i = 0; i < 16; ++i) o |= acc[dt][i] != acc[dt][i];
+        return __builtin_amdgcn_readfirstlane(__any(o)) != 0;
+    }
+    __device__ __forceinline__ static void put(const SharedArgs& A, int64_t i, float x) {
+        if constexpr (QBF16) static_cast<uint16_t*>(A.out)[i] = f32_to_bf16_rne(x);
+        else static_cast<float*>(A.out)[i] = x;
+    }
+    // The row's state out: channels 32 dt + 8 (i / 4) + 4 half + i % 4. WIDE: head_dim is DP.
+    template <bool WIDE>
+    __device__ __forceinline__ void store(const SharedArgs& A, const SharedTask& k) const {
+        const int half = threadIdx.x % WAVE / 32, D = WIDE ? DP : A.c.head_dim;
+        const float l = sa_sum_halves(l_run);
+        if (!k.live) return;
+        const bool alone = k.last < A.unit || A.n_units == 1;   // the row sees one unit
+        if (alone && k.u > 0) return;
+        float* part = A.part + (k.prow + k.u) * D;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
+        for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-            const int d = 32 * dt + 8 * (k / 4) + 4 * half + k % 4;
-            if (d >= D) continue;
-            if (alone) put(orow * D + d, acc[dt][k] / l);
-            else A.part[(prow + u) * D + d] = acc[dt][k];
+            for (int i = 0; i < 16; i += 4) {
+                const int d = 32 * dt + 2 * i + 4 * half;
+                if constexpr (WIDE) {
+                    const sa_f32x4 o = {acc[dt][i], acc[dt][i + 1], acc[dt][i + 2], acc[dt][i + 3]};
+                    if (!alone) {
+                        *reinterpret_cast<sa_f32x4*>(part + d) = o;
+                    } else if constexpr (QBF16) {
+                        sa_u16x4u w;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) w[e] = f32_to_bf16_rne(o[e] / l);
+                        *reinterpret_cast<sa_u16x4u*>(static_cast<uint16_t*>(A.out) + k.orow * D + d) = w;
+                    } else {
+                        *reinterpret_cast<sa_f32x4u*>(static_cast<float*>(A.out) + k.orow * D + d) = sa_f32x4u{o[0] / l, o[1] / l, o[2] / l, o[3] / l};
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if (d + e >= D) continue;
+                        if (alone) put(A, k.orow * D + d + e, acc[dt][i + e] / l);
+                        else part[d + e] = acc[dt][i + e];
+                    }
+                }
+            }
+        if (!alone && half == 0) A.ml[k.prow + k.u] = make_float2(m_run, l);
+    }
+};
+
+// The unit again, for walks that met a NaN: of a key that its row sees, or 0 times what it does not. Infinities and NaN of
+// V stay out of the products and go to the rows that see them by hand; other rows get the same bits. 32 channels at a time:
+// it is rare, and must not be what the kernel's registers are counted by.
+template <bool F32, bool QBF16>
+__device__ __forceinline__ void sa_again(const SharedArgs& A, const SharedTask& k) {
+    constexpr int NS = QBF16 ? 1 : 3, PS = QBF16 ? 2 : 3, N = F32 ? 4 : 8;
+    const dkv_paged_t& c = A.c;
+    const int lane = threadIdx.x % WAVE, col = lane % 32, half = lane / 32, D = c.head_dim, bs = c.block_size;
+    const int32_t* btab = c.block_table + ((int64_t)k.s0 * c.n_layers + A.layer) * c.max_blocks;
+    const int k_end = min(k.k_there, k.w_last + 1);
+    auto q = [&](int d) { return d < D ? load_elem(A.q, k.orow * D + d, QBF16 ? DKV_BF16 : DKV_F32) : 0.0f; };
+#pragma unroll 1
+    for (int dt = 0; 32 * dt < D; ++dt) {
+        sa_f32x16 acc;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
+        float m_run = -INFINITY, l_run = 0.0f;
+#pragma unroll 1
+        for (int kb = k.k_begin; kb < k_end; kb += SA_STEP) {
+            sa_f32x16 sc;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sc[i] = 0.0f;
+#pragma unroll 1
+            for (int j = 0; 2 * N * j < (D + 31) / 32 * 32; ++j) {
+                const sa_Kop<F32> x = sa_kop<F32>(A, k, btab, kb, j);
+                if constexpr (F32) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        sc = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], q(N * (2 * j + half) + e) * A.qscale, sc, 0, 0, 0);
+                } else {
+                    sa_bf16x8 qp[NS];
+                    const float f = NS == 1 ? 1.0f : A.qscale;
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) sa_split<NS>(q(N * (2 * j + half) + e) * f, q(N * (2 * j + half) + e + 1) * f, qp, e);
+#pragma unroll
+                    for (int i = 0; i < NS; ++i) sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, qp[i], sc, 0, 0, 0);
+                }
+            }
+            float p[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) p[i] = !F32 && NS == 1 ? sc[i] * A.qscale : sc[i];
+            if constexpr (!F32 && NS > 1) {
+                // An infinity times a query's parts is no number where they differ in sign or one is 0: its score again,
+                // channel by channel
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (p[i] == p[i]) continue;
+                    const int kp = min(kb + 16 * (i / 8) + 8 * half + i % 8, k.k_there - 1);
+                    const int32_t blk = btab[kp / bs];
+                    float x = 0.0f;
+#pragma unroll 1
+                    for (int d = 0; d < D; ++d) x += q(d) * A.qscale * load_elem(c.pool, paged_k_off(c, blk, kp % bs, k.h, d), c.dtype);
+                    p[i] = x;
+                }
+            }
+            const float alpha = sa_softmax(A, k, kb, p, m_run, l_run);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[i] *= alpha;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                __builtin_amdgcn_sched_barrier(0);
+                const sa_Vop<F32> v = sa_vop<F32, true>(A, k, btab, kb, dt, x);
+                if constexpr (F32) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(v.v[e / 4][e % 4], p[8 * x + e], acc, 0, 0, 0);
+                } else {
+                    sa_bf16x8 pp[PS];
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) sa_split<PS>(p[8 * x + e], p[8 * x + e + 1], pp, e);
+#pragma unroll
+                    for (int i = 0; i < PS; ++i) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v.v[0], pp[i], acc, 0, 0, 0);
+                }
+            }
+#pragma unroll 1
+            for (int key = 0; key < SA_STEP && kb + key < k.k_there; ++key) {
+                float pk = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) pk = 16 * (i / 8) + i % 8 == (key & ~8) ? p[i] : pk;
+                pk = __shfl(pk, col + 4 * (key & 8));
+                if (kb + key > k.row_last) continue;
+                const int32_t blk = btab[(kb + key) / bs];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {   // the lane's channels
+                    if (i % 4 == 0) __builtin_amdgcn_sched_barrier(0);
+                    const int d = 32 * dt + 8 * (i / 4) + 4 * half + i % 4;
+                    const float z = d < D ? load_elem(c.pool, paged_v_off(c, blk, (kb + key) % bs, k.h, d), c.dtype) : 0.0f;
+                    if (!(fabsf(z) < INFINITY)) acc[i] += pk * z;
+                }
+            }
         }
-    if (!alone && half == 0) A.ml[prow + u] = make_float2(m_run, l);
+        const float l = sa_sum_halves(l_run);
+        const bool alone = k.last < A.unit || A.n_units == 1;
+        if (!k.live || (alone && k.u > 0)) continue;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            if (i % 4 == 0) __builtin_amdgcn_sched_barrier(0);
+            const int d = 32 * dt + 8 * (i / 4) + 4 * half + i % 4;
+            if (d >= D) continue;
+            if (!alone) A.part[(k.prow + k.u) * D + d] = acc[i];
+            else if constexpr (QBF16) static_cast<uint16_t*>(A.out)[k.orow * D + d] = f32_to_bf16_rne(acc[i] / l);
+            else static_cast<float*>(A.out)[k.orow * D + d] = acc[i] / l;
+        }
+        if (!alone && half == 0) A.ml[k.prow + k.u] = make_float2(m_run, l);
+    }
+}
+
+// DP: head_dim rounded up to 32. FAST: head_dim a multiple of 32, blocks of whole 16-token runs, an aligned pool.
+template <bool F32, bool QBF16, int DP, bool FAST>
+__global__ void __launch_bounds__(64 * SA_WAVES, 2) shared_attn_kernel(SharedArgs A) {
+    using St = SharedStage<F32, DP>;
+    using Walk = SharedWalk<F32, QBF16, DP>;
+    using Kop = typename Walk::Kop;
+    using Vop = typename Walk::Vop;
+    const dkv_paged_t& c = A.c;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), lane = threadIdx.x % WAVE;
+    const int col = lane % 32, half = lane / 32;
+    const int bs = c.block_size, H = c.n_kv_heads;
+
+    // ---- the wave's task, or, where there are many rows (wide), four tiles and a unit for the workgroup
+    int64_t task = blockIdx.x;
+    const bool prefix = task < A.blocks_p;
+    const bool wide = FAST && (prefix ? A.wide_p : A.wide_s);
+    const int tiles = prefix ? A.tiles_p : A.tiles_s, units = prefix ? A.units_p : A.units_s;
+    if (!prefix) task -= A.blocks_p;
+    int tile;
+    if (wide) {
+        // workgroups of one unit and head on one XCD (they are dealt out round robin): its L2 holds the keys
+        const int tb = (tiles + SA_WAVES - 1) / SA_WAVES;
+        const int64_t q = task / (8 * tb), r = task % (8 * tb);
+        tile = (int)(r / 8) * SA_WAVES + wave;
+        task = q * 8 + r % 8;
+        if (task >= (prefix ? A.tasks_p : A.tasks_s)) return;
+    } else {
+        task = task * SA_WAVES + wave;
+        if (task >= (prefix ? A.tasks_p : A.tasks_s)) return;
+        tile = (int)(task % tiles), task /= tiles;
+    }
+    int u = (int)(task % units);
+    task /= units;
+    const int h = (int)(task % H);
+    int s0 = (int)(task / H), members = 1;
+    if (prefix) {
+        const int g = s0;
+        s0 = __builtin_amdgcn_readfirstlane(min(max(A.first[g], 0), c.batch));
+        members = __builtin_amdgcn_readfirstlane(min(max(A.first[g + 1], s0), c.batch)) - s0;
+    } else {
+        u += A.unit_s;
+    }
+    if (members <= 0) return;
+    // units of the group's shared keys: the prefix tasks', the others' the sequences' own
+    const int shared = A.units_p ? __builtin_amdgcn_readfirstlane(A.shared[s0]) : 0;
+    const int shared_units = min(max(min(shared, c.max_blocks * bs), 0) / A.unit, A.units_p);
+    if (prefix != (u < shared_units)) return;
+    SharedTask k;
+    const bool mine = sa_task(A, prefix, tile, u, h, s0, members, k);
+    if (!mine && (!wide || (tile - wave) * SA_ROWS >= members * A.Tn * A.G)) return;
+    if (u == 0 && k.rvalid && !k.live)   // an empty sequence
+        for (int d = half; d < c.head_dim; d += 2) Walk::put(A, k.orow * c.head_dim + d, 0.0f);
+    if (!wide && k.w_last < k.k_begin) return;
+
+    Walk w;
+    if constexpr (!FAST) {
+        w.queries(A, k);
+        w.unit(A, k);
+    } else {
+        {   // whole vectors; loaded before any is used
+            constexpr int N = F32 ? 4 : 8;
+            float x[Walk::KS][N];
+#pragma unroll
+            for (int j = 0; j < Walk::KS; ++j)
+#pragma unroll
+                for (int y = 0; y < N; y += 4) {
+                    const int64_t at = k.orow * DP + N * (2 * j + half) + y;
+                    if constexpr (QBF16) {
+                        const sa_u16x4u q = *reinterpret_cast<const sa_u16x4u*>(static_cast<const uint16_t*>(A.q) + at);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[j][y + e] = bf16_to_f32(q[e]);
+                    } else {
+                        const sa_f32x4u q = *reinterpret_cast<const sa_f32x4u*>(static_cast<const float*>(A.q) + at);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[j][y + e] = q[e];
+                    }
+                }
+#pragma unroll
+            for (int j = 0; j < Walk::KS; ++j) w.set_query(j, x[j], A.qscale);
+        }
+        // ---- K and V through LDS
+        extern __shared__ __align__(16) char lds[];
+        int k_last = k.w_last;   // the last key of any row that the stages are for
+        if (wide) {
+            int* wl = reinterpret_cast<int*>(lds);
+            if (lane == 0) wl[wave] = k.w_last;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < SA_WAVES; ++i) k_last = max(k_last, wl[i]);
+            k_last = __builtin_amdgcn_readfirstlane(k_last);
+            __syncthreads();
+            if (k_last < k.k_begin) return;
+        }
+        const int nsteps = (min(k.k_there, k_last + 1) - k.k_begin + SA_STEP - 1) / SA_STEP;
+        const int32_t* btab = c.block_table + ((int64_t)s0 * c.n_layers + A.layer) * c.max_blocks;
+        constexpr int ES = St::ESIZE;
+        const int64_t block_bytes = paged_block_elems(c) * ES;
+        // block ids of the 16-key runs from run0 on, one per lane (the last run that is there for those past it)
+        const int last_run = (k.k_there - 1) / 16, first_run = k.k_begin / 16;
+        int run0 = first_run;
+        auto load_ids = [&]() { return btab[min(run0 + lane, last_run) * 16 / bs]; };
+        int ids = load_ids();
+        // a run's rows of K and V of the head
+        auto run_k = [&](int run) -> const char* {
+            run = min(run, last_run);
+            const int32_t blk = __builtin_amdgcn_readlane(ids, run - run0);
+            return static_cast<const char*>(c.pool) + blk * block_bytes + ((int64_t)h * bs + run * 16 % bs) * DP * ES;
+        };
+        auto run_v = [&](int run) -> const char* {
+            run = min(run, last_run);
+            const int32_t blk = __builtin_amdgcn_readlane(ids, run - run0);
+            return static_cast<const char*>(c.pool) + blk * block_bytes + (((int64_t)H + h) * bs * DP + run * 16 % bs) * ES;
+        };
+        // byte offsets of the lane in a load: K rows, V^T rows
+        const uint32_t klane = (uint32_t)((lane % 16) * DP * ES + lane / 16 * 16);
+        constexpr int VL = ES;   // 16-byte chunks of a V^T row of 16 keys
+        // (the swap is the same in every load: their rows are 16 or 32 apart)
+        const uint32_t vlane = (uint32_t)(lane / VL * bs * ES + sa_v_chunk<F32>(lane / VL, lane % VL) * 16);
+        const int64_t vpiece = (int64_t)St::VROWS * bs * ES;
+        const uint32_t kread = (uint32_t)((sa_key_of(col) >> 4) * St::KPC * 1024 + half * 256 + (sa_key_of(col) & 15) * 16);
+        auto kop_at = [&](const char* st, int j) {
+            return *reinterpret_cast<const Kop*>(st + kread + (j >> 1) * 1024 + (j & 1) * 512);
+        };
+        auto vop_at = [&](const char* st, int dt, int x) {
+            Vop v;
+#pragma unroll
+            for (int y = 0; y < (F32 ? 2 : 1); ++y) {
+                const int chunk = sa_v_chunk<F32>(col, F32 ? 2 * half + y : half);
+                v.v[y] = *reinterpret_cast<const Kop*>(st + St::K_BYTES + (x * DP + 32 * dt + col) * (16 * ES) + chunk * 16);
+            }
+            return v;
+        };
+        // V^T past the cache's end becomes zero
+        auto zero_past = [&](char* st, int live_keys, int thread, int threads) {
+            for (int i = thread; i < St::V_BYTES / 16; i += threads) {
+                const int row = i / VL % DP, key = 16 * (i / VL / DP) + sa_v_chunk<F32>(row, i % VL) * (16 / ES);
+#pragma unroll
+                for (int e = 0; e < 16 / ES; ++e)
+                    if (key + e >= live_keys) {
+                        if constexpr (F32) reinterpret_cast<float*>(st + St::K_BYTES + 16 * i)[e] = 0.0f;
+                        else reinterpret_cast<uint16_t*>(st + St::K_BYTES + 16 * i)[e] = 0;
+                    }
+            }
+        };
+        w.clear();
+        if (wide) {
+            constexpr int S = St::STAGES, LPW = St::LOADS / SA_WAVES;
+            auto issue = [&](int i) {   // this wave's share of step i's loads: K of two runs, then V of two runs
+                const int run = first_run + 2 * i;
+                const uint32_t to = lds_offset(lds) + (i % S) * St::BYTES;
+#pragma unroll
+                for (int x = 0; x < LPW; ++x) {
+                    const int l = wave * LPW + x;   // LOADS / 4 = KPC: a wave's loads are all K or V, of one run
+                    if (wave < 2) dma_b128<false>(run_k(run + wave) + 64 * x, klane, to + l * 1024);
+                    else dma_b128<false>(run_v(run + wave - 2) + x * vpiece, vlane, to + l * 1024);
+                }
+            };
+            static_assert(LPW == St::KPC && SA_WAVES == 4, "a wave loads K or V of one run");
+#pragma unroll
+            for (int i = 0; i < S - 1; ++i)
+                if (i < nsteps) issue(i);
+            for (int i = 0; i < nsteps; ++i) {
+                // this wave's loads of step i are done once those of the S - 2 later steps alone remain; the barrier
+                // makes every wave's visible, and frees the stage of step i - 1
+                const int later = min(S - 2, nsteps - 1 - i);
+                if (later >= 2) wait_loads_barrier<2 * LPW>();
+                else if (later == 1) wait_loads_barrier<LPW>();
+                else wait_loads_barrier<0>();
+                if (i + S - 1 < nsteps) {
+                    if (first_run + 2 * (i + S - 1) - run0 >= WAVE) run0 += WAVE, ids = load_ids();
+                    issue(i + S - 1);
+                }
+                const int kb = k.k_begin + SA_STEP * i;
+                char* st = lds + (i % S) * St::BYTES;
+                if (kb + SA_STEP > k.k_there) {
+                    zero_past(st, k.k_there - kb, threadIdx.x, 64 * SA_WAVES);
+                    __syncthreads();
+                }
+                if (kb > k.w_last) continue;   // uniform over the wave
+                w.step(A, k, kb, [&](int j) { return kop_at(st, j); }, [] {}, [&](int dt, int x) { return vop_at(st, dt, x); });
+            }
+        } else {
+            // one stage: K of the next step is fetched once this one's scores are there, V once its products are
+            char* st = lds + wave * St::BYTES;
+            const uint32_t to = lds_offset(st);
+            auto issue_k = [&](int i) {
+                const int run = first_run + 2 * i;
+                if (run - run0 >= WAVE) run0 += WAVE, ids = load_ids();
+#pragma unroll
+                for (int x = 0; x < 2 * St::KPC; ++x) dma_b128<false>(run_k(run + x / St::KPC) + 64 * (x % St::KPC), klane, to + x * 1024);
+            };
+            auto issue_v = [&](int i) {   // (after its K: the ids are there)
+                const int run = first_run + 2 * i;
+#pragma unroll
+                for (int x = 0; x < 2 * St::VPC; ++x)
+                    dma_b128<false>(run_v(run + x / St::VPC) + (x % St::VPC) * vpiece, vlane, to + St::K_BYTES + x * 1024);
+            };
+            issue_k(0);
+            issue_v(0);
+            for (int i = 0; i < nsteps; ++i) {
+                const int kb = k.k_begin + SA_STEP * i;
+                const bool more = i + 1 < nsteps;
+                wait_loads<2 * St::VPC>();   // K is there, V may be on its way
+                w.step(A, k, kb, [&](int j) { return kop_at(st, j); },
+                       [&]() {
+                           wait_lds();
+                           if (more) {
+                               issue_k(i + 1);
+                               wait_loads<2 * St::KPC>();
+                           } else {
+                               wait_loads<0>();
+                           }
+                           if (kb + SA_STEP > k.k_there) {
+                               zero_past(st, k.k_there - kb, lane, WAVE);
+                               wait_lds();
+                           }
+                       },
+                       [&](int dt, int x) { return vop_at(st, dt, x); });
+                if (more) {
+                    wait_lds();
+                    issue_v(i + 1);
+                }
+            }
+        }
+        if (!mine || k.w_last < k.k_begin) return;
+    }
+    if (!w.odd()) {
+        w.template store<FAST>(A, k);
+        return;
+    }
+    sa_again<F32, QBF16>(A, k);
 }
 
 // Merge of each row's units: their common maximum first, then the weighted
@@ -492,14 +787,23 @@ static int sa_units(const dkv_paged_t& c, int max_len, int unit) {
     return (int)((keys + unit - 1) / unit);
 }
 
+template <bool F32, bool QBF16, int DP, bool FAST>
+static int sa_launch_one(const SharedArgs& a, dim3 grid, hipStream_t st) {
+    auto kfn = shared_attn_kernel<F32, QBF16, DP, FAST>;
+    const size_t lds = FAST ? SharedStage<F32, DP>::BYTES * SharedStage<F32, DP>::STAGES : 0;
+    static size_t lds_done[16] = {};
+    if (!reserve_lds(reinterpret_cast<const void*>(kfn), lds, lds_done))
+        return fail(DKV_ELAUNCH, "dkv_shared_attention: cannot reserve " + std::to_string(lds) + " B of LDS");
+    hipLaunchKernelGGL(kfn, grid, dim3(64 * SA_WAVES), lds, st, a);
+    return check_launch("dkv_shared_attention");
+}
 template <bool F32, bool QBF16, bool FAST>
-static void sa_launch(const SharedArgs& a, dim3 grid, hipStream_t st) {
-    const dim3 blk(64 * SA_WAVES);
+static int sa_launch(const SharedArgs& a, dim3 grid, hipStream_t st) {
     switch ((a.c.head_dim + 31) / 32) {
-        case 1: hipLaunchKernelGGL((shared_attn_kernel<F32, QBF16, 32, FAST>), grid, blk, 0, st, a); break;
-        case 2: hipLaunchKernelGGL((shared_attn_kernel<F32, QBF16, 64, FAST>), grid, blk, 0, st, a); break;
-        case 3: hipLaunchKernelGGL((shared_attn_kernel<F32, QBF16, 96, FAST>), grid, blk, 0, st, a); break;
-        default: hipLaunchKernelGGL((shared_attn_kernel<F32, QBF16, 128, FAST>), grid, blk, 0, st, a); break;
+        case 1: return sa_launch_one<F32, QBF16, 32, FAST>(a, grid, st);
+        case 2: return sa_launch_one<F32, QBF16, 64, FAST>(a, grid, st);
+        case 3: return sa_launch_one<F32, QBF16, 96, FAST>(a, grid, st);
+        default: return sa_launch_one<F32, QBF16, 128, FAST>(a, grid, st);
     }
 }
 
@@ -569,26 +873,29 @@ extern "C" int dkv_shared_attention(const dkv_paged_t* cache, const dkv_groups_t
         a.unit_s = g.n_groups ? std::min(g.min_shared / unit_keys, a.n_units - 1) : 0;
         a.units_s = a.n_units - a.unit_s;
         a.tiles_s = (int)((per + SA_ROWS - 1) / SA_ROWS);
-        a.n_prefix = (int64_t)a.n_groups * c.n_kv_heads * a.units_p * a.tiles_p;
-        a.n_tasks = a.n_prefix + (int64_t)c.batch * c.n_kv_heads * a.units_s * a.tiles_s;
-        const int64_t blocks = (a.n_tasks + SA_WAVES - 1) / SA_WAVES;
+        // (unit, head) pairs; a workgroup's four waves take four tiles of one (wide), or four tasks of a tile each
+        const int64_t pairs_p = (int64_t)a.n_groups * c.n_kv_heads * a.units_p, pairs_s = (int64_t)c.batch * c.n_kv_heads * a.units_s;
+        a.wide_p = fast && a.tiles_p >= 3, a.wide_s = fast && a.tiles_s >= 3;
+        auto blocks_of = [](bool wide, int64_t pairs, int tiles, int64_t& tasks) {
+            tasks = wide ? pairs : pairs * tiles;
+            return wide ? (pairs + 7) / 8 * 8 * ((tiles + SA_WAVES - 1) / SA_WAVES) : (tasks + SA_WAVES - 1) / SA_WAVES;
+        };
+        a.blocks_p = blocks_of(a.wide_p, pairs_p, a.tiles_p, a.tasks_p);
+        const int64_t blocks = a.blocks_p + blocks_of(a.wide_s, pairs_s, a.tiles_s, a.tasks_s);
         DKV_REQUIRE(blocks < (1LL << 31), "dkv_shared_attention: grid too large");
         const dim3 grid((unsigned)blocks);
-#define DKV_SA(FF, QQ)                                    \
-    do {                                                  \
-        if (fast) sa_launch<FF, QQ, true>(a, grid, st);   \
-        else sa_launch<FF, QQ, false>(a, grid, st);       \
-    } while (0)
+        int e;
+#define DKV_SA(FF, QQ) e = fast ? sa_launch<FF, QQ, true>(a, grid, st) : sa_launch<FF, QQ, false>(a, grid, st)
         if (f32 && qb) DKV_SA(true, true);
         else if (f32) DKV_SA(true, false);
         else if (qb) DKV_SA(false, true);
         else DKV_SA(false, false);
 #undef DKV_SA
-        if (const int e = check_launch("dkv_shared_attention")) return e;
+        if (e) return e;
         if (a.n_units == 1) continue;
         if (qb) hipLaunchKernelGGL(shared_merge_kernel<true>, dim3((unsigned)rows), dim3(64 * SM_CLASSES), 0, st, a);
         else hipLaunchKernelGGL(shared_merge_kernel<false>, dim3((unsigned)rows), dim3(64 * SM_CLASSES), 0, st, a);
-        if (const int e = check_launch("dkv_shared_attention(merge)")) return e;
+        if ((e = check_launch("dkv_shared_attention(merge)"))) return e;
     }
     return DKV_OK;
 }
