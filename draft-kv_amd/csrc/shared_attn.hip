@@ -6,13 +6,11 @@
 //     s_k = q . K_k / sqrt(D),  out = sum_k 2^(s_k - m) V_k / sum_k 2^(s_k - m)
 //     over the keys k <= position of the row (scores in base 2, m their maximum)
 //
-// Keys are cut at absolute positions into units of `unit` keys. A row's state
-// (m, l, o) over a unit is computed on its own by an online softmax in steps of
-// 32 keys, and the merge adds a row's units in an order of their own. So a
-// row's result is a function of its keys alone: not of T, of the other rows of
-// the call, nor of what is shared. The units that lie whole in a group's
-// shared keys are computed for 32 rows of any of its sequences at a time, the
-// others for 32 rows of one sequence.
+// Of a row's keys the first B, what its group shares rounded down to 32, are cut into pieces of `prefix` keys, the others
+// from B on into units of `unit`. A row's state (m, l, o) over a piece is computed on its own by an online softmax in
+// steps of 32 keys, and the merge adds a row's pieces in an order of their own. So a row's result is a function of its
+// keys and B alone: not of T, nor of the other rows of the call. A piece of shared keys is computed for 32 rows of any of
+// the group's sequences at a time, the others for 32 rows of one sequence.
 //
 // Products, the keys as the A operand:
 //     S^T[32 keys][32 rows] = K . Q^T,   O^T[32 d][32 rows] += V^T . P^T
@@ -50,10 +48,11 @@ struct SharedArgs {
     dkv_paged_t c;
     int layer, T, Hq, G;
     int t0, Tn;              // the rows of this launch: t0 .. t0 + Tn - 1 of every sequence
-    int unit, n_units;       // keys per unit; units that max_len reaches into
+    int prefix, unit;        // keys per piece of what groups share, and per unit of what sequences have of their own
     int n_groups;
-    int units_p, tiles_p;    // prefix tasks: units and row tiles per (group, KV head)
-    int unit_s, units_s, tiles_s;   // the sequences' own: first unit, units and row tiles per (sequence, KV head)
+    int units_p, tiles_p;    // prefix tasks: pieces and row tiles per (group, KV head)
+    int units_s, tiles_s;    // the sequences' own: units and row tiles per (sequence, KV head)
+    int n_slots;             // a row's partials: units_p, then units_s
     bool wide_p, wide_s;     // a workgroup's waves share a unit's keys
     int64_t blocks_p, tasks_p, tasks_s;   // prefix workgroups; tasks of waves, or of (unit, head) pairs where wide
     const int32_t* first;    // [n_groups + 1]
@@ -62,8 +61,8 @@ struct SharedArgs {
     const int32_t* start;
     const int32_t* count;
     float qscale;            // log2(e) / sqrt(head_dim)
-    float* part;             // o [row of the launch][n_units][D]
-    float2* ml;              // (m, l) [row of the launch][n_units]
+    float* part;             // o [row of the launch][n_slots][D]
+    float2* ml;              // (m, l) [row of the launch][n_slots]
     void* out;
 };
 
@@ -108,6 +107,18 @@ __device__ __forceinline__ int sa_len(const SharedArgs& A, int s) {
     return min(A.start[s] + (A.count ? A.count[s] : A.T), A.c.max_blocks * A.c.block_size);
 }
 
+// the keys that sequence s shares, as they are cut
+__device__ __forceinline__ int sa_shared(const SharedArgs& A, int s) {
+    return A.units_p ? min(min(max(A.shared[s], 0), A.c.max_blocks * A.c.block_size), A.units_p * A.prefix) & -SA_STEP : 0;
+}
+// the pieces of a row whose last key is `last`, `np` of them shared
+__device__ __forceinline__ int sa_pieces(const SharedArgs& A, int last, int B, int& np) {
+    if (last < 0) return np = 0;
+    if (last < B) return np = last / A.prefix + 1;
+    np = (B + A.prefix - 1) / A.prefix;
+    return np + min((last - B) / A.unit + 1, A.units_s);
+}
+
 // Staging of the FAST path: 1 KB loads straight to LDS, 16 bytes per lane, into a step's 32 keys of K and V.
 //   K: of 16 keys, 64 bytes each (channels 64 B * piece ..): lane = 16 * (16-byte chunk) + key. A K operand of the
 //     product (16 bytes of channels of one key per lane) is one conflict-free 16-byte read.
@@ -134,28 +145,32 @@ __device__ __forceinline__ int sa_v_chunk(int row, int chunk) {
 
 // A wave's task: a tile of 32 rows of one KV head and a unit of keys. The lane's row, and what is the same in the wave.
 struct SharedTask {
-    int u, h, s0;            // unit, KV head, the sequence whose table is read
-    int k_begin, k_there;    // the unit's first key, and where the keys that are there end
+    int slot, h, s0;         // the piece's partial, KV head, the sequence whose table is read
+    int k_begin, k_there;    // the piece's first key, and where its keys that are there end
     int w_last, w_all;       // the last key that any row of the wave sees, and that all of them see
     bool rvalid, live;       // the lane has a row; it sees a key
+    bool alone;              // and no piece but one
     int last, row_last;      // the row's last key; the same, and no bound for rows that do not count
     int64_t orow, prow;      // rows of q and out, and of the partials
 };
 
 // tile, u, h, s0: the same in the wave. False: no such task.
-__device__ __forceinline__ bool sa_task(const SharedArgs& A, bool prefix, int tile, int u, int h, int s0, int members, SharedTask& k) {
+__device__ __forceinline__ bool sa_task(const SharedArgs& A, bool prefix, int tile, int u, int h, int s0, int members, int B, SharedTask& k) {
     const dkv_paged_t& c = A.c;
     const int lane = threadIdx.x % WAVE, col = lane % 32;
     const int per = A.Tn * A.G, n_rows = members * per, r0 = tile * SA_ROWS;   // rows of one sequence, of all
-    k.u = u, k.h = h, k.s0 = s0;
-    k.k_begin = u * A.unit;
+    k.h = h, k.s0 = s0;
+    k.slot = prefix ? u : A.units_p + u;
+    k.k_begin = prefix ? u * A.prefix : B + u * A.unit;
     k.rvalid = r0 + col < n_rows;
     const int r = min(r0 + col, n_rows - 1);
     const int s = s0 + r / per, t = A.t0 + r % per / A.G, hq = h * A.G + r % A.G;
     k.last = min(A.start[s] + t, sa_len(A, s) - 1);
     k.live = k.rvalid && k.last >= 0;
     k.orow = ((int64_t)s * A.T + t) * A.Hq + hq;
-    k.prow = (((int64_t)s * A.Tn + (t - A.t0)) * A.Hq + hq) * A.n_units;
+    k.prow = (((int64_t)s * A.Tn + (t - A.t0)) * A.Hq + hq) * A.n_slots;
+    int np;
+    k.alone = sa_pieces(A, k.last, B, np) <= 1 || A.n_slots == 1;
     int w_last = k.live ? k.last : -1, w_all = k.live ? k.last : INT_MAX;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -164,9 +179,8 @@ __device__ __forceinline__ bool sa_task(const SharedArgs& A, bool prefix, int ti
     }
     k.w_last = __builtin_amdgcn_readfirstlane(w_last), k.w_all = __builtin_amdgcn_readfirstlane(w_all);
     k.row_last = k.live ? k.last : INT_MAX;
-    // (a prefix unit lies whole in the shared keys)
     const int len = __builtin_amdgcn_readfirstlane(sa_len(A, s0));
-    k.k_there = prefix ? k.k_begin + A.unit : min(len, k.k_begin + A.unit);
+    k.k_there = prefix ? min(B, k.k_begin + A.prefix) : min(len, k.k_begin + A.unit);
     return r0 < n_rows;
 }
 
@@ -360,9 +374,9 @@ struct SharedWalk {
         const int half = threadIdx.x % WAVE / 32, D = WIDE ? DP : A.c.head_dim;
         const float l = sa_sum_halves(l_run);
         if (!k.live) return;
-        const bool alone = k.last < A.unit || A.n_units == 1;   // the row sees one unit
-        if (alone && k.u > 0) return;
-        float* part = A.part + (k.prow + k.u) * D;
+        const bool alone = k.alone;
+        if (alone && k.k_begin > k.last) return;
+        float* part = A.part + (k.prow + k.slot) * D;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -389,7 +403,7 @@ struct SharedWalk {
                     }
                 }
             }
-        if (!alone && half == 0) A.ml[k.prow + k.u] = make_float2(m_run, l);
+        if (!alone && half == 0) A.ml[k.prow + k.slot] = make_float2(m_run, l);
     }
 };
 
@@ -485,18 +499,17 @@ __device__ __forceinline__ void sa_again(const SharedArgs& A, const SharedTask& 
             }
         }
         const float l = sa_sum_halves(l_run);
-        const bool alone = k.last < A.unit || A.n_units == 1;
-        if (!k.live || (alone && k.u > 0)) continue;
+        if (!k.live || (k.alone && k.k_begin > k.last)) continue;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             if (i % 4 == 0) __builtin_amdgcn_sched_barrier(0);
             const int d = 32 * dt + 8 * (i / 4) + 4 * half + i % 4;
             if (d >= D) continue;
-            if (!alone) A.part[(k.prow + k.u) * D + d] = acc[i];
+            if (!k.alone) A.part[(k.prow + k.slot) * D + d] = acc[i];
             else if constexpr (QBF16) static_cast<uint16_t*>(A.out)[k.orow * D + d] = f32_to_bf16_rne(acc[i] / l);
             else static_cast<float*>(A.out)[k.orow * D + d] = acc[i] / l;
         }
-        if (!alone && half == 0) A.ml[k.prow + k.u] = make_float2(m_run, l);
+        if (!k.alone && half == 0) A.ml[k.prow + k.slot] = make_float2(m_run, l);
     }
 }
 
@@ -531,7 +544,7 @@ __global__ void __launch_bounds__(64 * SA_WAVES, 2) shared_attn_kernel(SharedArg
         if (task >= (prefix ? A.tasks_p : A.tasks_s)) return;
         tile = (int)(task % tiles), task /= tiles;
     }
-    int u = (int)(task % units);
+    const int u = (int)(task % units);
     task /= units;
     const int h = (int)(task % H);
     int s0 = (int)(task / H), members = 1;
@@ -539,18 +552,14 @@ __global__ void __launch_bounds__(64 * SA_WAVES, 2) shared_attn_kernel(SharedArg
         const int g = s0;
         s0 = __builtin_amdgcn_readfirstlane(min(max(A.first[g], 0), c.batch));
         members = __builtin_amdgcn_readfirstlane(min(max(A.first[g + 1], s0), c.batch)) - s0;
-    } else {
-        u += A.unit_s;
     }
     if (members <= 0) return;
-    // units of the group's shared keys: the prefix tasks', the others' the sequences' own
-    const int shared = A.units_p ? __builtin_amdgcn_readfirstlane(A.shared[s0]) : 0;
-    const int shared_units = min(max(min(shared, c.max_blocks * bs), 0) / A.unit, A.units_p);
-    if (prefix != (u < shared_units)) return;
+    const int B = __builtin_amdgcn_readfirstlane(sa_shared(A, s0));
+    if (prefix && u * A.prefix >= B) return;
     SharedTask k;
-    const bool mine = sa_task(A, prefix, tile, u, h, s0, members, k);
+    const bool mine = sa_task(A, prefix, tile, u, h, s0, members, B, k);
     if (!mine && (!wide || (tile - wave) * SA_ROWS >= members * A.Tn * A.G)) return;
-    if (u == 0 && k.rvalid && !k.live)   // an empty sequence
+    if (k.k_begin == 0 && k.rvalid && !k.live)   // an empty sequence
         for (int d = half; d < c.head_dim; d += 2) Walk::put(A, k.orow * c.head_dim + d, 0.0f);
     if (!wide && k.w_last < k.k_begin) return;
 
@@ -733,9 +742,9 @@ __global__ void __launch_bounds__(64 * SA_WAVES, 2) shared_attn_kernel(SharedArg
     sa_again<F32, QBF16>(A, k);
 }
 
-// Merge of each row's units: their common maximum first, then the weighted
-// sums, units u, u + 4, ... in order and these four last, so the result depends
-// on the row's units alone. A wave per row and class.
+// Merge of each row's pieces: their common maximum first, then the weighted
+// sums, pieces u, u + 4, ... in order and these four last, so the result depends
+// on the row's pieces alone. A wave per row and class.
 constexpr int SM_CLASSES = 4;
 template <bool QBF16>
 __global__ void __launch_bounds__(64 * SM_CLASSES) shared_merge_kernel(SharedArgs A) {
@@ -745,21 +754,23 @@ __global__ void __launch_bounds__(64 * SM_CLASSES) shared_merge_kernel(SharedArg
     i /= A.Hq;
     const int t = A.t0 + (int)(i % A.Tn), s = (int)(i / A.Tn);
     const int last = min(A.start[s] + t, sa_len(A, s) - 1);
-    const int n = last < 0 ? 0 : min(last / A.unit + 1, A.n_units);
+    int np;
+    const int n = sa_pieces(A, last, sa_shared(A, s), np);
     if (n <= 1) return;   // the attention kernel wrote the row
-    const int64_t prow = (int64_t)blockIdx.x * A.n_units;
+    const int64_t prow = (int64_t)blockIdx.x * A.n_slots;
+    auto slot = [&](int i) { return prow + (i < np ? i : A.units_p + i - np); };
     float m = -INFINITY;
-    for (int u = lane; u < n; u += WAVE) m = fmaxf(m, A.ml[prow + u].x);
+    for (int u = lane; u < n; u += WAVE) m = fmaxf(m, A.ml[slot(u)].x);
     m = wave_max(m);
     const float ms = m == -INFINITY ? 0.0f : m;
     const int c0 = min(lane, D - 1), c1 = min(lane + WAVE, D - 1);
     float l = 0.0f, o0 = 0.0f, o1 = 0.0f;
     for (int u = w; u < n; u += SM_CLASSES) {
-        const float2 x = A.ml[prow + u];
+        const float2 x = A.ml[slot(u)];
         const float f = sa_exp2(x.x - ms);
         l = fmaf(x.y, f, l);
-        o0 = fmaf(A.part[(prow + u) * D + c0], f, o0);
-        o1 = fmaf(A.part[(prow + u) * D + c1], f, o1);
+        o0 = fmaf(A.part[slot(u) * D + c0], f, o0);
+        o1 = fmaf(A.part[slot(u) * D + c1], f, o1);
     }
     __shared__ float sl[SM_CLASSES], so[SM_CLASSES][2][WAVE];
     if (lane == 0) sl[w] = l;
@@ -776,15 +787,19 @@ __global__ void __launch_bounds__(64 * SM_CLASSES) shared_merge_kernel(SharedArg
 
 // Rows per launch: as many of the T as keep the partials within this
 constexpr size_t SA_WORK_BYTES = (size_t)512 << 20;
-static size_t sa_row_bytes(const dkv_paged_t& c, int Hq, int n_units) {   // of one t
-    return sizeof(float) * (size_t)c.batch * Hq * n_units * (c.head_dim + 2);
+static size_t sa_row_bytes(const dkv_paged_t& c, int Hq, int n_slots) {   // of one t
+    return sizeof(float) * (size_t)c.batch * Hq * n_slots * (c.head_dim + 2);
 }
-static int sa_rows(const dkv_paged_t& c, int T, int Hq, int n_units) {
-    return (int)std::min<size_t>(T, std::max<size_t>(1, SA_WORK_BYTES / sa_row_bytes(c, Hq, n_units)));
+static int sa_rows(const dkv_paged_t& c, int T, int Hq, int n_slots) {
+    return (int)std::min<size_t>(T, std::max<size_t>(1, SA_WORK_BYTES / sa_row_bytes(c, Hq, n_slots)));
 }
-static int sa_units(const dkv_paged_t& c, int max_len, int unit) {
+// Pieces that shared keys, and the others up to max_len, are cut into at most
+static void sa_units(const dkv_paged_t& c, const dkv_groups_t& g, int max_len, int prefix, int unit, int& units_p, int& units_s) {
     const int64_t keys = std::min<int64_t>(max_len, (int64_t)c.max_blocks * c.block_size);
-    return (int)((keys + unit - 1) / unit);
+    const int64_t most = g.n_groups ? std::min<int64_t>(g.max_shared / SA_STEP, (keys + SA_STEP - 1) / SA_STEP) * SA_STEP : 0;
+    const int64_t least = g.n_groups ? g.min_shared / SA_STEP * SA_STEP : 0;
+    units_p = (int)((most + prefix - 1) / prefix);
+    units_s = least < keys ? (int)((keys - least + unit - 1) / unit) : 0;
 }
 
 template <bool F32, bool QBF16, int DP, bool FAST>
@@ -807,7 +822,7 @@ static int sa_launch(const SharedArgs& a, dim3 grid, hipStream_t st) {
     }
 }
 
-static int sa_check(const dkv_paged_t& c, const dkv_groups_t& g, int T, int Hq, int max_len, int unit) {
+static int sa_check(const dkv_paged_t& c, const dkv_groups_t& g, int T, int Hq, int max_len, int prefix, int unit) {
     DKV_REQUIRE(c.dtype == DKV_F32 || c.dtype == DKV_BF16, "dkv_shared_attention: bad cache dtype");
     DKV_REQUIRE(c.batch > 0 && c.n_layers > 0 && c.n_kv_heads > 0 && c.block_size > 0 && c.max_blocks > 0,
                 "dkv_shared_attention: bad cache shape");
@@ -815,6 +830,7 @@ static int sa_check(const dkv_paged_t& c, const dkv_groups_t& g, int T, int Hq, 
     DKV_REQUIRE(c.head_dim > 0 && c.head_dim <= 128, "dkv_shared_attention: head_dim must be 1..128");
     DKV_REQUIRE(Hq > 0 && Hq % c.n_kv_heads == 0, "dkv_shared_attention: query heads must be a multiple of KV heads");
     DKV_REQUIRE(unit > 0 && unit % SA_STEP == 0, "dkv_shared_attention: unit_keys must be a multiple of 32");
+    DKV_REQUIRE(prefix > 0 && prefix % SA_STEP == 0, "dkv_shared_attention: prefix_keys must be a multiple of 32");
     DKV_REQUIRE(max_len > 0, "dkv_shared_attention: max_len must be > 0");
     DKV_REQUIRE(T >= 0 && (int64_t)c.batch * T * Hq < (1LL << 31), "dkv_shared_attention: too many rows");
     DKV_REQUIRE(g.n_groups >= 0 && g.n_groups <= c.batch, "dkv_shared_attention: n_groups must lie in 0..batch");
@@ -826,23 +842,24 @@ static int sa_check(const dkv_paged_t& c, const dkv_groups_t& g, int T, int Hq, 
 
 }  // namespace dkv
 
-extern "C" size_t dkv_shared_attention_workspace(const dkv_paged_t* cache, int32_t T, int32_t n_q_heads, int32_t max_len,
-                                                 int32_t unit_keys) {
-    if (!cache || T <= 0 || n_q_heads <= 0 || max_len <= 0 || unit_keys <= 0 || cache->batch <= 0) return 0;
-    const int n = dkv::sa_units(*cache, max_len, unit_keys);
-    if (n <= 1) return 0;
-    return dkv::sa_rows(*cache, T, n_q_heads, n) * dkv::sa_row_bytes(*cache, n_q_heads, n) + 8;   // (m, l) on 8 bytes
+extern "C" size_t dkv_shared_attention_workspace(const dkv_paged_t* cache, const dkv_groups_t* groups, int32_t T,
+                                                 int32_t n_q_heads, int32_t max_len, int32_t prefix_keys, int32_t unit_keys) {
+    if (!cache || !groups || T <= 0 || dkv::sa_check(*cache, *groups, T, n_q_heads, max_len, prefix_keys, unit_keys)) return 0;
+    int p, s;
+    dkv::sa_units(*cache, *groups, max_len, prefix_keys, unit_keys, p, s);
+    if (p + s <= 1) return 0;
+    return dkv::sa_rows(*cache, T, n_q_heads, p + s) * dkv::sa_row_bytes(*cache, n_q_heads, p + s) + 8;   // (m, l) on 8 bytes
 }
 
 extern "C" int dkv_shared_attention(const dkv_paged_t* cache, const dkv_groups_t* groups, int32_t layer, const void* q,
                                     int32_t q_dtype, int32_t T, int32_t n_q_heads, const int32_t* start,
-                                    const int32_t* count, int32_t max_len, int32_t unit_keys, void* out, void* work,
-                                    size_t work_bytes, dkv_stream_t stream) {
+                                    const int32_t* count, int32_t max_len, int32_t prefix_keys, int32_t unit_keys, void* out,
+                                    void* work, size_t work_bytes, dkv_stream_t stream) {
     using namespace dkv;
     DKV_REQUIRE(cache && groups, "dkv_shared_attention: NULL argument");
     const dkv_paged_t c = *cache;
     const dkv_groups_t g = *groups;
-    const int rc = sa_check(c, g, T, n_q_heads, max_len, unit_keys);
+    const int rc = sa_check(c, g, T, n_q_heads, max_len, prefix_keys, unit_keys);
     if (rc) return rc;
     DKV_REQUIRE(layer >= 0 && layer < c.n_layers, "dkv_shared_attention: layer out of range");
     DKV_REQUIRE(q_dtype == DKV_F32 || q_dtype == DKV_BF16, "dkv_shared_attention: bad query dtype");
@@ -851,14 +868,16 @@ extern "C" int dkv_shared_attention(const dkv_paged_t* cache, const dkv_groups_t
                 "dkv_shared_attention: NULL argument");
     SharedArgs a = {};
     a.c = c, a.layer = layer, a.T = T, a.Hq = n_q_heads, a.G = n_q_heads / c.n_kv_heads;
-    a.unit = unit_keys, a.n_units = sa_units(c, max_len, unit_keys);
+    a.prefix = prefix_keys, a.unit = unit_keys;
+    sa_units(c, g, max_len, prefix_keys, unit_keys, a.units_p, a.units_s);
+    a.n_slots = a.units_p + a.units_s;
     a.n_groups = g.n_groups, a.first = g.first, a.shared = g.shared;
     a.q = q, a.start = start, a.count = count, a.out = out;
     a.qscale = static_cast<float>(1.4426950408889634 / sqrt(static_cast<double>(c.head_dim)));
-    const size_t need = dkv_shared_attention_workspace(cache, T, n_q_heads, max_len, unit_keys);
+    const size_t need = dkv_shared_attention_workspace(cache, groups, T, n_q_heads, max_len, prefix_keys, unit_keys);
     if (need && (!work || work_bytes < need))
         return fail(DKV_EWORKSPACE, "dkv_shared_attention: workspace too small (need " + std::to_string(need) + ")");
-    const int step = sa_rows(c, T, n_q_heads, a.n_units);
+    const int step = sa_rows(c, T, n_q_heads, a.n_slots);
     hipStream_t st = as_stream(stream);
     const bool f32 = c.dtype == DKV_F32, qb = q_dtype == DKV_BF16;
     const bool fast = c.block_size % 16 == 0 && c.head_dim % 32 == 0 && reinterpret_cast<uintptr_t>(c.pool) % 16 == 0;
@@ -866,12 +885,9 @@ extern "C" int dkv_shared_attention(const dkv_paged_t* cache, const dkv_groups_t
         a.Tn = std::min(step, T - a.t0);
         const int64_t rows = (int64_t)c.batch * a.Tn * n_q_heads;
         a.part = static_cast<float*>(work);
-        a.ml = reinterpret_cast<float2*>(a.part + (rows * a.n_units * c.head_dim + 1) / 2 * 2);
+        a.ml = reinterpret_cast<float2*>(a.part + (rows * a.n_slots * c.head_dim + 1) / 2 * 2);
         const int64_t per = (int64_t)a.Tn * a.G;
-        a.units_p = g.n_groups ? std::min(g.max_shared / unit_keys, a.n_units) : 0;
         a.tiles_p = (int)((g.max_members * per + SA_ROWS - 1) / SA_ROWS);
-        a.unit_s = g.n_groups ? std::min(g.min_shared / unit_keys, a.n_units - 1) : 0;
-        a.units_s = a.n_units - a.unit_s;
         a.tiles_s = (int)((per + SA_ROWS - 1) / SA_ROWS);
         // (unit, head) pairs; a workgroup's four waves take four tiles of one (wide), or four tasks of a tile each
         const int64_t pairs_p = (int64_t)a.n_groups * c.n_kv_heads * a.units_p, pairs_s = (int64_t)c.batch * c.n_kv_heads * a.units_s;
@@ -892,7 +908,7 @@ extern "C" int dkv_shared_attention(const dkv_paged_t* cache, const dkv_groups_t
         else DKV_SA(false, false);
 #undef DKV_SA
         if (e) return e;
-        if (a.n_units == 1) continue;
+        if (a.n_slots == 1) continue;
         if (qb) hipLaunchKernelGGL(shared_merge_kernel<true>, dim3((unsigned)rows), dim3(64 * SM_CLASSES), 0, st, a);
         else hipLaunchKernelGGL(shared_merge_kernel<false>, dim3((unsigned)rows), dim3(64 * SM_CLASSES), 0, st, a);
         if ((e = check_launch("dkv_shared_attention(merge)"))) return e;

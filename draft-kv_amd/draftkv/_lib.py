@@ -67,8 +67,8 @@ _SIGS = {
     "dkv_paged8_attention": (C.c_int, [PPaged8, I32, P, I32, I32, I32, P, P, I32, P, P, SZ, P]),
     "dkv_paged8_read": (C.c_int, [PPaged8, I32, P, P, I32, P, P, P]),
     "dkv_paged_copy": (C.c_int, [P, I64, I64, P, P, I64, P]),
-    "dkv_shared_attention_workspace": (SZ, [PPaged, I32, I32, I32, I32]),
-    "dkv_shared_attention": (C.c_int, [PPaged, PGroups, I32, P, I32, I32, I32, P, P, I32, I32, P, P, SZ, P]),
+    "dkv_shared_attention_workspace": (SZ, [PPaged, PGroups, I32, I32, I32, I32, I32]),
+    "dkv_shared_attention": (C.c_int, [PPaged, PGroups, I32, P, I32, I32, I32, P, P, I32, I32, I32, P, P, SZ, P]),
     "dkv_page_bytes": (I64, [I32, I32, I32, I32]),
     "dkv_drafter_append": (C.c_int, [PDrafter, I32, QCfg, P, P, I32, I32, P, P, P, P]),
     "dkv_drafter_truncate": (C.c_int, [PDrafter, PQCfg, P, P]),

@@ -367,13 +367,14 @@ class PrefixGroups:
         return Groups(self.mem.data_ptr() + 4 * self.batch, self.mem.data_ptr(), *self.bounds())
 
 
-def shared_attention(desc: Paged, layer: int, q: torch.Tensor, start: torch.Tensor, max_len: int, unit_keys: int,
-                     groups: Optional[PrefixGroups] = None, out: Optional[torch.Tensor] = None,
+def shared_attention(desc: Paged, layer: int, q: torch.Tensor, start: torch.Tensor, max_len: int, prefix_keys: int,
+                     unit_keys: int, groups: Optional[PrefixGroups] = None, out: Optional[torch.Tensor] = None,
                      count: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Causal attention of q [batch, T, Hq, D] (float32 or bfloat16; the result has its type) over a paged cache whose
     sequences share prefixes: what ``groups`` have in common is read once for all their rows. start, max_len and count
-    as for ``paged_attention``. Keys are summed in units of ``unit_keys`` (a multiple of 32) at absolute positions: a
-    row's bits depend on its keys and on that alone, neither on the groups nor on T."""
+    as for ``paged_attention``. Shared keys (their number rounded down to 32) are summed in pieces of ``prefix_keys``, the
+    others in units of ``unit_keys`` (multiples of 32): a row's bits depend on its keys, on how many of them its group
+    shares and on these two, not on T or the other rows."""
     _need(q, "q", ndim=4)
     b, T, Hq, D = q.shape
     if b != desc.batch or D != desc.head_dim:
@@ -390,10 +391,10 @@ def shared_attention(desc: Paged, layer: int, q: torch.Tensor, start: torch.Tens
             raise ValueError(f"out must have q's shape {tuple(q.shape)} and device")
     g = Groups() if groups is None else groups.desc()
     with _device(q.device):
-        nbytes = lib().dkv_shared_attention_workspace(C.byref(desc), T, Hq, max_len, unit_keys)
+        nbytes = lib().dkv_shared_attention_workspace(C.byref(desc), C.byref(g), T, Hq, max_len, prefix_keys, unit_keys)
         ws = _WS.get(q.device, nbytes) if nbytes else None
         check(lib().dkv_shared_attention(C.byref(desc), C.byref(g), layer, q.data_ptr(), _dt(q), T, Hq, start.data_ptr(),
-                                         _ptr(count), max_len, unit_keys, out.data_ptr(), _ptr(ws),
+                                         _ptr(count), max_len, prefix_keys, unit_keys, out.data_ptr(), _ptr(ws),
                                          0 if ws is None else ws.numel(), _stream()), "dkv_shared_attention")
     return out
 

@@ -20,7 +20,7 @@ import numpy as np
 import torch
 
 from . import ops
-from .paged import BlockPool, BlockPoolExhausted, PagedKVCache, _torch_dtype, default_device
+from .paged import BlockPool, BlockPoolExhausted, PagedKVCache, _torch_dtype, auto_chunk_keys, default_device
 
 
 class PagePool(BlockPool):
@@ -59,22 +59,28 @@ class PagePool(BlockPool):
         assert set(np.flatnonzero(self.refs > 0).tolist()) == self._live, "holders of free blocks"
 
 
-def auto_unit_keys(batch: int, n_heads: int, max_tokens: int) -> int:
-    """Keys per unit of the shared attention, from the prompts at the cache's making: a power of two in [128, 1024]."""
-    units = max(1.0, batch * n_heads * max_tokens / 1024.0)
-    return int(min(1024, max(128, 1 << int(round(math.log2(units))))))
+def auto_prefix_keys(batch: int, n_heads: int, max_tokens: int) -> int:
+    """Keys per piece of what a prompt's continuations share, from the prompts at the cache's making: about 512 pieces (two
+    workgroups per CU) over them, a power of two in [128, 1024]."""
+    return int(min(1024, max(128, 1 << int(round(math.log2(max(1.0, batch * n_heads * max_tokens / 512.0)))))))
+
+
+UNIT_KEYS = 128   # keys per unit of a sequence's own
 
 
 class SharedKVCache(PagedKVCache):
     """``PagedKVCache`` with pages that sequences share.
 
     ``n_blocks`` is the pages of the one pool, each ``block_size`` tokens of all layers. ``batch`` is the number of
-    sequences at first (the prompts); ``fork`` changes it. float32 or bfloat16. ``chunk_keys`` is the unit of the
-    attention's sums (a multiple of 32): plain and drafted decoding over caches with the same unit agree bit for bit."""
+    sequences at first (the prompts); ``fork`` changes it. float32 or bfloat16. The attention sums what
+    a group shares in pieces of ``prefix_keys`` and the rest in units of ``unit_keys`` (multiples of 32): plain and drafted
+    decoding over caches with the same ones agree bit for bit. Prompts into an empty cache go through PagedKVCache's
+    attention, in chunks of ``chunk_keys``."""
 
     def __init__(self, n_layers: int, n_heads: int, d_head: int, block_size: int = 16, n_blocks: int = 512,
                  dtype=np.float32, *, batch: int = 1, max_tokens: Optional[int] = None, device=None,
-                 chunk_keys: Optional[int] = None) -> None:
+                 chunk_keys: Optional[int] = None, prefix_keys: Optional[int] = None,
+                 unit_keys: Optional[int] = None) -> None:
         self.dtype = _torch_dtype(dtype)
         if self.dtype == torch.float8_e4m3fn:
             raise ValueError("a cache in 8 bits does not share pages (its open blocks' rows are per sequence): float32 or bfloat16")
@@ -86,9 +92,12 @@ class SharedKVCache(PagedKVCache):
         self.block_size, self.n_blocks, self.batch = block_size, n_blocks, batch
         self.device = torch.device(device) if device is not None else default_device()
         self.max_tokens = max_tokens if max_tokens is not None else n_blocks * block_size
-        self.chunk_keys = chunk_keys if chunk_keys is not None else auto_unit_keys(batch, n_heads, self.max_tokens)
-        if self.chunk_keys < 32 or self.chunk_keys % 32:
-            raise ValueError(f"chunk_keys must be a multiple of 32, got {self.chunk_keys}")
+        self.chunk_keys = chunk_keys if chunk_keys is not None else auto_chunk_keys(batch, n_heads, self.max_tokens)
+        self.prefix_keys = prefix_keys if prefix_keys is not None else auto_prefix_keys(batch, n_heads, self.max_tokens)
+        self.unit_keys = unit_keys if unit_keys is not None else UNIT_KEYS
+        for name in ("chunk_keys", "prefix_keys", "unit_keys"):
+            if getattr(self, name) < 32 or getattr(self, name) % 32:
+                raise ValueError(f"{name} must be a multiple of 32, got {getattr(self, name)}")
         self.max_blocks = -(-self.max_tokens // block_size)
         self.fp8 = False
         self.pools = [PagePool(n_blocks, block_size)]
@@ -263,7 +272,7 @@ class SharedKVCache(PagedKVCache):
 
     def graph_key(self) -> tuple:
         """What a recorded forward over this cache depends on beside its buffers' addresses."""
-        return self.groups.bounds()
+        return (*self.groups.bounds(), self.prefix_keys, self.unit_keys)
 
     # ------------------------------------------------------------ device ops
     def append_layer(self, layer: int, k: torch.Tensor, v: torch.Tensor, start: torch.Tensor,
@@ -278,7 +287,11 @@ class SharedKVCache(PagedKVCache):
         start[s] .., with what the sequences share read once."""
         self._here(q)
         self._sync_groups()
-        return ops.shared_attention(self.desc(), layer, q, start, max_len, self.chunk_keys, self.groups, out, count)
+        if q.dtype == torch.float32 and q.shape[1] > 1 and not self.n_tokens.any():
+            # prompts: nothing is shared yet, and there are rows enough for the kernel whose workgroups walk the keys
+            return ops.paged_attention(self.desc(), layer, q, start, max_len, self.chunk_keys, out, count)
+        return ops.shared_attention(self.desc(), layer, q, start, max_len, self.prefix_keys, self.unit_keys, self.groups, out,
+                                    count)
 
     # ------------------------------------------------------------ views
     def read(self, layer: int, seq: int = 0):

@@ -230,19 +230,22 @@ typedef struct {
  * for all of its rows. q and out: DKV_F32 or DKV_BF16 (q_dtype both),
  * [batch][T][Hq][D]. Against a bf16 cache float32 queries and probabilities
  * enter the products in three bf16 parts, bf16 queries whole and their
- * probabilities in two; against a float32 cache the products are float32. Keys
- * are cut at absolute positions into units of unit_keys (a multiple of 32): a
- * row's result depends on its keys and on unit_keys, not on T, the groups, the
- * other rows or the launch. A row that sees no key is zero. head_dim 1..128,
- * any block_size. max_len bounds start + count of every sequence; keys from the
- * unit after it on are not seen. work: dkv_shared_attention_workspace() bytes,
- * 16-byte aligned; none (it may be NULL) where that is 0. */
-size_t dkv_shared_attention_workspace(const dkv_paged_t* cache, int32_t T, int32_t n_q_heads, int32_t max_len,
-                                      int32_t unit_keys);
+ * probabilities in two; against a float32 cache the products are float32. The
+ * shared keys, their number rounded down to 32, are cut into pieces of
+ * prefix_keys, the others from there on into units of unit_keys (both
+ * multiples of 32): a row's result depends on its keys, on how many of them
+ * its group shares and on these two, not on T, the other rows or the launch. A
+ * row that sees no key is zero. head_dim 1..128, any block_size. max_len bounds
+ * start + count of every sequence; of a longer one no key is seen past the
+ * piece or unit that max_len lies in. work:
+ * dkv_shared_attention_workspace() bytes, 16-byte aligned; none (it may be
+ * NULL) where that is 0. */
+size_t dkv_shared_attention_workspace(const dkv_paged_t* cache, const dkv_groups_t* groups, int32_t T,
+                                      int32_t n_q_heads, int32_t max_len, int32_t prefix_keys, int32_t unit_keys);
 int dkv_shared_attention(const dkv_paged_t* cache, const dkv_groups_t* groups, int32_t layer, const void* q,
                          int32_t q_dtype, int32_t T, int32_t n_q_heads, const int32_t* start, const int32_t* count,
-                         int32_t max_len, int32_t unit_keys, void* out, void* work, size_t work_bytes,
-                         dkv_stream_t stream);
+                         int32_t max_len, int32_t prefix_keys, int32_t unit_keys, void* out, void* work,
+                         size_t work_bytes, dkv_stream_t stream);
 
 /* ------------------------------------------------------------ mirror append / evict */
 /* Quantize and append T rows per sequence to one layer of the mirror, then

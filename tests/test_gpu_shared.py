@@ -3,9 +3,9 @@ the engine's calls that use them, against plain implementations in 64 bits.
 
 Tolerances. u = 2^-24 is half a step of float32. A score is a float32 sum of up to 3 D products (each query in three bf16
 parts, which leave u of it; D products for a float32 cache) of size at most top = max_k sum_d |q_d k_d| / sqrt(D): it is off
-by (3 D + 4) u top, and 2^score-max by that, the difference's rounding (u of at most 2 top) and the instruction's 2 u. Sums over a
-unit's keys are chains of unit / 2 (l) and 3 unit (o, three parts of a probability) additions, then unit / 32 rescalings and
-n / unit units of the merge. So out is off by (2 (3 D + 8) top + 4 unit + n / unit + 16) u times sum_k p_k |v_k|, numerator and
+by (3 D + 4) u top, and 2^score-max by that, the difference's rounding (u of at most 2 top) and the instruction's 2 u. Sums
+over the keys of a piece (at most `unit` of them) are chains of unit / 2 (l) and 3 unit (o, three parts of a probability)
+additions, then unit / 32 rescalings and at most n / 32 pieces of the merge. So out is off by (2 (3 D + 8) top + 4 unit + n / 32 + 16) u times sum_k p_k |v_k|, numerator and
 denominator each taking the scores' part once. bf16 queries: probabilities hold two bf16 parts (2^-16 of each), and the output is
 rounded to bf16 (2^-8 of it).
 """
@@ -31,7 +31,8 @@ def i32(x):
 
 def new_cache(batch, H, D, bs, most, dtype, unit, pages, layers=1):
     from draftkv import SharedKVCache
-    c = SharedKVCache(layers, H, D, bs, pages, dtype, batch=batch, max_tokens=most, device="cuda", chunk_keys=unit)
+    c = SharedKVCache(layers, H, D, bs, pages, dtype, batch=batch, max_tokens=most, device="cuda", unit_keys=unit // 2 // 32 * 32 or 32,
+                      prefix_keys=unit)
     c.store.fill_(math.nan)        # whatever no row was written to must not be seen
     return c
 
@@ -82,11 +83,15 @@ def attention(q, k, v, last):
 
 
 def bound(out, size, top, D, unit, n, qdtype, cache_dtype):
-    e = (2 * (3 * D + 8) * top + 4 * unit + n / unit + 16) * U
+    e = (2 * (3 * D + 8) * top + 4 * unit + n / 32 + 16) * U
     if qdtype == BF16:
         e += 2.0 ** -16 if cache_dtype == BF16 else 0.0
         return e * size + 2.0 ** -8 * (out.abs() + e * size)
     return e * size
+
+
+def attend(c, q, start, most, groups, layer=0, **kw):
+    return ops.shared_attention(c.desc(), layer, q, i32(start), most, c.prefix_keys, c.unit_keys, groups, **kw)
 
 
 # D, KV heads, query heads per KV head, block, cache, unit, prompts, continuations each, T
@@ -118,17 +123,19 @@ def test_attention(dev, case, qdtype):
         tol = bound(want, size, top, D, unit, start[s] + T, qdtype, dtype)
         err = (out[s].to(F64) - want).abs()
         assert (err <= tol).all(), (s, float((err / tol.clamp(min=1e-300)).max()))
-    # the same bits without groups, and with any bound on the lengths
-    for groups, most in ((None, max(s + T for s in start)), (c.groups, c.max_blocks * bs), (None, c.max_blocks * bs)):
-        again = ops.shared_attention(c.desc(), 0, q, i32(start), most, unit, groups)
-        assert torch.equal(again, out), (groups is None, most)
+        # the same without groups
+        alone = attend(c, q, start, max(s + T for s in start), None)[s]
+        assert ((alone.to(F64) - want).abs() <= tol).all(), s
+    # the same bits with any bound on the lengths
+    assert torch.equal(attend(c, q, start, c.max_blocks * bs, c.groups), out)
 
 
 @pytest.mark.parametrize("qdtype", [F32, BF16])
 @pytest.mark.parametrize("D,H,G,dtype,unit,ctx,n,T", [(128, 2, 4, BF16, 256, 2500, 6, 9), (64, 3, 3, F32, 128, 700, 8, 5),
                                                      (8, 2, 2, F32, 32, 100, 3, 4), (64, 1, 4, BF16, 128, 1290, 12, 17)])
 def test_rows_do_not_depend_on_the_call(dev, D, H, G, dtype, unit, ctx, n, T, qdtype):
-    """Bit for bit: all rows in one call, one row per call, one sequence per call, and a group cut in several."""
+    """Bit for bit: all rows in one call, one row per call, and groups cut up; a sequence alone, with what it shared as what a
+    group of one shares."""
     g = torch.Generator(device=dev)
     g.manual_seed(ctx)
     c, _, _, start = tree(g, H, D, 16, dtype, unit, [ctx], n, [3 * s for s in range(n)], T)
@@ -138,17 +145,26 @@ def test_rows_do_not_depend_on_the_call(dev, D, H, G, dtype, unit, ctx, n, T, qd
     for t in range(T):
         one = c.attend(0, q[:, t:t + 1].contiguous(), i32([s + t for s in start]), most)
         assert torch.equal(one[:, 0], out[:, t]), t
+    shared = c.groups._host[1][0]
+    assert shared >= 64
     for s in range(n):
         d = c.desc()
         d.batch = 1
         d.block_table += 4 * s * c.n_layers * c.max_blocks
-        one = ops.shared_attention(d, 0, q[s:s + 1].contiguous(), i32(start[s:s + 1]), start[s] + T, unit)
+        one = ops.shared_attention(d, 0, q[s:s + 1].contiguous(), i32(start[s:s + 1]), start[s] + T, c.prefix_keys, c.unit_keys,
+                                   ops.PrefixGroups([0, 1], [shared], dev))
         assert torch.equal(one[0], out[s]), s
-    shared = c.groups._host[1][0]
-    for first, sh in (([0, 1, n], [shared] * n), ([1, n - 1], [0] + [shared - 1] * (n - 2) + [0]), ([0, n], [unit] * n),
-                      ([0, 2, n], [0, 0] + [shared] * (n - 2)), (list(range(n + 1)), [shared] * n)):
-        again = ops.shared_attention(c.desc(), 0, q, i32(start), most, unit, ops.PrefixGroups(first, sh, dev))
+    for first in ([0, 1, n], [0, n - 1, n], [0, 2, n], list(range(n + 1))):
+        again = attend(c, q, start, most, ops.PrefixGroups(first, [shared] * n, dev))
         assert torch.equal(again, out), first
+    # another division of the keys: other bits, and the same result whichever sequences have it
+    for first, sh in (([1, n - 1], [0] + [shared - 1] * (n - 2) + [0]), ([0, n], [40] * n), ([0, 2, n], [0, 0] + [shared] * (n - 2))):
+        again = attend(c, q, start, most, ops.PrefixGroups(first, sh, dev))
+        for s in range(n):
+            if sh[s] // 32 == shared // 32:
+                assert torch.equal(again[s], out[s]), (first, s)
+            if sh[s] == 0:
+                assert torch.equal(again[s], attend(c, q, start, most, None)[s]), (first, s)
 
 
 def test_many_rows_are_cut_into_launches(dev):
@@ -159,7 +175,8 @@ def test_many_rows_are_cut_into_launches(dev):
     c, _, _, start = tree(g, H, D, 16, BF16, unit, [4000], 3, [0, 40, 80], T)
     from draftkv._lib import lib
     import ctypes
-    assert lib().dkv_shared_attention_workspace(ctypes.byref(c.desc()), T, H * G, max(start) + T, unit) < 600 << 20
+    assert lib().dkv_shared_attention_workspace(ctypes.byref(c.desc()), ctypes.byref(c.groups.desc()), T, H * G, max(start) + T,
+                                                c.prefix_keys, c.unit_keys) < 600 << 20
     q = torch.randn(3, T, H * G, D, generator=g, device=dev)
     out = c.attend(0, q, i32(start), max(start) + T)
     for t in (0, 1, 100, 131, 200, 258):
@@ -223,17 +240,20 @@ def test_a_mask_that_leaves_nothing_of_a_unit(dev):
             assert ((out[s].to(F64) - want).abs() <= bound(want, size, top, D, unit, start[s] + 2, F32, BF16)).all(), (ctx, s)
 
 
-def test_a_bound_that_is_too_short_drops_units_only(dev):
+def test_a_bound_that_is_too_short_drops_pieces_only(dev):
+    """max_len below what sequences hold: their rows see the keys up to the end of the piece or unit that it lies in."""
     g = torch.Generator(device=dev)
     g.manual_seed(1)
     D, unit = 64, 64
-    for most, n in ((100, 128), (64, 64), (1, 64)):
-        c, ks, vs, start = tree(g, 2, D, 16, BF16, unit, [300], 3, [1, 2, 3], 1)
+    for groups, most, n in ((True, 100, 128), (True, 64, 64), (True, 1, 64), (True, 33, 64), (False, 100, 128), (False, 1, 32), (False, 33, 64), (True, 290, 320)):
+        c, ks, vs, start = tree(g, 2, D, 16, BF16, unit, [300], 3, [51, 52, 53], 1)      # 288 shared keys, then units of 32
+        assert c.groups.bounds() == (1, 3, 288, 288)
         q = torch.randn(3, 1, 4, D, generator=g, device=dev)
-        out = c.attend(0, q, i32(start), most)
+        out = attend(c, q, start, most, c.groups if groups else None)
         for s in range(3):
             want, size, top = attention(q[s], ks[s][:n], vs[s][:n], [n - 1])
-            assert ((out[s].to(F64) - want).abs() <= bound(want, size, top, D, unit, n, F32, BF16)).all(), (most, s)
+            tol = bound(want, size, top, D, unit, n, F32, BF16)
+            assert ((out[s].to(F64) - want).abs() <= tol).all(), (most, s)
 
 
 def test_layers_and_streams_and_out(dev):
@@ -254,8 +274,10 @@ def test_layers_and_streams_and_out(dev):
     c.fork(par)
     c.compact()
     again = c.attend(2, q[par].contiguous(), i32([start[p] for p in par]), 300)
-    assert torch.equal(again, ref[par])
-    for s, p in enumerate(par):
+    for s, p in enumerate(par):      # (other groups, so other pieces)
+        want, size, top = attention(q[p], ks[p], vs[p], [start[p], start[p] + 1])
+        for got in (again[s], ref[p]):
+            assert ((got.to(F64) - want).abs() <= bound(want, size, top, 64, 64, start[p] + 2, F32, BF16)).all(), s
         k, v, _ = c.read(2, s)
         assert np.array_equal(k, ks[p].float().cpu().numpy()) and np.array_equal(v, vs[p].float().cpu().numpy())
 
@@ -267,7 +289,7 @@ def test_far_pages_pass_32_bits(dev):
     g = torch.Generator(device=dev)
     g.manual_seed(3)
     from draftkv import SharedKVCache
-    c = SharedKVCache(1, H, D, bs, pages, BF16, max_tokens=1000, device=dev, chunk_keys=64)
+    c = SharedKVCache(1, H, D, bs, pages, BF16, max_tokens=1000, device=dev, unit_keys=64, prefix_keys=64)
     k, v = (torch.randn(1, 300, H, D, generator=g, device=dev).to(BF16) for _ in range(2))
     c.reserve([300])
     assert int(c.pages[0, 0]) == pages - 1
@@ -322,6 +344,7 @@ def test_a_recorded_step_follows_the_groups(dev):
 def test_attention_refuses(dev):
     c = new_cache(2, 2, 64, 16, 100, BF16, 32, 20)
     c.reserve([10, 10])
+    c.commit([10, 10])
     q = torch.randn(2, 1, 4, 64, device=dev)
     st = i32([9, 9])
     with pytest.raises(ValueError, match="does not match"):
@@ -347,7 +370,9 @@ def test_attention_refuses(dev):
     with pytest.raises(ValueError, match="max_len"):
         c.attend(0, q, st, 0)
     with pytest.raises(ValueError, match="groups of"):
-        ops.shared_attention(c.desc(), 0, q, st, 10, 32, ops.PrefixGroups([], [0], dev))
+        attend(c, q, [9, 9], 10, ops.PrefixGroups([], [0], dev))
+    with pytest.raises(ValueError, match="prefix_keys"):
+        ops.shared_attention(c.desc(), 0, q, st, 10, 33, 32)
     assert c.attend(0, q[:, :0].contiguous(), st, 10).shape == (2, 0, 4, 64)
 
 
@@ -567,7 +592,7 @@ def test_samples(dev, name, temperature):
 def plain_tokens(m, prompt, new):
     """Greedy decoding over a shared cache of one sequence, token by token."""
     from draftkv import SharedKVCache
-    c = SharedKVCache(m.n_layers, m.n_kv_heads, m.d_head, 16, 20, batch=1, device="cuda", chunk_keys=128)
+    c = SharedKVCache(m.n_layers, m.n_kv_heads, m.d_head, 16, 20, batch=1, device="cuda", chunk_keys=2048)
     toks = list(prompt)
     lg = m.forward(toks, c, 0)[-1]
     for _ in range(new):

@@ -158,7 +158,7 @@ def test_refusals(host):
     with pytest.raises(ValueError, match="8 bits"):
         SharedKVCache(1, 1, 64, 16, 8, torch.float8_e4m3fn, device="cpu")
     with pytest.raises(ValueError, match="multiple of 32"):
-        SharedKVCache(1, 1, 64, 16, 8, device="cpu", chunk_keys=48)
+        SharedKVCache(1, 1, 64, 16, 8, device="cpu", unit_keys=48)
     with pytest.raises(ValueError, match="d_head"):
         SharedKVCache(1, 1, 129, 16, 8, device="cpu")
     with pytest.raises(ValueError, match="positive"):
@@ -194,7 +194,7 @@ def test_ops_refuse_cpu_tensors():
     with pytest.raises(ValueError, match="GPU tensor"):
         ops.paged_copy(x, torch.zeros(1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32))
     with pytest.raises(ValueError, match="GPU tensor"):
-        ops.shared_attention(_lib.Paged(), 0, x[None], torch.zeros(1, dtype=torch.int32), 4, 32)
+        ops.shared_attention(_lib.Paged(), 0, x[None], torch.zeros(1, dtype=torch.int32), 4, 32, 32)
 
 
 # ---------------------------------------------------------------- the C entries' checks, before any launch
@@ -241,12 +241,12 @@ def test_c_shared_attention_refuses():
     L = _lib.lib()
     cache = dict(pool=FAKE, block_table=FAKE, batch=2, n_layers=2, n_kv_heads=2, head_dim=64, block_size=16, max_blocks=8, dtype=1)
     groups = dict(first=FAKE, shared=FAKE, n_groups=1, max_members=2, min_shared=3, max_shared=3)
-    ok = dict(layer=0, q=FAKE, dt=0, T=1, hq=4, start=FAKE, count=None, max_len=128, unit=32, out=FAKE, w=FAKE, n=1 << 24)
+    ok = dict(layer=0, q=FAKE, dt=0, T=1, hq=4, start=FAKE, count=None, max_len=128, prefix=32, unit=32, out=FAKE, w=FAKE, n=1 << 24)
 
     def call(c={}, g={}, **kw):
         a = dict(ok, **kw)
         return L.dkv_shared_attention(C.byref(_lib.Paged(**dict(cache, **c))), C.byref(_lib.Groups(**dict(groups, **g))), a["layer"],
-                                      a["q"], a["dt"], a["T"], a["hq"], a["start"], a["count"], a["max_len"], a["unit"], a["out"],
+                                      a["q"], a["dt"], a["T"], a["hq"], a["start"], a["count"], a["max_len"], a["prefix"], a["unit"], a["out"],
                                       a["w"], a["n"], None)
 
     for c, g, kw, text in (
@@ -258,7 +258,7 @@ def test_c_shared_attention_refuses():
             ({}, dict(max_members=3), {}, "group bounds"), ({}, dict(first=None), {}, "NULL"), ({}, dict(shared=None), {}, "NULL"),
             ({}, {}, dict(layer=2), "layer"), ({}, {}, dict(layer=-1), "layer"), ({}, {}, dict(dt=2), "query dtype"),
             ({}, {}, dict(hq=3), "multiple"), ({}, {}, dict(hq=0), "multiple"), ({}, {}, dict(unit=48), "unit_keys"),
-            ({}, {}, dict(unit=0), "unit_keys"), ({}, {}, dict(max_len=0), "max_len"), ({}, {}, dict(T=-1), "rows"),
+            ({}, {}, dict(unit=0), "unit_keys"), ({}, {}, dict(prefix=40), "prefix_keys"), ({}, {}, dict(prefix=-32), "prefix_keys"), ({}, {}, dict(max_len=0), "max_len"), ({}, {}, dict(T=-1), "rows"),
             ({}, {}, dict(T=1 << 29), "rows"), ({}, {}, dict(q=None), "NULL"), ({}, {}, dict(out=None), "NULL"),
             ({}, {}, dict(start=None), "NULL")):
         refused(call(c, g, **kw), text)
