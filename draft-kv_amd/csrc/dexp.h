@@ -115,4 +115,28 @@ __device__ __forceinline__ double dexp(double y, const double* tab) {
     return v;
 }
 
+// The same for sums whose largest term is 1: out = exp(y) for y in -708 .. 0 (callers clamp). The multiple of ln2/256 comes
+// from the low bits of a sum with 1.5 * 2^52 (to nearest even, as rint), and 2^e goes into the exponent field: no
+// conversion, rounding or ldexp instruction, which run at a quarter of an addition's rate.
+template <int N>
+__device__ __forceinline__ void dexp_sum_n(const double* y, double* out, const double* tab) {
+    double r[N], t[N];
+    int n[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const double z = fma(y[k], 0x1.71547652b82fep+8, 0x1.8p+52);   // y * 256 / ln2
+        const double m = z - 0x1.8p+52;
+        r[k] = fma(-m, 0x1.cf79abc9e3b3ap-48, fma(-m, 0x1.62e42fefa0000p-9, y[k]));
+        n[k] = __double2loint(z);
+        t[k] = tab[n[k] & (EXP_TAB - 1)];
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const double q = fma(fma(0x1.5555555555555p-5, r[k], 0x1.5555555555555p-3), r[k], 0.5);   // 1/24, 1/6
+        const double p = fma(q, r[k] * r[k], r[k]);                                              // exp(r) - 1
+        const double v = fma(t[k], p, t[k]);
+        out[k] = __hiloint2double(__double2hiint(v) + ((n[k] & ~(EXP_TAB - 1)) << 12), __double2loint(v));
+    }
+}
+
 }  // namespace dkv

@@ -606,21 +606,23 @@ __global__ void __launch_bounds__(64 * SA_WAVES, 2) shared_attn_kernel(SharedArg
         const int32_t* btab = c.block_table + ((int64_t)s0 * c.n_layers + A.layer) * c.max_blocks;
         constexpr int ES = St::ESIZE;
         const int64_t block_bytes = paged_block_elems(c) * ES;
-        // block ids of the 16-key runs from run0 on, one per lane (the last run that is there for those past it)
+        // Where the 16-key runs from run0 on begin, one per lane (the last run that is there for those past it): byte
+        // offsets of the head's rows of K and of V^T in the pool. Worked out here once for 64 runs: in scalar registers at
+        // each load it was 140 instructions a step, as long as the step's products.
         const int last_run = (k.k_there - 1) / 16, first_run = k.k_begin / 16;
         int run0 = first_run;
-        auto load_ids = [&]() { return btab[min(run0 + lane, last_run) * 16 / bs]; };
-        int ids = load_ids();
-        // a run's rows of K and V of the head
-        auto run_k = [&](int run) -> const char* {
-            run = min(run, last_run);
-            const int32_t blk = __builtin_amdgcn_readlane(ids, run - run0);
-            return static_cast<const char*>(c.pool) + blk * block_bytes + ((int64_t)h * bs + run * 16 % bs) * DP * ES;
+        int64_t at_k, at_v;
+        auto load_ids = [&]() {
+            const int pos = min(run0 + lane, last_run) * 16;
+            const int64_t block = btab[pos / bs] * block_bytes;
+            at_k = block + ((int64_t)h * bs + pos % bs) * DP * ES;
+            at_v = block + (((int64_t)H + h) * bs * DP + pos % bs) * ES;
         };
-        auto run_v = [&](int run) -> const char* {
-            run = min(run, last_run);
-            const int32_t blk = __builtin_amdgcn_readlane(ids, run - run0);
-            return static_cast<const char*>(c.pool) + blk * block_bytes + (((int64_t)H + h) * bs * DP + run * 16 % bs) * ES;
+        load_ids();
+        auto base = [&](int64_t at, int run) -> const char* {   // run: uniform
+            const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)at, run - run0);
+            const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)at >> 32), run - run0);
+            return static_cast<const char*>(c.pool) + (int64_t)((uint64_t)hi << 32 | lo);
         };
         // byte offsets of the lane in a load: K rows, V^T rows
         const uint32_t klane = (uint32_t)((lane % 16) * DP * ES + lane / 16 * 16);
@@ -656,15 +658,15 @@ __global__ void __launch_bounds__(64 * SA_WAVES, 2) shared_attn_kernel(SharedArg
         w.clear();
         if (wide) {
             constexpr int S = St::STAGES, LPW = St::LOADS / SA_WAVES;
-            auto issue = [&](int i) {   // this wave's share of step i's loads: K of two runs, then V of two runs
-                const int run = first_run + 2 * i;
-                const uint32_t to = lds_offset(lds) + (i % S) * St::BYTES;
+            // this wave's share of step i's loads: K or V of one of its two runs
+            const bool is_v = wave >= 2;
+            const int64_t piece = is_v ? vpiece : 64;
+            const uint32_t off = is_v ? vlane : klane;
+            auto issue = [&](int i) {
+                const char* from = base(is_v ? at_v : at_k, first_run + 2 * i + (wave & 1));
+                const uint32_t to = lds_offset(lds) + (i % S) * St::BYTES + wave * LPW * 1024;
 #pragma unroll
-                for (int x = 0; x < LPW; ++x) {
-                    const int l = wave * LPW + x;   // LOADS / 4 = KPC: a wave's loads are all K or V, of one run
-                    if (wave < 2) dma_b128<false>(run_k(run + wave) + 64 * x, klane, to + l * 1024);
-                    else dma_b128<false>(run_v(run + wave - 2) + x * vpiece, vlane, to + l * 1024);
-                }
+                for (int x = 0; x < LPW; ++x) dma_b128<false>(from + x * piece, off, to + x * 1024);
             };
             static_assert(LPW == St::KPC && SA_WAVES == 4, "a wave loads K or V of one run");
 #pragma unroll
@@ -678,7 +680,7 @@ __global__ void __launch_bounds__(64 * SA_WAVES, 2) shared_attn_kernel(SharedArg
                 else if (later == 1) wait_loads_barrier<LPW>();
                 else wait_loads_barrier<0>();
                 if (i + S - 1 < nsteps) {
-                    if (first_run + 2 * (i + S - 1) - run0 >= WAVE) run0 += WAVE, ids = load_ids();
+                    if (first_run + 2 * (i + S - 1) - run0 >= WAVE) run0 += WAVE, load_ids();
                     issue(i + S - 1);
                 }
                 const int kb = k.k_begin + SA_STEP * i;
@@ -696,15 +698,17 @@ __global__ void __launch_bounds__(64 * SA_WAVES, 2) shared_attn_kernel(SharedArg
             const uint32_t to = lds_offset(st);
             auto issue_k = [&](int i) {
                 const int run = first_run + 2 * i;
-                if (run - run0 >= WAVE) run0 += WAVE, ids = load_ids();
+                if (run - run0 >= WAVE) run0 += WAVE, load_ids();
+                const char* from[2] = {base(at_k, run), base(at_k, run + 1)};
 #pragma unroll
-                for (int x = 0; x < 2 * St::KPC; ++x) dma_b128<false>(run_k(run + x / St::KPC) + 64 * (x % St::KPC), klane, to + x * 1024);
+                for (int x = 0; x < 2 * St::KPC; ++x) dma_b128<false>(from[x / St::KPC] + 64 * (x % St::KPC), klane, to + x * 1024);
             };
-            auto issue_v = [&](int i) {   // (after its K: the ids are there)
+            auto issue_v = [&](int i) {   // (after its K: the offsets are there)
                 const int run = first_run + 2 * i;
+                const char* from[2] = {base(at_v, run), base(at_v, run + 1)};
 #pragma unroll
                 for (int x = 0; x < 2 * St::VPC; ++x)
-                    dma_b128<false>(run_v(run + x / St::VPC) + (x % St::VPC) * vpiece, vlane, to + St::K_BYTES + x * 1024);
+                    dma_b128<false>(from[x / St::VPC] + (x % St::VPC) * vpiece, vlane, to + St::K_BYTES + x * 1024);
             };
             issue_k(0);
             issue_v(0);

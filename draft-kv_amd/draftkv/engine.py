@@ -243,8 +243,8 @@ class DraftKVEngine:
         """Beam search over the full cache: per prompt, up to n_beams ``BeamHypothesis``, best score first. A beam ends with
         the token ``eos`` (None: none does); a prompt is done when n_beams have ended and no living beam's score, at its
         present length, is above the worst of them."""
-        if not 1 <= n_beams <= 64:
-            raise ValueError(f"n_beams must be 1..64, got {n_beams}")
+        if not 1 <= n_beams <= 32:
+            raise ValueError(f"n_beams must be 1..32, got {n_beams}")
         model, B = self.model, int(n_beams)
         prompts = self._check_prompts(prompts, model.vocab_size)
         P = len(prompts)

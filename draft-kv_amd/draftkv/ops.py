@@ -568,8 +568,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, k: int):
         raise ValueError(f"scores must be [{p}, {b}] on {logits.device}, got {tuple(scores.shape)} on {scores.device}")
     k = int(k)
     dt = _dt(logits)
-    if b < 1 or V < 1 or not 1 <= k <= 128 or b * k > 4096:
-        raise ValueError(f"beam_select: bad sizes (logits {tuple(logits.shape)}, k {k}: k is 1..128, beams * k at most 4096)")
+    if b < 1 or V < 1 or not 1 <= k <= 64 or b * k > 4096:
+        raise ValueError(f"beam_select: bad sizes (logits {tuple(logits.shape)}, k {k}: k is 1..64, beams * k at most 4096)")
     dev = logits.device
     out = torch.empty((p, k), dtype=torch.float64, device=dev)
     parents, tokens = (torch.empty((p, k), dtype=torch.int32, device=dev) for _ in range(2))

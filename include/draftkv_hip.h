@@ -403,7 +403,7 @@ int dkv_accept_noalloc(const float* target, const float* draft, const int32_t* d
  * apart), in the order (score, lowest beam, largest logit, lowest token).
  * Outputs [prompts][k]: the score, its beam and its token, best first; -infinity,
  * -1 and -1 where there are fewer. Tokens at -infinity, rows that hold NaN or
- * +infinity and beams at -infinity or NaN have none. k 1..128, beams * k up to
+ * +infinity and beams at -infinity or NaN have none. k 1..64, beams * k up to
  * 4096, vocab up to 1048576, prompts * beams up to 65535. A row's scores do not
  * depend on the other rows. work: dkv_beam_select_workspace() bytes, 8-byte
  * aligned. */

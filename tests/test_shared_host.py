@@ -225,7 +225,7 @@ def test_c_beam_select_refuses():
         return L.dkv_beam_select(a["x"], a["dt"], a["stride"], a["p"], a["b"], a["v"], a["s"], a["k"], a["o"], a["q"], a["t"],
                                  a["w"], a["n"], None)
 
-    for kw, text in ((dict(k=0), "k must"), (dict(k=129), "k must"), (dict(b=0), "beams"), (dict(b=64, k=65), "4096"),
+    for kw, text in ((dict(k=0), "k must"), (dict(k=65), "k must"), (dict(b=0), "beams"), (dict(b=65, k=64), "4096"),
                      (dict(v=0), "vocab"), (dict(v=1048577, stride=1 << 21), "vocab"), (dict(p=-1), "prompts"),
                      (dict(p=40000), "65535"), (dict(dt=3), "dtype"), (dict(stride=99), "row_stride"), (dict(x=None), "NULL"),
                      (dict(t=None), "NULL")):
@@ -276,7 +276,7 @@ def test_engine_refuses(monkeypatch):
     e = DraftKVEngine(Model())
     with pytest.raises(ValueError, match="n must"):
         e.generate_samples([[1]], 0, 4)
-    for n in (0, 65):
+    for n in (0, 33):
         with pytest.raises(ValueError, match="n_beams"):
             e.generate_beams([[1]], n, 4)
     with pytest.raises(IndexError):
