@@ -748,45 +748,71 @@ __global__ void __launch_bounds__(64 * SA_WAVES, 2) shared_attn_kernel(SharedArg
 
 // Merge of each row's pieces: their common maximum first, then the weighted
 // sums, pieces u, u + 4, ... in order and these four last, so the result depends
-// on the row's pieces alone. A wave per row and class.
+// on the row's pieces alone. Four waves per row, one class each; a lane weighs
+// the piece of its number and holds channels 2 lane and 2 lane + 1. Eight
+// pieces' loads are in flight at once.
 constexpr int SM_CLASSES = 4;
 template <bool QBF16>
 __global__ void __launch_bounds__(64 * SM_CLASSES) shared_merge_kernel(SharedArgs A) {
-    const int w = threadIdx.x / WAVE, lane = threadIdx.x % WAVE, D = A.c.head_dim;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), lane = threadIdx.x % WAVE, D = A.c.head_dim;
     int64_t i = blockIdx.x;
     const int hq = (int)(i % A.Hq);
     i /= A.Hq;
     const int t = A.t0 + (int)(i % A.Tn), s = (int)(i / A.Tn);
     const int last = min(A.start[s] + t, sa_len(A, s) - 1);
     int np;
-    const int n = sa_pieces(A, last, sa_shared(A, s), np);
+    const int n = __builtin_amdgcn_readfirstlane(sa_pieces(A, last, sa_shared(A, s), np));
     if (n <= 1) return;   // the attention kernel wrote the row
+    np = __builtin_amdgcn_readfirstlane(np);
     const int64_t prow = (int64_t)blockIdx.x * A.n_slots;
     auto slot = [&](int i) { return prow + (i < np ? i : A.units_p + i - np); };
     float m = -INFINITY;
     for (int u = lane; u < n; u += WAVE) m = fmaxf(m, A.ml[slot(u)].x);
     m = wave_max(m);
     const float ms = m == -INFINITY ? 0.0f : m;
-    const int c0 = min(lane, D - 1), c1 = min(lane + WAVE, D - 1);
+    const int c0 = min(2 * lane, D - 1), c1 = min(2 * lane + 1, D - 1);
+    const bool pair = D % 2 == 0;
     float l = 0.0f, o0 = 0.0f, o1 = 0.0f;
-    for (int u = w; u < n; u += SM_CLASSES) {
-        const float2 x = A.ml[slot(u)];
-        const float f = sa_exp2(x.x - ms);
-        l = fmaf(x.y, f, l);
-        o0 = fmaf(A.part[slot(u) * D + c0], f, o0);
-        o1 = fmaf(A.part[slot(u) * D + c1], f, o1);
-    }
-    __shared__ float sl[SM_CLASSES], so[SM_CLASSES][2][WAVE];
-    if (lane == 0) sl[w] = l;
-    so[w][0][lane] = o0, so[w][1][lane] = o1;
-    __syncthreads();
-    if (w > 1 || lane + WAVE * w >= D) return;
-    float lt = 0.0f, ot = 0.0f;
+    for (int u0 = 0; u0 < n; u0 += WAVE) {
+        float f = 0.0f;
+        if (u0 + lane < n) {
+            const float2 x = A.ml[slot(u0 + lane)];
+            f = sa_exp2(x.x - ms);
+            l = fmaf(x.y, f, l);
+        }
+        const int ue = min(n - u0, WAVE);
+        for (int u = w; u < ue; u += 8 * SM_CLASSES) {
+            float2 v[8];
 #pragma unroll
-    for (int k = 0; k < SM_CLASSES; ++k) lt += sl[k], ot += so[k][w][lane];
-    const int64_t at = (((int64_t)s * A.T + t) * A.Hq + hq) * D + lane + WAVE * w;
-    if constexpr (QBF16) static_cast<uint16_t*>(A.out)[at] = f32_to_bf16_rne(ot / lt);
-    else static_cast<float*>(A.out)[at] = ot / lt;
+            for (int k = 0; k < 8; ++k) {
+                const float* p = A.part + slot(u0 + min(u + k * SM_CLASSES, ue - 1)) * D;
+                v[k] = pair ? *reinterpret_cast<const float2*>(p + min(c0, D - 2)) : make_float2(p[c0], p[c1]);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (u + k * SM_CLASSES < ue) {
+                    const float g = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(f), u + k * SM_CLASSES));
+                    o0 = fmaf(v[k].x, g, o0);
+                    o1 = fmaf(v[k].y, g, o1);
+                }
+        }
+    }
+    __shared__ float2 so[SM_CLASSES][WAVE];
+    if (w > 0) so[w][lane] = make_float2(o0, o1);
+    __syncthreads();
+    if (w > 0) return;
+    const float lt = wave_sum(l);   // (every wave holds all of l)
+    if (2 * lane >= D) return;
+#pragma unroll
+    for (int k = 1; k < SM_CLASSES; ++k) o0 += so[k][lane].x, o1 += so[k][lane].y;
+    const int64_t at = (((int64_t)s * A.T + t) * A.Hq + hq) * D + 2 * lane;
+    if constexpr (QBF16) {
+        static_cast<uint16_t*>(A.out)[at] = f32_to_bf16_rne(o0 / lt);
+        if (2 * lane + 1 < D) static_cast<uint16_t*>(A.out)[at + 1] = f32_to_bf16_rne(o1 / lt);
+    } else {
+        static_cast<float*>(A.out)[at] = o0 / lt;
+        if (2 * lane + 1 < D) static_cast<float*>(A.out)[at + 1] = o1 / lt;
+    }
 }
 
 // Rows per launch: as many of the T as keep the partials within this

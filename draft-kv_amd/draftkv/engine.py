@@ -33,7 +33,7 @@ import torch
 from . import ops
 from .compress import CompressedKVCache
 from .paged import PagedKVCache, auto_chunk_keys
-from .shared import SharedKVCache, auto_prefix_keys
+from .shared import SharedKVCache
 from .graphs import DraftStepGraph, FullStepGraph, full_graph_key, graph_key
 from .config import CompressionConfig
 from .controller import Controller, FixedPolicy
@@ -204,7 +204,7 @@ class DraftKVEngine:
     # ------------------------------------------------- many continuations of one prompt
     def _new_shared(self, toks: list, n: int, own_rows: int, max_tokens: int, span: int) -> SharedKVCache:
         """The full cache of the prompts, with pages for n continuations of each that write up to own_rows rows of their
-        own. ``span`` fixes the attention's pieces, as ``_new_full`` does the chunk."""
+        own. ``span`` fixes the prompts' attention chunk, as in ``_new_full``."""
         m = self.model
         bs = 16
         if m.kv_dtype not in (torch.float32, torch.bfloat16):
@@ -213,8 +213,7 @@ class DraftKVEngine:
         pages = sum(-(-len(t) // bs) for t in toks) + len(toks) * n * (-(-own_rows // bs) + 2)
         return SharedKVCache(m.n_layers, m.n_kv_heads, m.d_head, bs, pages, m.kv_dtype, batch=len(toks),
                              max_tokens=max_tokens, device=m.device,
-                             chunk_keys=auto_chunk_keys(len(toks), m.n_kv_heads, span),
-                             prefix_keys=auto_prefix_keys(len(toks), m.n_kv_heads, span))
+                             chunk_keys=auto_chunk_keys(len(toks), m.n_kv_heads, span))
 
     def generate_samples(self, prompts: Sequence, n: int, max_new_tokens: int, temperature: float = 1.0,
                          context_key: Optional[str] = None) -> list:

@@ -59,13 +59,22 @@ class PagePool(BlockPool):
         assert set(np.flatnonzero(self.refs > 0).tolist()) == self._live, "holders of free blocks"
 
 
-def auto_prefix_keys(batch: int, n_heads: int, max_tokens: int) -> int:
-    """Keys per piece of what a prompt's continuations share, from the prompts at the cache's making: about 512 pieces (two
-    workgroups per CU) over them, a power of two in [128, 1024]."""
-    return int(min(1024, max(128, 1 << int(round(math.log2(max(1.0, batch * n_heads * max_tokens / 512.0)))))))
+def auto_prefix_keys(keys: int, members: int, per: int, least: int) -> int:
+    """Keys per piece of what groups share, a power of two in [least, 1024]; keys: those of all groups and heads, members:
+    sequences of the largest group, per: query heads per KV head. Up to two tiles of 32 rows (of one token each): 1024
+    (piece, tile) pairs, one for each SIMD; more, which a workgroup's four waves take together: 256 pieces, one for each
+    CU. The tokens of a call do not count: verify and decode must cut alike. Measured (us; pieces of 256, 512 and 1024
+    keys; 32 / 8 heads of 128, bf16): 32 sequences on 32k 97 / 74 / 74, five tokens each 378 / 292 / 250; 4 x 16 on 16k
+    124 / 110 / 93; 8 x 4 on 4k 36 / 39 / 59; pieces of 64, 128 and 256 keys: 4 on 500, 9 / 3 heads of 64, float32 16 / 20
+    / 28."""
+    tiles = -(-members * per // 32)
+    want = keys * tiles / 1024.0 if tiles <= 2 else keys / 256.0
+    return int(min(1024, max(least, 1 << int(round(math.log2(max(1.0, want)))))))
 
 
-UNIT_KEYS = 128   # keys per unit of a sequence's own
+# Keys per unit of a sequence's own, and the least of a piece: the steps of 32 of the float32 products take twice as long.
+# (us, units of 64 and 128: 16 x 3 rows on 900 keys, 12 heads of 64, float32 18 / 22; 32 on 8k unshared, bf16 240 / 210)
+UNIT_KEYS = {torch.float32: 64, torch.bfloat16: 128}
 
 
 class SharedKVCache(PagedKVCache):
@@ -73,8 +82,8 @@ class SharedKVCache(PagedKVCache):
 
     ``n_blocks`` is the pages of the one pool, each ``block_size`` tokens of all layers. ``batch`` is the number of
     sequences at first (the prompts); ``fork`` changes it. float32 or bfloat16. The attention sums what
-    a group shares in pieces of ``prefix_keys`` and the rest in units of ``unit_keys`` (multiples of 32): plain and drafted
-    decoding over caches with the same ones agree bit for bit. Prompts into an empty cache go through PagedKVCache's
+    a group shares in pieces of ``prefix_keys`` (by default chosen from the groups) and the rest in units of ``unit_keys``
+    (multiples of 32): plain and drafted decoding over caches whose sequences share the same agree bit for bit. Prompts into an empty cache go through PagedKVCache's
     attention, in chunks of ``chunk_keys``."""
 
     def __init__(self, n_layers: int, n_heads: int, d_head: int, block_size: int = 16, n_blocks: int = 512,
@@ -93,11 +102,12 @@ class SharedKVCache(PagedKVCache):
         self.device = torch.device(device) if device is not None else default_device()
         self.max_tokens = max_tokens if max_tokens is not None else n_blocks * block_size
         self.chunk_keys = chunk_keys if chunk_keys is not None else auto_chunk_keys(batch, n_heads, self.max_tokens)
-        self.prefix_keys = prefix_keys if prefix_keys is not None else auto_prefix_keys(batch, n_heads, self.max_tokens)
-        self.unit_keys = unit_keys if unit_keys is not None else UNIT_KEYS
+        self.prefix_keys = prefix_keys             # None: auto_prefix_keys
+        self.unit_keys = unit_keys if unit_keys is not None else UNIT_KEYS[self.dtype]
         for name in ("chunk_keys", "prefix_keys", "unit_keys"):
-            if getattr(self, name) < 32 or getattr(self, name) % 32:
-                raise ValueError(f"{name} must be a multiple of 32, got {getattr(self, name)}")
+            n = getattr(self, name)
+            if n is not None and (n < 32 or n % 32):
+                raise ValueError(f"{name} must be a multiple of 32, got {n}")
         self.max_blocks = -(-self.max_tokens // block_size)
         self.fp8 = False
         self.pools = [PagePool(n_blocks, block_size)]
@@ -109,6 +119,7 @@ class SharedKVCache(PagedKVCache):
         self.d_tables = torch.zeros((batch, n_layers, self.max_blocks), dtype=torch.int32, device=self.device)
         self.groups = ops.PrefixGroups([], [0] * batch, self.device)
         self._regroup = False                      # groups are to be worked out anew
+        self._shared_keys = 0                      # keys that groups share, of all groups and heads
 
     # ------------------------------------------------------------ pages
     def _set_pages(self, entries: list) -> None:
@@ -268,11 +279,16 @@ class SharedKVCache(PagedKVCache):
             rows = min(common * bs, int(self.n_tokens[x:y].min()))
             shared[x:y] = [rows] * (y - x)
         self.groups.update(cuts if any(shared) else [], shared)
+        self._shared_keys = self.n_heads * sum(shared[x] for x in cuts[:-1])
         self._regroup = False
 
     def graph_key(self) -> tuple:
         """What a recorded forward over this cache depends on beside its buffers' addresses."""
-        return (*self.groups.bounds(), self.prefix_keys, self.unit_keys)
+        return (*self.groups.bounds(), self._shared_keys, self.prefix_keys, self.unit_keys)
+
+    def _piece(self, q: torch.Tensor) -> int:
+        return self.prefix_keys or auto_prefix_keys(self._shared_keys, self.groups.max_members, q.shape[2] // self.n_heads or 1,
+                                                    UNIT_KEYS[self.dtype])
 
     # ------------------------------------------------------------ device ops
     def append_layer(self, layer: int, k: torch.Tensor, v: torch.Tensor, start: torch.Tensor,
@@ -290,8 +306,7 @@ class SharedKVCache(PagedKVCache):
         if q.dtype == torch.float32 and q.shape[1] > 1 and not self.n_tokens.any():
             # prompts: nothing is shared yet, and there are rows enough for the kernel whose workgroups walk the keys
             return ops.paged_attention(self.desc(), layer, q, start, max_len, self.chunk_keys, out, count)
-        return ops.shared_attention(self.desc(), layer, q, start, max_len, self.prefix_keys, self.unit_keys, self.groups, out,
-                                    count)
+        return ops.shared_attention(self.desc(), layer, q, start, max_len, self._piece(q), self.unit_keys, self.groups, out, count)
 
     # ------------------------------------------------------------ views
     def read(self, layer: int, seq: int = 0):
