@@ -122,21 +122,21 @@ class SharedKVCache(PagedKVCache):
         self._shared_keys = 0                      # keys that groups share, of all groups and heads
 
     # ------------------------------------------------------------ pages
-    def _set_pages(self, entries: list) -> None:
-        """Table entries (sequence, index, page) on the host and the device."""
-        if not entries:
+    def _set_pages(self, s: np.ndarray, i: np.ndarray, p: np.ndarray) -> None:
+        """Table entries (sequence, index) -> page on the host and the device."""
+        if len(s) == 0:
             return
-        s, i, p = np.array(entries, np.int64).T
+        s, i, p = (np.asarray(x, np.int64) for x in (s, i, p))
         self.pages[s, i] = p
         L = np.arange(self.n_layers)
         at = ((s[:, None] * self.n_layers + L) * self.max_blocks + i[:, None]).reshape(-1)
         ids = (p[:, None] * self.n_layers + L).reshape(-1).astype(np.int32)
         self.d_tables.view(-1).index_copy_(0, ops.to_device(at, self.device), ops.to_device(ids, self.device))
 
-    def _copy_pages(self, pairs: list) -> None:
-        if not pairs:
+    def _copy_pages(self, src, dst) -> None:
+        if len(src) == 0:
             return
-        ab = ops.to_device(np.array(pairs, np.int32).T, self.device)
+        ab = ops.to_device(np.array([src, dst], np.int32), self.device)
         ops.paged_copy(self.store.view(self.n_blocks, -1), ab[0], ab[1])
 
     def _own(self, lo: np.ndarray, hi: np.ndarray) -> None:
@@ -162,21 +162,23 @@ class SharedKVCache(PagedKVCache):
             return
         if need > pool.n_free:
             raise BlockPoolExhausted(f"{need} pages wanted, {pool.n_free} of {pool.n_blocks} free")
-        entries, pairs = [], []
+        s_, i_, p_, src, dst = [], [], [], [], []
         for s, i in shared:
             p = int(self.pages[s, i])
             if refs[p] > 1:                        # (the last holder keeps it)
                 q = pool.allocate()
                 pool.free(p)
-                pairs.append((p, q))
-                entries.append((s, i, q))
-        for s in np.flatnonzero(new):
-            n0, n = int(self.n_pages[s]), int(new[s])
-            entries += [(int(s), n0 + i, p) for i, p in enumerate(pool.allocate_many(n))]
-            self.n_pages[s] += n
-        self._copy_pages(pairs)
-        self._set_pages(entries)
-        self._regroup = self._regroup or bool(pairs)
+                src.append(p), dst.append(q)
+                s_.append(s), i_.append(i), p_.append(q)
+        grow = np.flatnonzero(new)
+        n = new[grow]
+        got = np.asarray(pool.allocate_many(int(n.sum())), np.int64)
+        index = np.arange(got.size) - np.repeat(np.cumsum(n) - n, n) + np.repeat(self.n_pages[grow], n)
+        self.n_pages[grow] += n
+        self._copy_pages(src, dst)
+        self._set_pages(np.concatenate([np.asarray(s_, np.int64), np.repeat(grow, n)]),
+                        np.concatenate([np.asarray(i_, np.int64), index]), np.concatenate([np.asarray(p_, np.int64), got]))
+        self._regroup = self._regroup or bool(src)
 
     def reserve(self, counts: Sequence[int]) -> None:
         """Pages for ``counts[s]`` more tokens of every layer, of the sequence's own: new ones, and a copy of its open page
@@ -244,12 +246,12 @@ class SharedKVCache(PagedKVCache):
             raise ValueError(f"compact(): {n} pages are live, {n_blocks} are too few")
         move = live[live >= n]
         holes = np.setdiff1d(np.arange(n), live)
-        self._copy_pages(list(zip(move.tolist(), holes.tolist())))
+        self._copy_pages(move, holes)
         to = np.arange(self.n_blocks, dtype=np.int32)
         to[move] = holes
         moved = np.isin(self.pages, move) & (self.pages >= 0)
         s, i = np.nonzero(moved)
-        self._set_pages(list(zip(s.tolist(), i.tolist(), to[self.pages[s, i]].tolist())))
+        self._set_pages(s, i, to[self.pages[s, i]])
         size = self.n_blocks if n_blocks is None else n_blocks
         refs = np.zeros(size, np.int64)
         refs[to[live]] = pool.refs[live]
