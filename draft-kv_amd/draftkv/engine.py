@@ -22,6 +22,7 @@ consumed, so the stream stays where the reference's would be.
 
 from __future__ import annotations
 
+import contextlib
 import time
 import warnings
 from dataclasses import dataclass, field
@@ -135,7 +136,8 @@ class DraftKVEngine:
         tk = np.zeros((len(prompts), T), np.int32)
         for s, p in enumerate(prompts):
             tk[s, : len(p) - 1] = p[:-1]
-        self.model.forward_batch(torch.as_tensor(tk).to(self.model.device), full, [0] * len(prompts), lens - 1)
+        with full.filling() if isinstance(full, SharedKVCache) else contextlib.nullcontext():
+            self.model.forward_batch(torch.as_tensor(tk).to(self.model.device), full, [0] * len(prompts), lens - 1)
 
     def _pending(self, toks) -> torch.Tensor:
         return ops.to_device(np.array([t[-1] for t in toks], np.int32), self.model.device)

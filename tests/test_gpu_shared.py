@@ -282,6 +282,32 @@ def test_layers_and_streams_and_out(dev):
         assert np.array_equal(k, ks[p].float().cpu().numpy()) and np.array_equal(v, vs[p].float().cpu().numpy())
 
 
+def test_prompts_take_the_unshared_kernel_inside_filling_alone(dev):
+    """Rows of prompts there are those of an ordinary cache bit for bit; outside, and once something is shared, a row is the
+    same in a call of one and of many."""
+    from draftkv import PagedKVCache
+    g = torch.Generator(device=dev)
+    g.manual_seed(8)
+    n, H, D = 70, 2, 64
+    q, k, v = (torch.randn(2, n, h, D, generator=g, device=dev) for h in (8, H, H))
+    c = new_cache(2, H, D, 16, 100, BF16, 32, 30)
+    c.reserve([n, n])
+    with c.filling():
+        out = c.append_attend(0, q, k, v, i32([0, 0]), n)
+    p = PagedKVCache(1, H, D, 16, 10, BF16, batch=2, device=dev, chunk_keys=c.chunk_keys)
+    p.reserve([n, n])
+    assert torch.equal(out, p.append_attend(0, q, k, v, i32([0, 0]), n))
+    out = c.attend(0, q, i32([0, 0]), n)
+    one = torch.cat([c.attend(0, q[:, t:t + 1].contiguous(), i32([t, t]), n) for t in range(n)], 1)
+    assert torch.equal(out, one)
+    c.commit([n, n])
+    c.fork([0, 0])
+    rows = lambda: c.attend(0, q[:, :3].contiguous(), i32([n - 3] * 2), n)
+    want = rows()
+    with c.filling():
+        assert torch.equal(rows(), want)
+
+
 def test_far_pages_pass_32_bits(dev):
     """Pages behind 2^31 elements of the store."""
     H, D, bs = 8, 128, 16
@@ -587,6 +613,15 @@ def test_samples(dev, name, temperature):
     whole = (len(PROMPTS[0]) - 1) // 16
     assert (full.pages[:, :whole] == full.pages[0, :whole]).all() and full.groups.max_shared >= 16 * whole
     assert [list(r.tokens) for r in e.generate_samples(PROMPTS[:1], 1, 8, 0.0)[0]] == [plain_tokens(m, PROMPTS[0], 8)]
+
+
+@pytest.mark.parametrize("name", ["llama", "tiny"])
+def test_samples_of_one_token_prompts(dev, name):
+    from draftkv import CompressionConfig, DraftKVEngine, FixedPolicy
+    m = _models()[name]()
+    runs = [DraftKVEngine(m, FixedPolicy(CompressionConfig(8, 0.9), gamma)).generate_samples([[7], [3, 4]], 3, 24, 0.0) for gamma in (0, 5)]
+    for p in range(2):
+        assert all(r.tokens == runs[0][p][0].tokens for x in runs for r in x[p])
 
 
 def plain_tokens(m, prompt, new):
