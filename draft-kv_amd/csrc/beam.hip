@@ -316,13 +316,13 @@ __global__ void __launch_bounds__(BEAM_THREADS, KM > 32 ? 3 : 6) beam_scan_kerne
     const int64_t at = (int64_t)row * A.segs + seg;
     uint64_t* out = A.lists + at * A.list;
     int n = 0;
-    for (int i = lane; i < have[w] || (i - lane < have[w]); i += WAVE) {
+    for (int i = lane; i - lane < have[w]; i += WAVE) {   // (whole waves)
         const uint64_t key = i < have[w] ? cand[w * CAP + i] : 0;
         const uint64_t in = __ballot((uint32_t)(key >> 32) >= floor && key != 0);
         if (in >> lane & 1) cand[w * CAP + n + __popcll(in & ((1ull << lane) - 1))] = key;   // (at or before where it was)
         n += __popcll(in);
     }
-    if (lane == 0) n_cand[w] = n;
+    if (lane == 0) n_cand[w] = n;   // (a wave still reading the lengths of the last tile uses its own alone)
     __syncthreads();
     int first = 0, total = 0;
 #pragma unroll

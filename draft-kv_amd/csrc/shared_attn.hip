@@ -43,6 +43,7 @@ typedef float sa_f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint16_t sa_u16x4u __attribute__((ext_vector_type(4), aligned(2)));
 
 constexpr int SA_ROWS = 32, SA_STEP = 32, SA_WAVES = 4;
+constexpr int SA_MOST_KEYS = 1 << 16;   // of a piece: a position and as many more stay within 32 bits
 
 struct SharedArgs {
     dkv_paged_t c;
@@ -856,11 +857,13 @@ static int sa_check(const dkv_paged_t& c, const dkv_groups_t& g, int T, int Hq, 
     DKV_REQUIRE(c.dtype == DKV_F32 || c.dtype == DKV_BF16, "dkv_shared_attention: bad cache dtype");
     DKV_REQUIRE(c.batch > 0 && c.n_layers > 0 && c.n_kv_heads > 0 && c.block_size > 0 && c.max_blocks > 0,
                 "dkv_shared_attention: bad cache shape");
-    DKV_REQUIRE((int64_t)c.max_blocks * c.block_size < (1LL << 31) - (1 << 16), "dkv_shared_attention: more than 2^31 positions");
+    DKV_REQUIRE((int64_t)c.max_blocks * c.block_size < (1LL << 31) - SA_MOST_KEYS, "dkv_shared_attention: more than 2^31 positions");
     DKV_REQUIRE(c.head_dim > 0 && c.head_dim <= 128, "dkv_shared_attention: head_dim must be 1..128");
     DKV_REQUIRE(Hq > 0 && Hq % c.n_kv_heads == 0, "dkv_shared_attention: query heads must be a multiple of KV heads");
-    DKV_REQUIRE(unit > 0 && unit % SA_STEP == 0, "dkv_shared_attention: unit_keys must be a multiple of 32");
-    DKV_REQUIRE(prefix > 0 && prefix % SA_STEP == 0, "dkv_shared_attention: prefix_keys must be a multiple of 32");
+    DKV_REQUIRE(unit > 0 && unit <= SA_MOST_KEYS && unit % SA_STEP == 0,
+                "dkv_shared_attention: unit_keys must be a multiple of 32, at most 65536");
+    DKV_REQUIRE(prefix > 0 && prefix <= SA_MOST_KEYS && prefix % SA_STEP == 0,
+                "dkv_shared_attention: prefix_keys must be a multiple of 32, at most 65536");
     DKV_REQUIRE(max_len > 0, "dkv_shared_attention: max_len must be > 0");
     DKV_REQUIRE(T >= 0 && (int64_t)c.batch * T * Hq < (1LL << 31), "dkv_shared_attention: too many rows");
     DKV_REQUIRE(g.n_groups >= 0 && g.n_groups <= c.batch, "dkv_shared_attention: n_groups must lie in 0..batch");

@@ -346,6 +346,8 @@ class PrefixGroups:
             raise ValueError("shared must not be negative, and 0 outside groups")
         if (first, shared) == self._host:
             return False
+        if self.device.type == "cuda" and _is_capturing():
+            raise RuntimeError("PrefixGroups: groups are not changed inside a recorded graph (it would replay the first change)")
         self._host = (first, shared)
         self.n_groups = max(len(first) - 1, 0)
         self.max_members = max((y - x for x, y in zip(first, first[1:])), default=0)
@@ -373,7 +375,7 @@ def shared_attention(desc: Paged, layer: int, q: torch.Tensor, start: torch.Tens
     """Causal attention of q [batch, T, Hq, D] (float32 or bfloat16; the result has its type) over a paged cache whose
     sequences share prefixes: what ``groups`` have in common is read once for all their rows. start, max_len and count
     as for ``paged_attention``. Shared keys (their number rounded down to 32) are summed in pieces of ``prefix_keys``, the
-    others in units of ``unit_keys`` (multiples of 32): a row's bits depend on its keys, on how many of them its group
+    others in units of ``unit_keys`` (multiples of 32, at most 65536): a row's bits depend on its keys, on how many of them its group
     shares and on these two, not on T or the other rows."""
     _need(q, "q", ndim=4)
     b, T, Hq, D = q.shape

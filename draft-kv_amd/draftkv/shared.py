@@ -107,8 +107,8 @@ class SharedKVCache(PagedKVCache):
         self.unit_keys = unit_keys if unit_keys is not None else UNIT_KEYS[self.dtype]
         for name in ("chunk_keys", "prefix_keys", "unit_keys"):
             n = getattr(self, name)
-            if n is not None and (n < 32 or n % 32):
-                raise ValueError(f"{name} must be a multiple of 32, got {n}")
+            if n is not None and (n < 32 or n % 32 or n > 65536):
+                raise ValueError(f"{name} must be a multiple of 32, at most 65536, got {n}")
         self.max_blocks = -(-self.max_tokens // block_size)
         self.fp8 = False
         self.pools = [PagePool(n_blocks, block_size)]
@@ -122,6 +122,10 @@ class SharedKVCache(PagedKVCache):
         self._regroup = False                      # groups are to be worked out anew
         self._filling = False
         self._shared_keys = 0                      # keys that groups share, of all groups and heads
+
+    def _not_recorded(self, why: str) -> None:
+        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(why)
 
     # ------------------------------------------------------------ pages
     def _set_pages(self, s: np.ndarray, i: np.ndarray, p: np.ndarray) -> None:
@@ -162,6 +166,7 @@ class SharedKVCache(PagedKVCache):
         need = int(new.sum()) + sum(min(n, int(refs[p]) - 1) for p, n in writers.items())
         if need == 0:
             return
+        self._not_recorded("reserve() before a forward is recorded: pages are taken on the host")
         if need > pool.n_free:
             raise BlockPoolExhausted(f"{need} pages wanted, {pool.n_free} of {pool.n_blocks} free")
         s_, i_, p_, src, dst = [], [], [], [], []
@@ -209,6 +214,7 @@ class SharedKVCache(PagedKVCache):
             raise ValueError(f"fork(): parents must be sequences 0..{self.batch - 1}, got {parents!r}")
         if par.size == self.batch and np.array_equal(par, np.arange(self.batch)):
             return
+        self._not_recorded("fork() cannot be recorded: pages change hands on the host")
         idx = ops.to_device(par, self.device)
         tables = self.d_tables.index_select(0, idx)
         if par.size == self.batch:
@@ -246,6 +252,7 @@ class SharedKVCache(PagedKVCache):
         n = live.size
         if n_blocks is not None and n_blocks < max(n, 1):
             raise ValueError(f"compact(): {n} pages are live, {n_blocks} are too few")
+        self._not_recorded("compact() cannot be recorded: pages change places on the host")
         move = live[live >= n]
         holes = np.setdiff1d(np.arange(n), live)
         self._copy_pages(move, holes)
@@ -271,8 +278,7 @@ class SharedKVCache(PagedKVCache):
         """The groups of sequences next to each other that come from one prompt, and the rows they all have in common."""
         if not self._regroup:
             return
-        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("reserve() before a forward is recorded: the groups of sequences changed")
+        self._not_recorded("reserve() before a forward is recorded: the groups of sequences changed")
         b, bs = self.batch, self.block_size
         shared = [0] * b
         cuts = [0, *(np.flatnonzero(np.diff(self.root)) + 1).tolist(), b]
@@ -288,7 +294,7 @@ class SharedKVCache(PagedKVCache):
 
     def graph_key(self) -> tuple:
         """What a recorded forward over this cache depends on beside its buffers' addresses."""
-        return (*self.groups.bounds(), self._shared_keys, self.prefix_keys, self.unit_keys)
+        return (self.groups.mem.data_ptr(), *self.groups.bounds(), self._shared_keys, self.prefix_keys, self.unit_keys)
 
     def _piece(self, q: torch.Tensor) -> int:
         return self.prefix_keys or auto_prefix_keys(self._shared_keys, self.groups.max_members, q.shape[2] // self.n_heads or 1,

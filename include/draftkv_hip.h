@@ -233,7 +233,7 @@ typedef struct {
  * probabilities in two; against a float32 cache the products are float32. The
  * shared keys, their number rounded down to 32, are cut into pieces of
  * prefix_keys, the others from there on into units of unit_keys (both
- * multiples of 32): a row's result depends on its keys, on how many of them
+ * multiples of 32, at most 65536): a row's result depends on its keys, on how many of them
  * its group shares and on these two, not on T, the other rows or the launch. A
  * row that sees no key is zero. head_dim 1..128, any block_size. max_len bounds
  * start + count of every sequence; of a longer one no key is seen past the

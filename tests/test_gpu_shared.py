@@ -367,6 +367,27 @@ def test_a_recorded_step_follows_the_groups(dev):
         assert torch.equal(got, ref), step
 
 
+def test_pages_do_not_change_hands_while_a_graph_is_recorded(dev):
+    c = new_cache(2, 2, 64, 16, 100, BF16, 32, 20)
+    c.reserve([20, 20])
+    c.commit([20, 20])
+    c.fork([0, 0])
+    g = ops.PrefixGroups([], [0, 0], dev)
+    x, at = torch.zeros(4, device=dev), i32([19, 19])
+    q = torch.zeros(2, 1, 4, 64, device=dev)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for call in (lambda: c.fork([1, 0]), lambda: c.compact(), lambda: c.reserve([9, 9]),
+                     lambda: g.update([0, 2], [16, 16]), lambda: c.attend(0, q, at, 20)):
+            with pytest.raises(RuntimeError, match="record"):
+                call()
+        x += 1
+    graph.replay()
+    c.reserve([9, 9])
+    assert g.update([0, 2], [16, 16]) and x.tolist() == [1.0] * 4 and c.groups.bounds() == (1, 2, 16, 16)
+
+
 def test_attention_refuses(dev):
     c = new_cache(2, 2, 64, 16, 100, BF16, 32, 20)
     c.reserve([10, 10])
@@ -495,7 +516,7 @@ def check_select(x, cum, k, dev, dtype=F32):
     # lse: each exp and sum within a few float64 roundings of a positive sum of V terms (chains of 32 + 12), the logarithm one ulp
     live = ws > -np.inf
     assert np.array_equal(s == -np.inf, ~live)
-    assert (np.abs(s[live] - ws[live]) <= 2.0 ** -53 * (100 + 8 * np.abs(ws[live]) + 8 * np.abs(x[np.isfinite(x)]).max())).all()
+    assert (np.abs(s[live] - ws[live]) <= 2.0 ** -53 * (100 + 8 * np.abs(ws[live]) + 8 * float(np.abs(x[np.isfinite(x)]).max()))).all()
     return s, b, v
 
 
@@ -612,6 +633,8 @@ def test_samples(dev, name, temperature):
     full.pools[0].check_invariants()
     whole = (len(PROMPTS[0]) - 1) // 16
     assert (full.pages[:, :whole] == full.pages[0, :whole]).all() and full.groups.max_shared >= 16 * whole
+    assert e.generate_samples([], 2, 5) == []
+    assert [[r.tokens for r in x] for x in e.generate_samples(PROMPTS, 2, 0, temperature)] == [[p, p] for p in PROMPTS]
     assert [list(r.tokens) for r in e.generate_samples(PROMPTS[:1], 1, 8, 0.0)[0]] == [plain_tokens(m, PROMPTS[0], 8)]
 
 

@@ -267,6 +267,28 @@ def test_c_shared_attention_refuses():
     assert call(T=0) == 0
 
 
+@needs_lib
+@pytest.mark.parametrize("keys", [65536 + 32, (1 << 31) - 32])
+def test_pieces_are_bounded(keys):
+    """A position and a piece's keys more stay within 32 bits: longer pieces are refused, by the cache and by the C entry."""
+    for name in ("prefix_keys", "unit_keys", "chunk_keys"):
+        with pytest.raises(ValueError, match="at most 65536"):
+            SharedKVCache(1, 1, 64, 16, 8, device="cpu", **{name: keys})
+    L = _lib.lib()
+    cache = _lib.Paged(pool=FAKE, block_table=FAKE, batch=1, n_layers=1, n_kv_heads=1, head_dim=64, block_size=16, max_blocks=8, dtype=1)
+    groups = _lib.Groups(first=FAKE, shared=FAKE, n_groups=1, max_members=1, min_shared=64, max_shared=64)
+    for prefix, unit, text in ((keys, 32, "prefix_keys"), (32, keys, "unit_keys")):
+        refused(L.dkv_shared_attention(C.byref(cache), C.byref(groups), 0, FAKE, 0, 1, 1, FAKE, None, 128, prefix, unit, FAKE, FAKE,
+                                       1 << 24, None), text)
+        assert L.dkv_shared_attention_workspace(C.byref(cache), C.byref(groups), 1, 1, 128, prefix, unit) == 0
+
+
+def test_a_recorded_step_belongs_to_its_groups():
+    """Two caches alike in every bound: what a graph was recorded with tells their groups' memory apart."""
+    made = [SharedKVCache(1, 1, 2, 4, 8, batch=2, device="cpu") for _ in range(2)]
+    assert made[0].graph_key()[1:] == made[1].graph_key()[1:] and made[0].graph_key() != made[1].graph_key()
+
+
 def test_engine_refuses(monkeypatch):
     from draftkv.engine import DraftKVEngine
 
