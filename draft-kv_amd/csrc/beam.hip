@@ -15,8 +15,13 @@
 //   2. select  one workgroup per prompt: each row's lse and k largest, a wave
 //              per row, then the k best of all rows (a rank is a binary
 //              search in every other row).
-// Bound: memory, the logits once; the exponentials (about 20 VALU
-// instructions per logit) run beside it.
+// Bound: 256 rows of 128256 take 51 us in all, 38 of them the scan: 131 MB of
+// float32 logits at 3.4 TB/s, and 50 us with bf16 logits, so it is the
+// float64 exponentials and the ranking (about 20 VALU instructions per logit),
+// not the bytes. 32 rows 18 us, four of 49152 16: two dependent launches of 7
+// and 7 (the select: one workgroup per prompt, a chain of loads, two ranks).
+// One instance for every k: a scan whose lists were sized for k up to 32 (twice
+// the workgroups per CU) took 52, 18.5 and 15.7.
 #include <algorithm>
 
 #include "dexp.h"
@@ -156,13 +161,14 @@ __device__ __forceinline__ uint32_t beam_nth(uint32_t v, int r) {
     return (uint32_t)__builtin_amdgcn_readlane((int)v, __ffsll((unsigned long long)__ballot(rank == r - 1)) - 1);
 }
 
-// KM: the most k this instance takes. What a logit must reach to be ranked: of the threads' largest, the ceil(k / 4)-th of
+// What a logit must reach to be ranked: of the threads' largest, the ceil(k / 4)-th of
 // each of the four waves, and of those the least (k logits are as large), or what an earlier tile of the segment asked for.
 // Rows of model logits pass little more than k per tile that way. Each wave lists its own; the lists are ranked when one is
 // half full, and at the end. A tile that overflows one (equal logits) takes the k-th of all threads' largest by value and
 // index, which at most k threads' logits pass.
-template <bool BF16, bool VEC, int KM>
-__global__ void __launch_bounds__(BEAM_THREADS, KM > 32 ? 3 : 6) beam_scan_kernel(BeamArgs A) {
+template <bool BF16, bool VEC>
+__global__ void __launch_bounds__(BEAM_THREADS, 3) beam_scan_kernel(BeamArgs A) {
+    constexpr int KM = BEAM_MAX_K;
     constexpr int NW = BEAM_THREADS / WAVE;
     constexpr int CAP = KM * BEAM_PER / NW + KM;    // a wave's list; all of them hold k threads' logits and the k best before
     __shared__ double tab[EXP_TAB];
@@ -498,18 +504,12 @@ extern "C" int dkv_beam_select(const void* logits, int32_t dtype, int64_t row_st
     a.out_score = out_scores, a.out_parent = out_parents, a.out_token = out_tokens;
     hipStream_t st = as_stream(stream);
     const bool bf = dtype == DKV_BF16;
+    // (256 rows of 128256 by vectors and by elements: float32 51 / 52 us, bf16 50 / 54; 32 rows 18 / 19.5)
     const bool vec = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && row_stride % 4 == 0 && vocab % 4 == 0;
     const dim3 grid(a.segs, (unsigned)rows);
-#define DKV_SCAN(BB, VV)                                                                                                    \
-    do {                                                                                                                    \
-        if (k <= 32) hipLaunchKernelGGL((beam_scan_kernel<BB, VV, 32>), grid, dim3(BEAM_THREADS), 0, st, a);                \
-        else hipLaunchKernelGGL((beam_scan_kernel<BB, VV, BEAM_MAX_K>), grid, dim3(BEAM_THREADS), 0, st, a);                \
-    } while (0)
-    if (bf && vec) DKV_SCAN(true, true);
-    else if (bf) DKV_SCAN(true, false);
-    else if (vec) DKV_SCAN(false, true);
-    else DKV_SCAN(false, false);
-#undef DKV_SCAN
+    const auto scan = bf ? (vec ? beam_scan_kernel<true, true> : beam_scan_kernel<true, false>)
+                         : (vec ? beam_scan_kernel<false, true> : beam_scan_kernel<false, false>);
+    hipLaunchKernelGGL(scan, grid, dim3(BEAM_THREADS), 0, st, a);
     if (const int e = check_launch("dkv_beam_select(scan)")) return e;
     const size_t lds = sizeof(double) * (2 * (size_t)beams * k + (size_t)(BEAM_SEL_THREADS / WAVE) * a.segs * a.list) +
                        sizeof(int) * beams;

@@ -3,8 +3,8 @@
 // nothing, draftkv/paged.py:76-176).
 //
 // dst page <- src page, byte for byte. Bound: memory, each byte read and
-// written once. A thread moves one vector: 160 pages of 2 MB 120 us (5.6 TB/s;
-// a contiguous copy of as many bytes 126), 24 of them 16.5, 6 of 720 KB 3.3.
+// written once. A thread moves one vector: 160 pages of 2 MB 112 us (6.0 TB/s;
+// a contiguous copy of as many bytes 126), 24 of them 15, 6 of 720 KB 3.3.
 // Four vectors per thread, a bound before each: 136, 25.7 and 17.4.
 #include "dkv_common.h"
 

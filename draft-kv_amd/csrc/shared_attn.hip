@@ -23,6 +23,25 @@
 //   bf16 cache, bf16 queries: queries whole, probabilities in two parts (2^-16
 //     of each, far below the rounding of the bf16 output)
 //   float32 cache: float32 matrix instructions
+//
+// Two roles (measured at the choice, dkv_shared_attention()). Where a unit's
+// rows are three tiles or more, the four waves of a workgroup take four tiles
+// and share its keys through a ring of four stages in LDS: K and V come from
+// L2 once for 128 rows. Otherwise each wave has a tile and a unit of its own and
+// one stage: many short units are in flight, which is what hides their latency.
+//
+// Bound (32 / 8 heads of 128, bf16 cache; under the profiler):
+//   many rows: the matrix cores. 32 sequences x 5 rows on 32.7k shared keys and
+//     100 of their own, float32 queries: 238 us, 258 GFLOP in parts at 1080
+//     TFLOP/s (a large library product 1164). One row each: 64 us; 256
+//     workgroups walk the shared keys, one per CU, and 128 the others beside
+//     them. Twice the workgroups with half the keys 62, and 8 instead of 6 in
+//     the merge.
+//   few rows: memory. 4 prompts of 16k x 16 sequences, bf16 queries: 82 us, 367
+//     MB at 4.5 TB/s (a large copy 4.83).
+//   small calls: the chain of loads before the first product and the steps of a
+//     unit. 4 sequences on 500 rows, 9 / 3 heads of 64, float32: 11 us and 5 for
+//     the merge.
 #include <algorithm>
 #include <type_traits>
 
@@ -913,6 +932,7 @@ extern "C" int dkv_shared_attention(const dkv_paged_t* cache, const dkv_groups_t
     const int step = sa_rows(c, T, n_q_heads, a.n_slots);
     hipStream_t st = as_stream(stream);
     const bool f32 = c.dtype == DKV_F32, qb = q_dtype == DKV_BF16;
+    // (by whole vectors through LDS, or element by element: 32 sequences on 16k 47 us and 527, 4 on 500 float32 17 and 39)
     const bool fast = c.block_size % 16 == 0 && c.head_dim % 32 == 0 && reinterpret_cast<uintptr_t>(c.pool) % 16 == 0;
     for (a.t0 = 0; a.t0 < T; a.t0 += step) {
         a.Tn = std::min(step, T - a.t0);
@@ -924,6 +944,8 @@ extern "C" int dkv_shared_attention(const dkv_paged_t* cache, const dkv_groups_t
         a.tiles_s = (int)((per + SA_ROWS - 1) / SA_ROWS);
         // (unit, head) pairs; a workgroup's four waves take four tiles of one (wide), or four tasks of a tile each
         const int64_t pairs_p = (int64_t)a.n_groups * c.n_kv_heads * a.units_p, pairs_s = (int64_t)c.batch * c.n_kv_heads * a.units_s;
+        // (us, wide and not; one row each on 16k shared keys, 32 / 8 heads of 128, bf16 cache: four groups of 8, 16, 24 and 32
+        // sequences, 1, 2, 3 and 4 tiles: 88 / 59, 112 / 84, 118 / 131, 134 / 142; 20 tiles on 32k 257 / 298)
         a.wide_p = fast && a.tiles_p >= 3, a.wide_s = fast && a.tiles_s >= 3;
         auto blocks_of = [](bool wide, int64_t pairs, int tiles, int64_t& tasks) {
             tasks = wide ? pairs : pairs * tiles;
