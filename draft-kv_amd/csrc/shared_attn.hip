@@ -32,7 +32,7 @@
 //
 // Bound (32 / 8 heads of 128, bf16 cache; under the profiler):
 //   many rows: the matrix cores. 32 sequences x 5 rows on 32.7k shared keys and
-//     100 of their own, float32 queries: 238 us, 258 GFLOP in parts at 1080
+//     100 of their own, float32 queries: 231 us, 258 GFLOP in parts at 1120
 //     TFLOP/s (a large library product 1164). One row each: 64 us; 256
 //     workgroups walk the shared keys, one per CU, and 128 the others beside
 //     them. Twice the workgroups with half the keys 62, and 8 instead of 6 in
