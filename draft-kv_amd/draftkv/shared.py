@@ -130,6 +130,10 @@ class SharedKVCache(PagedKVCache):
         if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
             raise RuntimeError(why)
 
+    def _put(self, a: np.ndarray) -> torch.Tensor:
+        with ops._device(self.store.device):
+            return ops.to_device(a, self.device)
+
     # ------------------------------------------------------------ pages
     def _set_pages(self, s: np.ndarray, i: np.ndarray, p: np.ndarray) -> None:
         """Table entries (sequence, index) -> page on the host and the device."""
@@ -140,12 +144,12 @@ class SharedKVCache(PagedKVCache):
         L = np.arange(self.n_layers)
         at = ((s[:, None] * self.n_layers + L) * self.max_blocks + i[:, None]).reshape(-1)
         ids = (p[:, None] * self.n_layers + L).reshape(-1).astype(np.int32)
-        self.d_tables.view(-1).index_copy_(0, ops.to_device(at, self.device), ops.to_device(ids, self.device))
+        self.d_tables.view(-1).index_copy_(0, self._put(at), self._put(ids))
 
     def _copy_pages(self, src, dst) -> None:
         if len(src) == 0:
             return
-        ab = ops.to_device(np.array([src, dst], np.int32), self.device)
+        ab = self._put(np.array([src, dst], np.int32))
         ops.paged_copy(self.store.view(self.n_blocks, -1), ab[0], ab[1])
 
     def _own(self, lo: np.ndarray, hi: np.ndarray) -> None:
@@ -218,7 +222,7 @@ class SharedKVCache(PagedKVCache):
         if par.size == self.batch and np.array_equal(par, np.arange(self.batch)):
             return
         self._not_recorded("fork() cannot be recorded: pages change hands on the host")
-        idx = ops.to_device(par, self.device)
+        idx = self._put(par)
         tables = self.d_tables.index_select(0, idx)
         if par.size == self.batch:
             self.d_tables.copy_(tables)            # (recorded graphs hold its address)
