@@ -17,8 +17,8 @@
 //              search in every other row).
 // Bound: 256 rows of 128256 take 51 us in all, 38 of them the scan: 131 MB of
 // float32 logits at 3.4 TB/s, and 50 us with bf16 logits, so it is the
-// float64 exponentials and the ranking (about 20 VALU instructions per logit),
-// not the bytes. 32 rows 18 us, four of 49152 16: two dependent launches of 7
+// float64 exponentials and the ranking (30 VALU instructions per logit, the
+// VALU busy two thirds of the time), not the bytes. 32 rows 18 us, four of 49152 16: two dependent launches of 7
 // and 7 (the select: one workgroup per prompt, a chain of loads, two ranks).
 // One instance for every k: a scan whose lists were sized for k up to 32 (twice
 // the workgroups per CU) took 52, 18.5 and 15.7.
