@@ -786,28 +786,35 @@ __global__ void __launch_bounds__(64 * SM_CLASSES) shared_merge_kernel(SharedArg
     np = __builtin_amdgcn_readfirstlane(np);
     const int64_t prow = (int64_t)blockIdx.x * A.n_slots;
     auto slot = [&](int i) { return prow + (i < np ? i : A.units_p + i - np); };
-    float m = -INFINITY;
-    for (int u = lane; u < n; u += WAVE) m = fmaxf(m, A.ml[slot(u)].x);
-    m = wave_max(m);
-    const float ms = m == -INFINITY ? 0.0f : m;
     const int c0 = min(2 * lane, D - 1), c1 = min(2 * lane + 1, D - 1);
     const bool pair = D % 2 == 0;
+    float2 v[8];
+    auto fetch = [&](int u0, int u, int ue) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float* p = A.part + slot(u0 + min(u + k * SM_CLASSES, ue - 1)) * D;
+            v[k] = pair ? *reinterpret_cast<const float2*>(p + min(c0, D - 2)) : make_float2(p[c0], p[c1]);
+        }
+    };
+    // the first loads at once: the lanes' weights and the class's first eight pieces
+    const float2 x0 = A.ml[slot(min(lane, n - 1))];
+    fetch(0, w, min(n, WAVE));
+    float m = x0.x;
+    for (int u = lane + WAVE; u < n; u += WAVE) m = fmaxf(m, A.ml[slot(u)].x);
+    m = wave_max(m);
+    const float ms = m == -INFINITY ? 0.0f : m;
     float l = 0.0f, o0 = 0.0f, o1 = 0.0f;
     for (int u0 = 0; u0 < n; u0 += WAVE) {
         float f = 0.0f;
         if (u0 + lane < n) {
-            const float2 x = A.ml[slot(u0 + lane)];
+            float2 x = x0;
+            if (u0 > 0) x = A.ml[slot(u0 + lane)];
             f = sa_exp2(x.x - ms);
             l = fmaf(x.y, f, l);
         }
         const int ue = min(n - u0, WAVE);
         for (int u = w; u < ue; u += 8 * SM_CLASSES) {
-            float2 v[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float* p = A.part + slot(u0 + min(u + k * SM_CLASSES, ue - 1)) * D;
-                v[k] = pair ? *reinterpret_cast<const float2*>(p + min(c0, D - 2)) : make_float2(p[c0], p[c1]);
-            }
+            if (u0 > 0 || u > w) fetch(u0, u, ue);
 #pragma unroll
             for (int k = 0; k < 8; ++k)
                 if (u + k * SM_CLASSES < ue) {
