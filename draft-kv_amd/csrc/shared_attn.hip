@@ -32,15 +32,14 @@
 //
 // Bound (32 / 8 heads of 128, bf16 cache; under the profiler):
 //   many rows: the matrix cores. 32 sequences x 5 rows on 32.7k shared keys and
-//     100 of their own, float32 queries: 231 us, 258 GFLOP in parts at 1120
+//     100 of their own, float32 queries: 230 us, 258 GFLOP in parts at 1120
 //     TFLOP/s (a large library product 1164). One row each: 64 us; 256
 //     workgroups walk the shared keys, one per CU, and 128 the others beside
-//     them. Twice the workgroups with half the keys 62, and 8 instead of 6 in
-//     the merge.
-//   few rows: memory. 4 prompts of 16k x 16 sequences, bf16 queries: 82 us, 367
-//     MB at 4.5 TB/s (a large copy 4.83).
+//     them; 5 in the merge. Twice the workgroups with half the keys 62, and 7.
+//   few rows: memory. 4 prompts of 16k x 16 sequences, bf16 queries: 83 us, 367
+//     MB at 4.4 TB/s (a large copy 4.83).
 //   small calls: the chain of loads before the first product and the steps of a
-//     unit. 4 sequences on 500 rows, 9 / 3 heads of 64, float32: 11 us and 5 for
+//     unit. 4 sequences on 500 rows, 9 / 3 heads of 64, float32: 11 us and 4 for
 //     the merge.
 #include <algorithm>
 #include <type_traits>
@@ -770,7 +769,9 @@ __global__ void __launch_bounds__(64 * SA_WAVES, 2) shared_attn_kernel(SharedArg
 // sums, pieces u, u + 4, ... in order and these four last, so the result depends
 // on the row's pieces alone. Four waves per row, one class each; a lane weighs
 // the piece of its number and holds channels 2 lane and 2 lane + 1. Eight
-// pieces' loads are in flight at once.
+// pieces' loads are in flight at once, the first beside the weights'. Bound: a
+// chain of three loads where rows are few (4 us), else memory: 5120 rows of 32
+// pieces and one, 88 MB in 18 us.
 constexpr int SM_CLASSES = 4;
 template <bool QBF16>
 __global__ void __launch_bounds__(64 * SM_CLASSES) shared_merge_kernel(SharedArgs A) {
