@@ -45,6 +45,7 @@
 #include <type_traits>
 
 #include "dkv_common.h"
+#include "shared_plan.h"
 
 // (every instantiation rounds alike, whatever the compiler would fuse in it)
 #pragma clang fp contract(off)
@@ -60,8 +61,7 @@ typedef float sa_f32x16 __attribute__((ext_vector_type(16)));
 typedef float sa_f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint16_t sa_u16x4u __attribute__((ext_vector_type(4), aligned(2)));
 
-constexpr int SA_ROWS = 32, SA_STEP = 32, SA_WAVES = 4;
-constexpr int SA_MOST_KEYS = 1 << 16;   // of a piece: a position and as many more stay within 32 bits
+constexpr int SA_ROWS = 32, SA_WAVES = 4;
 
 struct SharedArgs {
     dkv_paged_t c;
@@ -173,14 +173,15 @@ struct SharedTask {
     int64_t orow, prow;      // rows of q and out, and of the partials
 };
 
-// tile, u, h, s0: the same in the wave. False: no such task.
+// tile, u, h, s0: the same in the wave. False: no such task. k_begin is -1 where the sequence has no such unit.
 __device__ __forceinline__ bool sa_task(const SharedArgs& A, bool prefix, int tile, int u, int h, int s0, int members, int B, SharedTask& k) {
     const dkv_paged_t& c = A.c;
     const int lane = threadIdx.x % WAVE, col = lane % 32;
     const int per = A.Tn * A.G, n_rows = members * per, r0 = tile * SA_ROWS;   // rows of one sequence, of all
     k.h = h, k.s0 = s0;
     k.slot = prefix ? u : A.units_p + u;
-    k.k_begin = prefix ? u * A.prefix : B + u * A.unit;
+    const int len = __builtin_amdgcn_readfirstlane(sa_len(A, s0));
+    k.k_begin = prefix ? u * A.prefix : sa_unit_begin(B, u, A.unit, len);
     k.rvalid = r0 + col < n_rows;
     const int r = min(r0 + col, n_rows - 1);
     const int s = s0 + r / per, t = A.t0 + r % per / A.G, hq = h * A.G + r % A.G;
@@ -198,7 +199,6 @@ __device__ __forceinline__ bool sa_task(const SharedArgs& A, bool prefix, int ti
     }
     k.w_last = __builtin_amdgcn_readfirstlane(w_last), k.w_all = __builtin_amdgcn_readfirstlane(w_all);
     k.row_last = k.live ? k.last : INT_MAX;
-    const int len = __builtin_amdgcn_readfirstlane(sa_len(A, s0));
     k.k_there = prefix ? min(B, k.k_begin + A.prefix) : min(len, k.k_begin + A.unit);
     return r0 < n_rows;
 }
@@ -577,6 +577,7 @@ __global__ void __launch_bounds__(64 * SA_WAVES, 2) shared_attn_kernel(SharedArg
     if (prefix && u * A.prefix >= B) return;
     SharedTask k;
     const bool mine = sa_task(A, prefix, tile, u, h, s0, members, B, k);
+    if (k.k_begin < 0) return;
     if (!mine && (!wide || (tile - wave) * SA_ROWS >= members * A.Tn * A.G)) return;
     if (k.k_begin == 0 && k.rvalid && !k.live)   // an empty sequence
         for (int d = half; d < c.head_dim; d += 2) Walk::put(A, k.orow * c.head_dim + d, 0.0f);
@@ -851,13 +852,8 @@ static size_t sa_row_bytes(const dkv_paged_t& c, int Hq, int n_slots) {   // of 
 static int sa_rows(const dkv_paged_t& c, int T, int Hq, int n_slots) {
     return (int)std::min<size_t>(T, std::max<size_t>(1, SA_WORK_BYTES / sa_row_bytes(c, Hq, n_slots)));
 }
-// Pieces that shared keys, and the others up to max_len, are cut into at most
 static void sa_units(const dkv_paged_t& c, const dkv_groups_t& g, int max_len, int prefix, int unit, int& units_p, int& units_s) {
-    const int64_t keys = std::min<int64_t>(max_len, (int64_t)c.max_blocks * c.block_size);
-    const int64_t most = g.n_groups ? std::min<int64_t>(g.max_shared / SA_STEP, (keys + SA_STEP - 1) / SA_STEP) * SA_STEP : 0;
-    const int64_t least = g.n_groups ? g.min_shared / SA_STEP * SA_STEP : 0;
-    units_p = (int)((most + prefix - 1) / prefix);
-    units_s = least < keys ? (int)((keys - least + unit - 1) / unit) : 0;
+    sa_units((int64_t)c.max_blocks * c.block_size, max_len, g.n_groups > 0, g.min_shared, g.max_shared, prefix, unit, units_p, units_s);
 }
 
 template <bool F32, bool QBF16, int DP, bool FAST>

@@ -1,0 +1,77 @@
+"""How the attention over shared pages cuts keys (csrc/shared_plan.h), compiled for the host: every begin that a task may form lies
+within 32 bits, and where it lies is what the definition says, for all that the entry accepts (no GPU)."""
+
+import os
+import shutil
+import subprocess
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+CSRC = os.path.join(ROOT, "draft-kv_amd", "csrc")
+
+PROGRAM = r"""
+#include <cstdio>
+#include <initializer_list>
+#include "shared_plan.h"
+int main() {
+    long long keys, max_len, groups, least, most, prefix, unit, B, held;
+    while (scanf("%lld %lld %lld %lld %lld %lld %lld %lld %lld", &keys, &max_len, &groups, &least, &most, &prefix, &unit, &B, &held) == 9) {
+        int p = 0, s = 0;
+        dkv::sa_units(keys, (int)max_len, groups != 0, (int)least, (int)most, (int)prefix, (int)unit, p, s);
+        printf("%d %d", p, s);
+        for (int u : {0, 1, s / 2, s - 2, s - 1}) printf(" %d %d", u, u < 0 ? 0 : dkv::sa_unit_begin((int)B, u, (int)unit, (int)held));
+        printf("\n");
+    }
+}
+"""
+
+MOST_POSITIONS = (1 << 31) - (1 << 16) - 1      # what the entry accepts
+
+
+@pytest.fixture(scope="module")
+def plan(tmp_path_factory):
+    cxx = shutil.which("g++")
+    if not cxx:
+        pytest.skip("needs g++")
+    d = tmp_path_factory.mktemp("plan")
+    (d / "plan.cpp").write_text(PROGRAM)
+    subprocess.run([cxx, "-std=c++17", "-O1", "-fwrapv", "-I", CSRC, str(d / "plan.cpp"), "-o", str(d / "plan")], check=True)
+
+    def run(rows):
+        text = "\n".join(" ".join(str(int(x)) for x in r) for r in rows)
+        out = subprocess.run([str(d / "plan")], input=text, check=True, capture_output=True, text=True).stdout
+        return [[int(x) for x in line.split()] for line in out.splitlines()]
+
+    return run
+
+
+def test_begins_stay_within_32_bits(plan):
+    """Units are counted from the least that any sequence shares, and begin behind what their own shares: a unit past the
+    sequence's keys has no begin (-1), and no other passes 2^31."""
+    rows = []
+    for keys in (MOST_POSITIONS, 16 * 134213631, 1 << 30, (1 << 30) + 4096, 5000, 1):
+        for unit in (32, 128, 65536):
+            for B in (0, 32, 4096, 131072, 1 << 29, 1 << 30, keys // 2 // 32 * 32, keys // 32 * 32):
+                for held in (keys, keys - 1, keys // 2, B + 1, B, 1, 0):
+                    if B <= keys and 0 <= held <= keys:
+                        for least in {0, min(B, 64), B}:
+                            rows.append((keys, keys, 1, least, B, 65536, unit, B, held))
+    assert len(rows) > 1000
+    past = 0
+    for r, got in zip(rows, plan(rows)):
+        keys, _, _, least, most, prefix, unit, B, held = r
+        units_p, units_s = got[:2]
+        assert units_p == -(-(most // 32 * 32) // prefix)
+        assert units_s == (-(-(keys - least // 32 * 32) // unit) if least // 32 * 32 < keys else 0)
+        assert units_p * prefix < 1 << 31 and max(units_s - 1, 0) * unit < 1 << 31
+        for u, begin in zip(got[2::2], got[3::2]):
+            if u < 0 or u >= max(units_s, 1):
+                continue
+            true = B + u * unit
+            if u > 0 and true >= held:
+                assert begin == -1, (r, u)
+                past += true >= 1 << 31
+            else:
+                assert begin == true and begin + unit < 1 << 31, (r, u)
+    assert past > 0
