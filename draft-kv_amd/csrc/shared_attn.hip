@@ -889,6 +889,8 @@ static int sa_check(const dkv_paged_t& c, const dkv_groups_t& g, int T, int Hq, 
                 "dkv_shared_attention: prefix_keys must be a multiple of 32, at most 65536");
     DKV_REQUIRE(max_len > 0, "dkv_shared_attention: max_len must be > 0");
     DKV_REQUIRE(T >= 0 && (int64_t)c.batch * T * Hq < (1LL << 31), "dkv_shared_attention: too many rows");
+    // (a padding row's position is formed before it is cut to the last one's)
+    DKV_REQUIRE((int64_t)c.max_blocks * c.block_size + T < (1LL << 31), "dkv_shared_attention: positions past 2^31 (the table's, and T more)");
     DKV_REQUIRE(g.n_groups >= 0 && g.n_groups <= c.batch, "dkv_shared_attention: n_groups must lie in 0..batch");
     DKV_REQUIRE(g.n_groups == 0 || (g.max_members > 0 && g.max_members <= c.batch && g.min_shared >= 0 &&
                                     g.min_shared <= g.max_shared),

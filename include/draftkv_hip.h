@@ -235,7 +235,8 @@ typedef struct {
  * prefix_keys, the others from there on into units of unit_keys (both
  * multiples of 32, at most 65536): a row's result depends on its keys, on how many of them
  * its group shares and on these two, not on T, the other rows or the launch. A
- * row that sees no key is zero. head_dim 1..128, any block_size. max_len bounds
+ * row that sees no key is zero. head_dim 1..128, any block_size; the table's
+ * positions (max_blocks * block_size) below 2^31 - 65536 and 2^31 - T. max_len bounds
  * start + count of every sequence; of a longer one no key is seen past the
  * piece or unit that max_len lies in. work:
  * dkv_shared_attention_workspace() bytes, 16-byte aligned; none (it may be

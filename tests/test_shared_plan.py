@@ -1,11 +1,14 @@
 """How the attention over shared pages cuts keys (csrc/shared_plan.h), compiled for the host: every begin that a task may form lies
 within 32 bits, and where it lies is what the definition says, for all that the entry accepts (no GPU)."""
 
+import ctypes as C
 import os
 import shutil
 import subprocess
 
 import pytest
+
+from draftkv import _lib
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "draft-kv_amd", "csrc")
@@ -75,3 +78,20 @@ def test_begins_stay_within_32_bits(plan):
             else:
                 assert begin == true and begin + unit < 1 << 31, (r, u)
     assert past > 0
+
+
+@pytest.mark.skipif(not os.path.exists(_lib.LIB_PATH), reason="library not built")
+def test_padding_rows_stay_within_32_bits():
+    """start + t of a padding row, t up to T past the table's last position: calls in which it passes 2^31 are refused."""
+    L = _lib.lib()
+    fake = 4096      # an address that is never read
+    groups = _lib.Groups()
+    for blocks, T, fine in (((1 << 31) - (1 << 16) - 1, 70000, False), ((1 << 31) - 100000, 100000, False), ((1 << 31) - 100000, 99999, True),
+                            (1 << 20, 1 << 20, True)):
+        cache = _lib.Paged(pool=fake, block_table=fake, batch=1, n_layers=1, n_kv_heads=1, head_dim=64, block_size=1, max_blocks=blocks,
+                           dtype=1)
+        need = L.dkv_shared_attention_workspace(C.byref(cache), C.byref(groups), T, 1, 100, 32, 32)
+        assert (need > 0) == fine, (blocks, T)
+        if not fine:
+            rc = L.dkv_shared_attention(C.byref(cache), C.byref(groups), 0, fake, 0, T, 1, fake, fake, 100, 32, 32, fake, None, 0, None)
+            assert rc == -1 and b"2^31" in L.dkv_last_error()
