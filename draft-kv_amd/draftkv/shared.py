@@ -140,11 +140,11 @@ class SharedKVCache(PagedKVCache):
         if len(s) == 0:
             return
         s, i, p = (np.asarray(x, np.int64) for x in (s, i, p))
-        self.pages[s, i] = p
         L = np.arange(self.n_layers)
         at = ((s[:, None] * self.n_layers + L) * self.max_blocks + i[:, None]).reshape(-1)
         ids = (p[:, None] * self.n_layers + L).reshape(-1).astype(np.int32)
         self.d_tables.view(-1).index_copy_(0, self._put(at), self._put(ids))
+        self.pages[s, i] = p                       # (last: what comes before may find no memory)
 
     def _copy_pages(self, src, dst) -> None:
         if len(src) == 0:
@@ -253,31 +253,34 @@ class SharedKVCache(PagedKVCache):
 
     def compact(self, n_blocks: Optional[int] = None) -> int:
         """Move the live pages to the front of the pool, and with ``n_blocks`` make it that many pages long (more, or
-        fewer: at least the live ones). Returns the live pages."""
+        fewer: at least the live ones). Returns the live pages. Where memory is short it raises and changes nothing (the
+        old store and the new one are there at once)."""
         pool = self.pools[0]
         live = np.flatnonzero(pool.refs > 0)
         n = live.size
         if n_blocks is not None and n_blocks < max(n, 1):
             raise ValueError(f"compact(): {n} pages are live, {n_blocks} are too few")
         self._not_recorded("compact() cannot be recorded: pages change places on the host")
+        size = self.n_blocks if n_blocks is None else n_blocks
+        store = self.store
+        if size != self.n_blocks:
+            store = torch.empty((size * self.n_layers, store.shape[1]), dtype=self.dtype, device=self.device)
         move = live[live >= n]
         holes = np.setdiff1d(np.arange(n), live)
-        self._copy_pages(move, holes)
+        self._copy_pages(move, holes)              # (to pages that nobody holds)
+        if store is not self.store:
+            store[: n * self.n_layers].copy_(self.store[: n * self.n_layers])
         to = np.arange(self.n_blocks, dtype=np.int32)
         to[move] = holes
         moved = np.isin(self.pages, move) & (self.pages >= 0)
         s, i = np.nonzero(moved)
         self._set_pages(s, i, to[self.pages[s, i]])
-        size = self.n_blocks if n_blocks is None else n_blocks
         refs = np.zeros(size, np.int64)
         refs[to[live]] = pool.refs[live]
         pool.refs, pool.n_blocks = refs, size
         pool._live = set(range(n))
         pool._stack = list(range(size - 1, n - 1, -1))     # the lowest next
-        if size != self.n_blocks:
-            store = torch.empty((size * self.n_layers, self.store.shape[1]), dtype=self.dtype, device=self.device)
-            store[: n * self.n_layers].copy_(self.store[: n * self.n_layers])
-            self.store, self.n_blocks = store, size
+        self.store, self.n_blocks = store, size
         return n
 
     # ------------------------------------------------------------ groups

@@ -1,0 +1,70 @@
+"""Calls of the shared cache that fail, or whose leftovers a later call might meet, on the host (no GPU)."""
+
+import numpy as np
+import pytest
+import torch
+
+from draftkv import ops
+from draftkv.shared import SharedKVCache
+
+
+@pytest.fixture
+def host(monkeypatch):
+    """Page copies by indexing, so that a cache works on the CPU (all but its kernels)."""
+    def copy(store, src, dst):
+        store[dst.long()] = store[src.long()]
+        return store
+
+    monkeypatch.setattr(ops, "paged_copy", copy)
+
+
+def made(layers=2, bs=4, pages=8, rows=(6, 5, 9)):
+    """A cache of sequences with rows of their own, the second dropped: live pages with a hole before them."""
+    c = SharedKVCache(layers, 1, 2, bs, pages, batch=len(rows), max_tokens=40, device="cpu")
+    c.reserve(rows)
+    c.commit(rows)
+    c.store.copy_(torch.arange(c.store.numel(), dtype=torch.float32).view(c.store.shape))
+    c.fork([0, 2])
+    return c
+
+
+def state(c):
+    return [c.batch, c.n_blocks, c.store.shape[0], c.pages.copy(), c.n_pages.copy(), c.n_tokens.copy(), c.d_tables.clone(),
+            list(c.pools[0]._stack), set(c.pools[0]._live), c.pools[0].refs.copy(), c.pools[0].n_blocks]
+
+
+def same(a, b):
+    return all(np.array_equal(x, y) if isinstance(x, np.ndarray) else torch.equal(x, y) if torch.is_tensor(x) else x == y
+               for x, y in zip(a, b))
+
+
+def works(c):
+    """Forks, grows and reads as a cache does whose parts agree; every page that it hands out is in the store."""
+    c.pools[0].check_invariants()
+    assert c.store.shape[0] == c.n_blocks * c.n_layers and c.pools[0].refs.size == c.n_blocks == c.pools[0].n_blocks
+    before = [c.read(1, s)[0] for s in range(c.batch)]
+    c.fork([1, 1, 0])
+    c.reserve([5, 0, 5])
+    c.commit([5, 0, 5])
+    assert c.pages.max() < c.n_blocks and int(c.d_tables.max()) < c.store.shape[0]
+    for s, p in enumerate([1, 1, 0]):
+        assert np.array_equal(c.read(1, s)[0][: len(before[p])], before[p])
+    c.pools[0].check_invariants()
+
+
+@pytest.mark.parametrize("pages", [40, 5, 6])
+def test_a_compaction_without_memory_changes_nothing(host, monkeypatch, pages):
+    c = made()
+    was = state(c)
+
+    def full(*a, **kw):
+        raise torch.OutOfMemoryError("no memory")
+
+    with monkeypatch.context() as m:
+        m.setattr(torch, "empty", full)
+        with pytest.raises(torch.OutOfMemoryError):
+            c.compact(pages)
+    assert same(state(c), was)
+    works(c)
+    assert c.compact(pages + 10) == c.blocks_in_use
+    works(c)
