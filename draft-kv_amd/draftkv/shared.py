@@ -274,7 +274,10 @@ class SharedKVCache(PagedKVCache):
         to[move] = holes
         moved = np.isin(self.pages, move) & (self.pages >= 0)
         s, i = np.nonzero(moved)
+        there = self._put(np.arange(self.max_blocks) < self.n_pages[:, None]) if size < self.n_blocks else None
         self._set_pages(s, i, to[self.pages[s, i]])
+        if there is not None:                      # (entries past a sequence's pages: ids that may lie behind the new store)
+            self.d_tables.mul_(there[:, None])
         refs = np.zeros(size, np.int64)
         refs[to[live]] = pool.refs[live]
         pool.refs, pool.n_blocks = refs, size

@@ -68,3 +68,20 @@ def test_a_compaction_without_memory_changes_nothing(host, monkeypatch, pages):
     works(c)
     assert c.compact(pages + 10) == c.blocks_in_use
     works(c)
+
+
+@pytest.mark.parametrize("pages", [None, 7, 9, 30])
+def test_tables_name_no_page_behind_a_pool_that_shrank(host, pages):
+    """Entries past a sequence's pages hold ids of pages that it gave back: none lies outside the store."""
+    c = made(pages=20, rows=(30, 30, 13))
+    c.truncate([9, 13])
+    assert int(c.d_tables.max()) > 9 * c.n_layers          # (of pages that were given back)
+    n = c.compact(pages)
+    assert n == c.blocks_in_use == 7
+    assert int(c.d_tables.min()) >= 0 and int(c.d_tables.max()) < c.store.shape[0]
+    for s in range(c.batch):
+        for L in range(c.n_layers):
+            assert c.d_tables[s, L, : c.n_pages[s]].tolist() == [int(p) * c.n_layers + L for p in c.pages[s, : c.n_pages[s]]]
+    if pages is not None and pages < 20:
+        c.compact(40)
+    works(c)
