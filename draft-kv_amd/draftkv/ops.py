@@ -348,10 +348,6 @@ class PrefixGroups:
             return False
         if self.device.type == "cuda" and _is_capturing():
             raise RuntimeError("PrefixGroups: groups are not changed inside a recorded graph (it would replay the first change)")
-        self._host = (first, shared)
-        self.n_groups = max(len(first) - 1, 0)
-        self.max_members = max((y - x for x, y in zip(first, first[1:])), default=0)
-        self.min_shared, self.max_shared = min(shared, default=0), max(shared, default=0)
         import numpy as np
         row = np.zeros(2 * b + 1, np.int32)
         row[:b] = shared
@@ -359,6 +355,10 @@ class PrefixGroups:
         if b:
             with _device(self.device):
                 self.mem.copy_(to_device(row, self.device))
+        self._host = (first, shared)               # (last: a copy that finds no memory leaves the groups as they were)
+        self.n_groups = max(len(first) - 1, 0)
+        self.max_members = max((y - x for x, y in zip(first, first[1:])), default=0)
+        self.min_shared, self.max_shared = min(shared, default=0), max(shared, default=0)
         return True
 
     def bounds(self) -> tuple:

@@ -41,6 +41,10 @@ class PagePool(BlockPool):
         self.refs[got] = 1
         return got
 
+    def next(self, n: int) -> list:
+        """The blocks that allocate_many(n) will hand out, 0 < n <= n_free."""
+        return self._stack[-n:][::-1]
+
     def free(self, block: int) -> None:
         if not 0 <= block < self.n_blocks or self.refs[block] == 0:
             raise RuntimeError(f"double free of block {block}")
@@ -154,7 +158,7 @@ class SharedKVCache(PagedKVCache):
 
     def _own(self, lo: np.ndarray, hi: np.ndarray) -> None:
         """Give every sequence s pages lo[s] .. hi[s] - 1 of its own: new ones past its last, copies of those that others
-        hold too. Raises before anything changes when the pool is short."""
+        hold too. Raises before anything changes when the pool, or memory, is short."""
         pool, refs, b = self.pools[0], self.pools[0].refs, self.batch
         write = hi > lo
         if int(hi[write].max(initial=0)) > self.max_blocks:
@@ -176,22 +180,24 @@ class SharedKVCache(PagedKVCache):
         self._not_recorded("reserve() before a forward is recorded: pages are taken on the host")
         if need > pool.n_free:
             raise BlockPoolExhausted(f"{need} pages wanted, {pool.n_free} of {pool.n_blocks} free")
-        s_, i_, p_, src, dst = [], [], [], [], []
+        s_, i_, src = [], [], []
+        left = {p: int(refs[p]) for p in writers}  # holders
         for s, i in shared:
             p = int(self.pages[s, i])
-            if refs[p] > 1:                        # (the last holder keeps it)
-                q = pool.allocate()
-                pool.free(p)
-                src.append(p), dst.append(q)
-                s_.append(s), i_.append(i), p_.append(q)
+            if left[p] > 1:                        # (the last holder keeps it)
+                left[p] -= 1
+                s_.append(s), i_.append(i), src.append(p)
+        got = np.asarray(pool.next(need), np.int64)   # copies first; they are taken once the device's work is queued
         grow = np.flatnonzero(new)
         n = new[grow]
-        got = np.asarray(pool.allocate_many(int(n.sum())), np.int64)
-        index = np.arange(got.size) - np.repeat(np.cumsum(n) - n, n) + np.repeat(self.n_pages[grow], n)
-        self.n_pages[grow] += n
-        self._copy_pages(src, dst)
+        index = np.arange(int(n.sum())) - np.repeat(np.cumsum(n) - n, n) + np.repeat(self.n_pages[grow], n)
+        self._copy_pages(src, got[: len(src)])
         self._set_pages(np.concatenate([np.asarray(s_, np.int64), np.repeat(grow, n)]),
-                        np.concatenate([np.asarray(i_, np.int64), index]), np.concatenate([np.asarray(p_, np.int64), got]))
+                        np.concatenate([np.asarray(i_, np.int64), index]), got)
+        pool.allocate_many(need)
+        for p in src:
+            pool.free(p)
+        self.n_pages[grow] += n
         self._regroup = self._regroup or bool(src)
 
     def reserve(self, counts: Sequence[int]) -> None:
@@ -227,9 +233,8 @@ class SharedKVCache(PagedKVCache):
         if par.size == self.batch:
             self.d_tables.copy_(tables)            # (recorded graphs hold its address)
         else:
-            self.d_tables = tables
-            self.groups = ops.PrefixGroups([], [0] * par.size, self.device)
-            self.batch = par.size
+            self.groups = ops.PrefixGroups([], [0] * par.size, self.device)   # (where memory is short nothing has changed yet)
+            self.d_tables, self.batch = tables, par.size
         self.pages, self.n_pages = self.pages[par], self.n_pages[par]
         self.n_tokens, self.root = self.n_tokens[par], self.root[par]
         held = self.pages[self.pages >= 0]

@@ -85,3 +85,86 @@ def test_tables_name_no_page_behind_a_pool_that_shrank(host, pages):
     if pages is not None and pages < 20:
         c.compact(40)
     works(c)
+
+
+class Short:
+    """Uploads and new tensors that find no memory from the n-th on."""
+
+    def __init__(self, m, n):
+        self.left = n
+        for where, name in ((ops, "to_device"), (torch, "zeros"), (ops, "paged_copy")):
+            m.setattr(where, name, self.wrap(getattr(where, name)))
+
+    def wrap(self, f):
+        def call(*a, **kw):
+            self.left -= 1
+            if self.left < 0:
+                raise torch.OutOfMemoryError("no memory")
+            return f(*a, **kw)
+        return call
+
+
+@pytest.mark.parametrize("call", [lambda c: c.fork([1, 0, 1]), lambda c: c.fork([1, 0]), lambda c: c.fork([1, 1]), lambda c: c.reserve([3, 9]),
+                                  lambda c: c.compact(5), lambda c: c.compact(33), lambda c: c.compact()],
+                         ids=["fork to more", "fork the other way", "fork", "reserve", "compact to fewer", "compact to more", "compact"])
+@pytest.mark.parametrize("shared", [False, True])
+def test_no_memory_anywhere_in_a_call(host, monkeypatch, call, shared):
+    """Wherever memory runs out, the cache is what it was, or what the call makes of it; the call again does what it would have done."""
+    def fresh():
+        c = made(pages=30)
+        if shared:
+            c.fork([1, 1])
+        return c
+
+    want = fresh()
+    call(want)
+    for n in range(20):
+        c = fresh()
+        was = state(c)
+        rows = [c.read(1, s)[0] for s in range(c.batch)]
+        with monkeypatch.context() as m:
+            short = Short(m, n)
+            try:
+                call(c)
+            except torch.OutOfMemoryError:
+                failed = True
+            else:
+                failed = False
+                assert short.left >= 0 and same(state(c), state(want))
+                break
+        now = state(c)
+        c.pools[0].check_invariants()
+        held = np.bincount(c.pages[c.pages >= 0], minlength=c.n_blocks)
+        assert np.array_equal(held, c.pools[0].refs)
+        assert now[0] == was[0] and now[1:3] == was[1:3] and c.d_tables.shape[0] == c.groups.batch == c.batch
+        for s in range(c.batch):
+            assert np.array_equal(c.read(1, s)[0], rows[s])
+            assert c.d_tables[s, 1, : c.n_pages[s]].tolist() == [int(p) * c.n_layers + 1 for p in c.pages[s, : c.n_pages[s]]]
+        call(c)
+        for a, b in zip(state(c)[3:6], state(want)[3:6]):
+            assert np.array_equal(a, b)
+        c.reserve([0] * c.batch)
+        assert c.groups.mem.tolist() == [*c.groups._host[1], *c.groups._host[0],
+                                         *[0] * (c.batch + 1 - len(c.groups._host[0]))]
+        works_any(c)
+    assert n > 0 and not failed
+
+
+def works_any(c):
+    c.pools[0].check_invariants()
+    before = [c.read(0, s)[0] for s in range(c.batch)]
+    c.reserve([2] * c.batch)
+    c.commit([2] * c.batch)
+    for s in range(c.batch):
+        assert np.array_equal(c.read(0, s)[0][: len(before[s])], before[s])
+    c.pools[0].check_invariants()
+
+
+def test_groups_that_were_not_written_are_written_again(monkeypatch):
+    g = ops.PrefixGroups([0, 2], [3, 3], "cpu")
+    with monkeypatch.context() as m:
+        Short(m, 0)
+        with pytest.raises(torch.OutOfMemoryError):
+            g.update([0, 1, 2], [5, 7])
+    assert g.bounds() == (1, 2, 3, 3) and g.mem.tolist() == [3, 3, 0, 2, 0]
+    assert g.update([0, 1, 2], [5, 7]) and g.bounds() == (2, 1, 5, 7) and g.mem.tolist() == [5, 7, 0, 1, 2]
