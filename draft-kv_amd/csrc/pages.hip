@@ -7,10 +7,9 @@
 // a contiguous copy of as many bytes 126), 24 of them 15, 6 of 720 KB 3.3.
 // Four vectors per thread, a bound before each: 136, 25.7 and 17.4.
 #include "dkv_common.h"
+#include "pages.h"
 
 namespace dkv {
-
-constexpr int COPY_THREADS = 256;
 
 // Grid x: pair * pieces + piece. V is the widest type that the pages' size and
 // address allow. A pair with an id outside the store is skipped.
@@ -31,14 +30,15 @@ static int copy_pages(char* store, int64_t n_pages, int64_t page_bytes, const in
                       int64_t n_pairs, hipStream_t st) {
     const int64_t span = (int64_t)COPY_THREADS * sizeof(V);
     const int64_t pieces = (page_bytes + span - 1) / span;
-    DKV_REQUIRE(pieces < (1 << 24), "dkv_paged_copy: pages too large");
-    const int64_t most = (1 << 24) / pieces;   // pairs per launch
+    DKV_REQUIRE(pieces <= COPY_BLOCKS, "dkv_paged_copy: pages too large");
+    const int64_t most = COPY_BLOCKS / pieces;   // pairs per launch
     for (int64_t i = 0; i < n_pairs; i += most) {
         const int64_t n = n_pairs - i < most ? n_pairs - i : most;
         hipLaunchKernelGGL(paged_copy_kernel<V>, dim3((unsigned)(n * pieces)), dim3(COPY_THREADS), 0, st, store, n_pages, page_bytes,
                            src, dst, i, (int)pieces);
+        if (const int e = check_launch("dkv_paged_copy")) return e;
     }
-    return check_launch("dkv_paged_copy");
+    return DKV_OK;
 }
 
 }  // namespace dkv

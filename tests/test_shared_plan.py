@@ -16,8 +16,10 @@ CSRC = os.path.join(ROOT, "draft-kv_amd", "csrc")
 PROGRAM = r"""
 #include <cstdio>
 #include <initializer_list>
+#include "pages.h"
 #include "shared_plan.h"
-int main() {
+int main(int n, char**) {
+    if (n > 1) return printf("%lld %d\n", (long long)dkv::COPY_BLOCKS, dkv::COPY_THREADS), 0;
     long long keys, max_len, groups, least, most, prefix, unit, B, held;
     while (scanf("%lld %lld %lld %lld %lld %lld %lld %lld %lld", &keys, &max_len, &groups, &least, &most, &prefix, &unit, &B, &held) == 9) {
         int p = 0, s = 0;
@@ -42,6 +44,8 @@ def plan(tmp_path_factory):
     subprocess.run([cxx, "-std=c++17", "-O1", "-fwrapv", "-I", CSRC, str(d / "plan.cpp"), "-o", str(d / "plan")], check=True)
 
     def run(rows):
+        if rows is None:
+            return [int(x) for x in subprocess.run([str(d / "plan"), "copies"], check=True, capture_output=True, text=True).stdout.split()]
         text = "\n".join(" ".join(str(int(x)) for x in r) for r in rows)
         out = subprocess.run([str(d / "plan")], input=text, check=True, capture_output=True, text=True).stdout
         return [[int(x) for x in line.split()] for line in out.splitlines()]
@@ -78,6 +82,14 @@ def test_begins_stay_within_32_bits(plan):
             else:
                 assert begin == true and begin + unit < 1 << 31, (r, u)
     assert past > 0
+
+
+def test_launches_of_page_copies_stay_below_2_to_the_32_work_items(plan):
+    """The runtime refuses a launch of 2^32 work-items and more, which pages of any power of two would come to."""
+    blocks, threads = plan(None)
+    assert blocks * threads < 1 << 32
+    for pieces in (1, 2, 3, 512, 4096, 1 << 23, blocks):
+        assert 1 <= blocks // pieces * pieces <= blocks
 
 
 @pytest.mark.skipif(not os.path.exists(_lib.LIB_PATH), reason="library not built")
