@@ -62,6 +62,7 @@ typedef float sa_f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint16_t sa_u16x4u __attribute__((ext_vector_type(4), aligned(2)));
 
 constexpr int SA_ROWS = 32, SA_WAVES = 4;
+static_assert(SA_THREADS == 64 * SA_WAVES, "launches are cut by it");
 
 struct SharedArgs {
     dkv_paged_t c;
@@ -774,6 +775,7 @@ __global__ void __launch_bounds__(64 * SA_WAVES, 2) shared_attn_kernel(SharedArg
 // chain of three loads where rows are few (4 us), else memory: 5120 rows of 32
 // pieces and one, 88 MB in 18 us.
 constexpr int SM_CLASSES = 4;
+static_assert(SA_THREADS == 64 * SM_CLASSES, "launches are cut by it");
 template <bool QBF16>
 __global__ void __launch_bounds__(64 * SM_CLASSES) shared_merge_kernel(SharedArgs A) {
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), lane = threadIdx.x % WAVE, D = A.c.head_dim;
@@ -844,13 +846,14 @@ __global__ void __launch_bounds__(64 * SM_CLASSES) shared_merge_kernel(SharedArg
     }
 }
 
-// Rows per launch: as many of the T as keep the partials within this
+// Rows per launch: as many of the T as keep the partials within this, and the merge's workgroups within a launch
 constexpr size_t SA_WORK_BYTES = (size_t)512 << 20;
 static size_t sa_row_bytes(const dkv_paged_t& c, int Hq, int n_slots) {   // of one t
     return sizeof(float) * (size_t)c.batch * Hq * n_slots * (c.head_dim + 2);
 }
 static int sa_rows(const dkv_paged_t& c, int T, int Hq, int n_slots) {
-    return (int)std::min<size_t>(T, std::max<size_t>(1, SA_WORK_BYTES / sa_row_bytes(c, Hq, n_slots)));
+    const size_t most = std::min<size_t>(SA_WORK_BYTES / sa_row_bytes(c, Hq, n_slots), SA_BLOCKS / ((int64_t)c.batch * Hq));
+    return (int)std::min<size_t>(T, std::max<size_t>(1, most));
 }
 static void sa_units(const dkv_paged_t& c, const dkv_groups_t& g, int max_len, int prefix, int unit, int& units_p, int& units_s) {
     sa_units((int64_t)c.max_blocks * c.block_size, max_len, g.n_groups > 0, g.min_shared, g.max_shared, prefix, unit, units_p, units_s);
@@ -959,7 +962,7 @@ extern "C" int dkv_shared_attention(const dkv_paged_t* cache, const dkv_groups_t
         };
         a.blocks_p = blocks_of(a.wide_p, pairs_p, a.tiles_p, a.tasks_p);
         const int64_t blocks = a.blocks_p + blocks_of(a.wide_s, pairs_s, a.tiles_s, a.tasks_s);
-        DKV_REQUIRE(blocks < (1LL << 31), "dkv_shared_attention: grid too large");
+        DKV_REQUIRE(blocks <= SA_BLOCKS && (a.n_slots == 1 || rows <= SA_BLOCKS), "dkv_shared_attention: grid too large");
         const dim3 grid((unsigned)blocks);
         int e;
 #define DKV_SA(FF, QQ) e = fast ? sa_launch<FF, QQ, true>(a, grid, st) : sa_launch<FF, QQ, false>(a, grid, st)

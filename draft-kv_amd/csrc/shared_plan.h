@@ -7,6 +7,8 @@ namespace dkv {
 
 constexpr int SA_STEP = 32;
 constexpr int SA_MOST_KEYS = 1 << 16;   // of a piece or unit: a position and as many more stay within 32 bits
+constexpr int SA_THREADS = 256;
+constexpr int64_t SA_BLOCKS = ((int64_t)1 << 32) / SA_THREADS - 1;   // most workgroups of a launch: fewer than 2^32 work-items
 
 // Pieces that shared keys, and units that the others up to max_len, are cut into at most. Units are counted from the least
 // that any sequence shares; keys: the block table's positions.

@@ -107,3 +107,28 @@ def test_padding_rows_stay_within_32_bits():
         if not fine:
             rc = L.dkv_shared_attention(C.byref(cache), C.byref(groups), 0, fake, 0, T, 1, fake, fake, 100, 32, 32, fake, None, 0, None)
             assert rc == -1 and b"2^31" in L.dkv_last_error()
+
+
+@pytest.mark.skipif(not os.path.exists(_lib.LIB_PATH), reason="library not built")
+def test_attention_of_more_workgroups_than_a_launch_takes():
+    """Work-items of a launch stay below 2^32: rows are cut into launches, and where one row per sequence is too much the call is
+    refused before anything is launched."""
+    L = _lib.lib()
+    fake = 4096      # an address that is never read
+    groups = _lib.Groups()
+
+    def cache(**kw):
+        return _lib.Paged(**dict(dict(pool=fake, block_table=fake, batch=1, n_layers=1, n_kv_heads=1, head_dim=1, block_size=1, max_blocks=64,
+                                      dtype=1), **kw))
+
+    c = cache(batch=2, max_blocks=MOST_POSITIONS)      # 2^27 units, a wave each
+    need = L.dkv_shared_attention_workspace(C.byref(c), C.byref(groups), 1, 1, MOST_POSITIONS, 32, 32)
+    assert need >= 2 * 12 * 67106816
+    rc = L.dkv_shared_attention(C.byref(c), C.byref(groups), 0, fake, 0, 1, 1, fake, None, MOST_POSITIONS, 32, 32, fake, fake, need, None)
+    assert rc == -1 and b"grid too large" in L.dkv_last_error(), (rc, L.dkv_last_error())
+    # the merge takes a workgroup per row: 64 keys in two units, rows of a call by the workspace and by the launch
+    c = cache(batch=8)
+    for Hq, T in ((1, 1 << 22), (1 << 10, 1 << 12)):
+        need = L.dkv_shared_attention_workspace(C.byref(c), C.byref(groups), T, Hq, 64, 32, 32)
+        rows = (need - 8) // (4 * 2 * 3)
+        assert 0 < rows < 1 << 24 and rows % (8 * Hq) == 0, rows
