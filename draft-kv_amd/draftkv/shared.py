@@ -92,7 +92,7 @@ class SharedKVCache(PagedKVCache):
     sequences at first (the prompts); ``fork`` changes it. float32 or bfloat16. The attention sums what
     a group shares in pieces of ``prefix_keys`` (by default chosen from the groups) and the rest in units of ``unit_keys``
     (multiples of 32): plain and drafted decoding over caches whose sequences share the same agree bit for
-    bit. Inside ``filling()``, for prompts, it is PagedKVCache's attention, in chunks of ``chunk_keys``."""
+    bit. Inside ``filling()``, for prompts, that of float32 queries is PagedKVCache's, in chunks of ``chunk_keys``."""
 
     def __init__(self, n_layers: int, n_heads: int, d_head: int, block_size: int = 16, n_blocks: int = 512,
                  dtype=np.float32, *, batch: int = 1, max_tokens: Optional[int] = None, device=None,
@@ -328,8 +328,8 @@ class SharedKVCache(PagedKVCache):
 
     @contextlib.contextmanager
     def filling(self):
-        """The rows inside are those of prompts, before anything is shared: attention takes the kernel whose workgroups walk
-        the keys of many rows (4096 of a prompt, 32 / 8 heads of 128: 381 us; in units 1190)."""
+        """The rows inside are those of prompts, before anything is shared: attention of float32 queries takes the kernel
+        whose workgroups walk the keys of many rows (4096 of a prompt, 32 / 8 heads of 128: 381 us; in units 1190)."""
         self._filling = True
         try:
             yield self
@@ -342,7 +342,7 @@ class SharedKVCache(PagedKVCache):
         start[s] .., with what the sequences share read once."""
         self._here(q)
         self._sync_groups()
-        if self._filling and self.groups.n_groups == 0:
+        if self._filling and self.groups.n_groups == 0 and q.dtype == torch.float32:   # (that kernel takes no other)
             with ops._device(q.device):
                 return ops.paged_attention(self.desc(), layer, q, start, max_len, self.chunk_keys, out, count)
         return ops.shared_attention(self.desc(), layer, q, start, max_len, self._piece(q), self.unit_keys, self.groups, out, count)

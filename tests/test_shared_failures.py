@@ -168,3 +168,18 @@ def test_groups_that_were_not_written_are_written_again(monkeypatch):
             g.update([0, 1, 2], [5, 7])
     assert g.bounds() == (1, 2, 3, 3) and g.mem.tolist() == [3, 3, 0, 2, 0]
     assert g.update([0, 1, 2], [5, 7]) and g.bounds() == (2, 1, 5, 7) and g.mem.tolist() == [5, 7, 0, 1, 2]
+
+
+@pytest.mark.parametrize("dtype,name", [(torch.float32, "paged_attention"), (torch.bfloat16, "shared_attention")])
+def test_queries_of_prompts_go_to_a_kernel_that_takes_them(monkeypatch, dtype, name):
+    """The unshared kernel, which prompts take, has float32 queries alone."""
+    c = SharedKVCache(1, 1, 2, 4, 8, batch=1, device="cpu")
+    called = []
+    for f in ("paged_attention", "shared_attention"):
+        monkeypatch.setattr(ops, f, lambda *a, f=f: called.append(f))
+    q, start = torch.zeros(1, 3, 1, 2, dtype=dtype), torch.zeros(1, dtype=torch.int32)
+    with c.filling():
+        c.attend(0, q, start, 3)
+    assert called == [name]
+    c.attend(0, q, start, 3)
+    assert called == [name, "shared_attention"]
