@@ -313,3 +313,42 @@ def test_beams_of_long_prompts(dev, name, B, new, eos, penalty):
             compared += 1
             assert [h.tokens for h in got[p]] == [t for _, t in want]
     assert compared > 0 or (B, new) == (3, 40)
+
+
+# ---------------------------------------------------------------- beam selection at its largest
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("P,B,V,k", [(1, 2, 1048576, 64), (1, 3, 1048573, 7), (20000, 3, 9, 3), (65535, 1, 5, 6), (2, 64, 8200, 64), (9, 7, 262145, 33)])
+def test_beam_select_at_its_bounds(dev, P, B, V, k, dtype):
+    from test_gpu_shared import check_select
+    rng = np.random.default_rng(V + k)
+    x = (rng.standard_normal((P, B, V), dtype=np.float32) * 2)
+    check_select(x, -5 * rng.random((P, B)), k, dev, dtype)
+
+
+@pytest.mark.parametrize("k", [2, 16, 64])
+def test_beam_select_of_long_rows_of_equal_logits(dev, k):
+    """Every tile of a row overflows its lists: steps, one value, two values, the last tile alone above."""
+    from test_gpu_shared import check_select
+    V = 300001
+    i = np.arange(V)
+    rows = [np.zeros(V), np.where(i % 3 == 1, 2.0, 1.0), (i // 4096).astype(np.float64), -(i // 20000).astype(np.float64), np.where(i >= V - 70, 1.0, 0.0),
+            np.where(i < 50, 1.0, 0.0)]
+    for a in rows:
+        check_select(np.stack([a, rows[1], a])[None], np.array([[0.0, -0.25, 0.0]]), k, dev)
+
+
+@pytest.mark.parametrize("name", ["llama", "tiny"])
+@pytest.mark.parametrize("gamma", [0, 5])
+def test_a_shared_cache_in_place_of_the_ordinary_one(dev, name, gamma):
+    """full_cache_factory may make it: drafted and plain decoding of unlike prompts are the same."""
+    from draftkv import CompressionConfig, DraftKVEngine, FixedPolicy, SharedKVCache
+    m = models()[name]()
+    P = prompts(9)
+    make = lambda: SharedKVCache(m.n_layers, m.n_kv_heads, m.d_head, 16, 40, m.kv_dtype, batch=2, max_tokens=300, device=m.device)
+    e = DraftKVEngine(m, FixedPolicy(CompressionConfig(4, 0.5), gamma), full_cache_factory=make)
+    want = e.generate_baseline_batch(P, 40)
+    got = e.generate_batch(P, 40)
+    assert [list(r.tokens) for r in got] == want
+    for p, t in zip(P, want):
+        lp = whole(m, t[:-1])[len(p) - 1:]
+        assert (lp[np.arange(40), t[len(p):]] >= lp.max(-1) - NEAR).all()
