@@ -69,18 +69,20 @@ def auto_prefix_keys(keys: int, members: int, per: int, least: int) -> int:
     sequences of the largest group, per: query heads per KV head. The tokens of a call do not count: verify and decode must
     cut alike. A wave walks a piece for 32 rows, so a call takes the longer of a piece and of the pieces' share of the 1024
     SIMDs, and beside it writes and reads a state per row and piece, 75 of which take as long as a key of the walk (150 of
-    a float32 cache's, whose products take twice as long): the least of max(P, keys tiles / 1024) + keys rows / 75 P.
+    a float32 cache's, whose products count as twice as long; at the rates of large products they take 2.6 times): the least
+    of max(P, keys tiles / 1024) + keys rows / 75 P.
     Measured (us; pieces of 128, 256, 512, 1024 and 2048 keys; one token each, 32 / 8 heads of 128, bf16): 8 sequences on
     8k 23 / 27 / 37, on 16k 35 / 29 / 37; 32 on 32k 123 / 85 / 72 / 68; 16 on 130k 310 / 220 / 170 / 151 / 147; 8 x 4 on 4k
     43 / 36 / 40; five tokens, 32 on 4k 83 / 65 / 64 / 68; pieces of 64, 128 and 256: 4 on 500, 9 / 3 heads of 64, float32
     16 / 20 / 28. Of 56 such calls of one token its choice takes 1 % longer than the best power of two (23 % at most),
-    of 18 with five tokens 8 % (20 %)."""
+    of 18 with five tokens 8 % (20 %). It does not count how many workgroups a CU holds (one of a float32 cache with heads
+    of 128, two of a bf16 one), and was not fitted to the former."""
     tiles = -(-members * per // 32)
     want = max(keys * tiles / 1024, math.sqrt(keys * members * per * least / (75 * 128)), 1)
     return int(min(2048, max(least, 1 << round(math.log2(want)))))
 
 
-# Keys per unit of a sequence's own, and the least of a piece: the steps of 32 of the float32 products take twice as long.
+# Keys per unit of a sequence's own, and the least of a piece: a step of 32 takes longer with float32 products.
 # (us, units of 64 and 128: 16 x 3 rows on 900 keys, 12 heads of 64, float32 18 / 22; 32 on 8k unshared, bf16 240 / 210)
 UNIT_KEYS = {torch.float32: 64, torch.bfloat16: 128}
 
